@@ -1,0 +1,38 @@
+// Arguments of the windowed attention's launchers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+namespace wattn {
+
+// A bf16 tensor [batch, heads, seq, D] with a dense last dimension; strides in elements.
+struct Tensor {
+  const __nv_bfloat16* p;
+  long long b, h, s;
+  __host__ __device__ __nv_bfloat16* at(int batch, int head, long long pos) const { return const_cast<__nv_bfloat16*>(p) + batch * b + head * h + pos * s; }
+};
+
+struct Args {
+  Tensor q, k, v, out, dout, dq, dk, dv;
+  float* lse;          // [batch, heads, seq]: log2 of the sum of exp over a row's visible scores; rows that see nothing are not written
+  float* delta;        // [batch, heads, seq]: sum of dout * out over a row (backward)
+  const int* lengths;  // [batch] or nullptr
+  int B, H, KV, S, D;
+  int window, sinks;   // window >= 1 (S or more: everything)
+  float scale;
+
+  __host__ __device__ int group() const { return H / KV; }
+};
+
+__device__ __forceinline__ int lengthOf(const Args& a, int batch) {
+  const int n = a.lengths ? a.lengths[batch] : a.S;
+  return n < 0 ? 0 : n > a.S ? a.S : n;
+}
+// Key j is visible to query i of a sequence of L tokens.
+__device__ __forceinline__ bool visible(const Args& a, int i, int j) { return j <= i && (i - j < a.window || j < a.sinks); }
+
+}  // namespace wattn
+}  // namespace b200

@@ -15,7 +15,7 @@ MODULES = [
     "rocm_systems_b200.comm", "rocm_systems_b200.shmem",
     "rocm_systems_b200.parallel.dist", "rocm_systems_b200.parallel.fsdp", "rocm_systems_b200.parallel.tp", "rocm_systems_b200.parallel.ep",
     "rocm_systems_b200.parallel.pp", "rocm_systems_b200.parallel.cp",
-    "rocm_systems_b200.models.llama", "rocm_systems_b200.ops.train_ops", "rocm_systems_b200.ops.fp8",
+    "rocm_systems_b200.models.llama", "rocm_systems_b200.ops.train_ops", "rocm_systems_b200.ops.attention", "rocm_systems_b200.ops.fp8",
     "rocm_systems_b200.utils.checkpoint", "rocm_systems_b200.utils.elastic", "rocm_systems_b200.utils.markers", "rocm_systems_b200.utils.profiler",
     "rocm_systems_b200.utils.causal", "rocm_systems_b200.utils.affinity", "rocm_systems_b200.utils.hang_dump",
     "rocm_systems_b200.tools.smi", "rocm_systems_b200.tools.telemetry", "rocm_systems_b200.tools.tracedb", "rocm_systems_b200.tools.counters",
