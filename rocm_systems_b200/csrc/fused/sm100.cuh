@@ -74,6 +74,13 @@ __device__ __forceinline__ void tmaLoad2d(void* smemDst, const CUtensorMap* map,
                "l"(map), "r"(x), "r"(y), "r"(smemAddr(bar))
                : "memory");
 }
+// The same from a 4-D tensor: a box of one matrix of it.
+__device__ __forceinline__ void tmaLoad4d(void* smemDst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smemAddr(smemDst)), "l"(map), "r"(x),
+      "r"(y), "r"(z), "r"(w), "r"(smemAddr(bar))
+      : "memory");
+}
 __device__ __forceinline__ void tmaStore2d(const CUtensorMap* map, const void* smemSrc, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smemAddr(smemSrc)), "r"(x), "r"(y)
                : "memory");
@@ -124,6 +131,15 @@ __device__ __forceinline__ void mmaF16(uint32_t tmemD, uint64_t descA, uint64_t 
       "l"(descA), "l"(descB), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same with A in tensor memory: row = lane, two consecutive elements of the reduction per 32-bit column.
+__device__ __forceinline__ void mmaF16FromTmem(uint32_t tmemD, uint32_t tmemA, uint64_t descB, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmemD),
+      "r"(tmemA), "l"(descB), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void mmaF8(uint32_t tmemD, uint64_t descA, uint64_t descB, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -160,6 +176,16 @@ __device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+// 32 lanes x 16 consecutive 32-bit columns, the other way.
+__device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmemLoadWait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---- CTA pairs (cta_group::2) ---------------------------------------------------------------------------------

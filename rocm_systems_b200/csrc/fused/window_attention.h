@@ -17,6 +17,7 @@ struct Tensor {
 
 struct Args {
   Tensor q, k, v, out, dout, dq, dk, dv;
+  Tensor rest;         // what rounding took from out (bf16), kept for the backward pass, or nullptr
   float* lse;          // [batch, heads, seq]: log2 of the sum of exp over a row's visible scores; rows that see nothing are not written
   float* delta;        // [batch, heads, seq]: sum of dout * out over a row (backward)
   const int* lengths;  // [batch] or nullptr

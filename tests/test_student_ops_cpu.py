@@ -113,14 +113,14 @@ def test_c_entries_refuse_what_they_cannot_run():
     lib = attention._lib_attn()
     none = (ctypes.c_longlong * 24)()
     p = 4096  # an address that nothing reads: every call below is refused
-    fwd = lambda B=1, H=2, KV=1, S=4, D=64, w=0, si=0, q=p: lib.b200ops_window_attention_fwd(q, p, p, p, None, None, none, B, H, KV, S, D, w, si, 1.0, None)
+    fwd = lambda B=1, H=2, KV=1, S=4, D=64, w=0, si=0, q=p: lib.b200ops_window_attention_fwd(q, p, p, p, None, None, None, none, B, H, KV, S, D, w, si, 1.0, None)
     for bad in ({"B": 0}, {"H": 0}, {"KV": 0}, {"H": 3, "KV": 2}, {"S": 0}, {"D": 136}, {"D": 20}, {"D": 0}, {"w": -1}, {"si": -1}, {"q": p + 2}, {"q": None}):
         assert fwd(**bad) == invalid, bad
-    assert lib.b200ops_window_attention_fwd(p, p, p, p, None, None, none, 1, 2, 1, 4, 64, 0, 0, -1.0, None) == invalid
+    assert lib.b200ops_window_attention_fwd(p, p, p, p, None, None, None, none, 1, 2, 1, 4, 64, 0, 0, -1.0, None) == invalid
     odd = (ctypes.c_longlong * 24)(*([4] * 24))
-    assert lib.b200ops_window_attention_fwd(p, p, p, p, None, None, odd, 1, 2, 1, 4, 64, 0, 0, 1.0, None) == invalid
-    assert lib.b200ops_window_attention_bwd(p, p, p, p, p, None, p, p, p, p, None, none, 1, 2, 1, 4, 64, 0, 0, 1.0, None) == invalid
-    assert lib.b200ops_window_attention_bwd(p, p, p, p, p + 8, p, p, p, p, p, None, none, 1, 2, 1, 4, 64, 0, 0, 1.0, None) == invalid
+    assert lib.b200ops_window_attention_fwd(p, p, p, p, None, None, None, odd, 1, 2, 1, 4, 64, 0, 0, 1.0, None) == invalid
+    assert lib.b200ops_window_attention_bwd(p, p, p, p, p, p, None, p, p, p, p, None, none, 1, 2, 1, 4, 64, 0, 0, 1.0, None) == invalid
+    assert lib.b200ops_window_attention_bwd(p, p, p, p, p, p + 8, p, p, p, p, p, None, none, 1, 2, 1, 4, 64, 0, 0, 1.0, None) == invalid
     for seq, heads, kv, D in ((0, 4, 2, 64), (8, 0, 2, 64), (8, 4, 0, 64), (8, 4, 2, 12), (8, 4, 2, 512)):
         assert lib.b200ops_qk_norm_rope_fwd(p, p, p, 1, p, p, p, 8, seq, heads, kv, D, 1e-5, None) == invalid
         assert lib.b200ops_qk_norm_rope_bwd(p, p, p, none, p, p, p, 1, p, p, p, p, p, 8, seq, heads, kv, D, 1e-5, None) == invalid
