@@ -81,6 +81,12 @@ __device__ __forceinline__ void tmaLoad4d(void* smemDst, const CUtensorMap* map,
       "r"(y), "r"(z), "r"(w), "r"(smemAddr(bar))
       : "memory");
 }
+// `bytes` (a multiple of 16) from global to shared memory, both on 16-byte boundaries, counted on `bar`.
+__device__ __forceinline__ void bulkLoad(void* smemDst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smemAddr(smemDst)), "l"(src), "r"(bytes),
+               "r"(smemAddr(bar))
+               : "memory");
+}
 __device__ __forceinline__ void tmaStore2d(const CUtensorMap* map, const void* smemSrc, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smemAddr(smemSrc)), "r"(x), "r"(y)
                : "memory");

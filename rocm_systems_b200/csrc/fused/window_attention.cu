@@ -10,82 +10,20 @@
 namespace b200 {
 namespace wattn {
 
-constexpr int kThreads = 256;
-
-// One warp per row, four elements of the head per lane.
-__device__ __forceinline__ void load4(const __nv_bfloat16* row, int D, float (&f)[4]) {
-  const int lane = threadIdx.x & 31;
-  f[0] = f[1] = f[2] = f[3] = 0.f;
-  if (4 * lane < D) unpack4(*reinterpret_cast<const uint2*>(row + 4 * lane), f);
-}
-__device__ __forceinline__ void store4(__nv_bfloat16* row, int D, const float (&f)[4]) {
-  const int lane = threadIdx.x & 31;
-  if (4 * lane < D) *reinterpret_cast<uint2*>(row + 4 * lane) = pack4(f);
-}
-__device__ __forceinline__ float dot4(const float (&x)[4], const float (&y)[4]) { return laneSum<32>(x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3]); }
-
-// Next visible key from j on: the sinks, then the window.
-__device__ __forceinline__ int nextKey(const Args& a, int i, int j) { return visible(a, i, j) || j > i ? j : max(j, i - a.window + 1); }
-
-__global__ void __launch_bounds__(kThreads) queryGradRows(const Args a) {
-  const long long row = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (row >= (long long)a.B * a.H * a.S) return;
-  const int i = (int)(row % a.S), h = (int)(row / a.S % a.H), b = (int)(row / a.S / a.H), kh = h / a.group();
-  float acc[4] = {}, q[4], g[4], o[4];
-  if (i < lengthOf(a, b)) {
-    load4(a.q.at(b, h, i), a.D, q);
-    load4(a.dout.at(b, h, i), a.D, g);
-    load4(a.out.at(b, h, i), a.D, o);
-    float rest[4];
-    load4(a.rest.at(b, h, i), a.D, rest);
-    const float delta = dot4(g, o) + dot4(g, rest), lse = a.lse[row], c = a.scale * kLog2e;
-    if ((threadIdx.x & 31) == 0) a.delta[row] = delta;
-    for (int j = nextKey(a, i, 0); j <= i; j = nextKey(a, i, j + 1)) {
-      float k[4], v[4];
-      load4(a.k.at(b, kh, j), a.D, k);
-      load4(a.v.at(b, kh, j), a.D, v);
-      const float ds = exp2Fast(dot4(q, k) * c - lse) * (dot4(g, v) - delta) * a.scale;
-#pragma unroll
-      for (int e = 0; e < 4; e++) acc[e] += ds * k[e];
-    }
-  }
-  store4(a.dq.at(b, h, i), a.D, acc);
-}
-
-__global__ void __launch_bounds__(kThreads) keyGradRows(const Args a) {
-  const long long row = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (row >= (long long)a.B * a.KV * a.S) return;
-  const int j = (int)(row % a.S), kh = (int)(row / a.S % a.KV), b = (int)(row / a.S / a.KV), L = lengthOf(a, b);
-  float dk[4] = {}, dv[4] = {}, k[4], v[4];
-  if (j < L) {
-    load4(a.k.at(b, kh, j), a.D, k);
-    load4(a.v.at(b, kh, j), a.D, v);
-    const float c = a.scale * kLog2e;
-    const int last = j < a.sinks || a.window > L - j ? L : j + a.window;
-    for (int h = kh * a.group(); h < (kh + 1) * a.group(); h++)
-      for (int i = j; i < last; i++) {
-        float q[4], g[4];
-        load4(a.q.at(b, h, i), a.D, q);
-        load4(a.dout.at(b, h, i), a.D, g);
-        const size_t r = ((size_t)b * a.H + h) * a.S + i;
-        const float p = exp2Fast(dot4(q, k) * c - a.lse[r]), ds = p * (dot4(g, v) - a.delta[r]) * a.scale;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          dk[e] += ds * q[e];
-          dv[e] += p * g[e];
-        }
-      }
-  }
-  store4(a.dk.at(b, kh, j), a.D, dk);
-  store4(a.dv.at(b, kh, j), a.D, dv);
-}
-
 static bool good(const Args& a) {
   return a.B > 0 && a.H > 0 && a.KV > 0 && a.H % a.KV == 0 && a.S > 0 && a.D >= 8 && a.D <= 128 && a.D % 8 == 0 && a.window > 0 && a.sinks >= 0 && a.scale >= 0.f &&
          (long long)a.B * a.H * a.S <= 0x3fffffffffLL;
 }
 static Tensor packed(const void* p, const Args& a) { return {(const __nv_bfloat16*)p, (long long)a.S * a.H * a.D, a.D, (long long)a.H * a.D}; }
 static bool aligned(const Tensor& t) { return t.p && ((uintptr_t)t.p & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.s % 8 == 0; }
+
+// The device's context made current on this thread: encoding a tensor map asks for one, and a backward pass may be the first that its
+// thread does.
+static void bindContext() {
+  static thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
+}
 
 // Boxes of 128 positions x 64 elements of one head, 128-byte swizzle; what lies outside the tensor reads as zeros.
 static bool headMap(CUtensorMap* map, const Tensor& t, int B, int heads, int S, int D) {
@@ -111,6 +49,7 @@ template <typename K> static cudaError_t allowSmem(K kernel, size_t bytes, bool 
 
 template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
   static bool done[64] = {};
+  bindContext();
   FwdParams p{};
   p.a = a;
   p.c = fmaxf(a.scale * kLog2e, 1e-30f);  // times the scores' minus infinities it has to stay one
@@ -126,7 +65,46 @@ template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-static unsigned rowCtas(long long rows) { return (unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32)); }
+// How the sinks' far queries are split: every key tile that holds sinks and is not through with its window's queries.
+static void splitSinks(const Args& a, BwdParams& p) {
+  p.tiles = (a.S + kTile - 1) / kTile;
+  if (a.sinks == 0 || a.window >= a.S) return;
+  const int near = (kTile + a.window - 2) / kTile + 1;  // query tiles that see a key tile through the window
+  const int far = p.tiles - near;                       // of the first tile; the others have fewer
+  if (far <= 0) return;
+  p.sinkTiles = (a.sinks + kTile - 1) / kTile;
+  p.farChunk = near < 4 ? 4 : near;
+  p.farCount = (far + p.farChunk - 1) / p.farChunk;
+}
+static long long partialWords(const Args& a, const BwdParams& p) {
+  return (long long)a.B * a.KV * p.sinkTiles * (1 + p.farCount) * 2 * (a.sinks < kTile ? a.sinks : kTile) * a.D;
+}
+
+template <int HD> static cudaError_t backward(const Args& a, float* partials, cudaStream_t s) {
+  static bool doneQ[64] = {}, doneK[64] = {};
+  using C = BwdCfg<HD>;
+  bindContext();
+  BwdParams p{};
+  p.a = a;
+  p.c = fmaxf(a.scale * kLog2e, 1e-30f);
+  p.err = gemm::errWord();
+  if (!p.err) return cudaErrorMemoryAllocation;
+  splitSinks(a, p);
+  p.partials = partials;
+  const long long ctasQ = (long long)p.tiles * a.B * a.H, ctasK = (long long)(p.tiles + p.sinkTiles * p.farCount) * a.B * a.KV;
+  BwdParams k = p;
+  if (ctasQ > 0x7fffffffLL || ctasK > 0x7fffffffLL || a.B * (long long)a.KV > 65535 || !headMap(&p.x1, a.q, a.B, a.H, a.S, a.D) ||
+      !headMap(&p.x2, a.dout, a.B, a.H, a.S, a.D) || !headMap(&p.y1, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.y2, a.v, a.B, a.KV, a.S, a.D))
+    return cudaErrorInvalidValue;
+  k.x1 = p.y1, k.x2 = p.y2, k.y1 = p.x1, k.y2 = p.x2;
+  cudaError_t e = allowSmem(backwardKernel<HD, kQueries>, C::kSmem, doneQ);
+  if (e == cudaSuccess) e = allowSmem(backwardKernel<HD, kKeys>, C::kSmem, doneK);
+  if (e != cudaSuccess) return e;
+  backwardKernel<HD, kQueries><<<(unsigned)ctasQ, C::kThreads, C::kSmem, s>>>(p);
+  backwardKernel<HD, kKeys><<<(unsigned)ctasK, C::kThreads, C::kSmem, s>>>(k);
+  if (p.sinkTiles) joinSinks<<<dim3(a.sinks, a.B * a.KV), 128, 0, s>>>(k);
+  return cudaGetLastError();
+}
 
 }  // namespace wattn
 }  // namespace b200
@@ -136,7 +114,7 @@ using namespace b200::wattn;
 extern "C" {
 
 // q, out [B, H, S, D], k, v [B, KV, S, D] bf16, 16-byte aligned, with strides (batch, head, position) of q, k, v, out in turn (elements,
-// multiples of 8). lse (fp32 [B, H, S]) and rest (bf16 [B, S, H, D], what rounding took from out) are for the backward call, or nullptr. lengths: int32 [B] on the device, or nullptr. window 0: no window.
+// multiples of 8). lse (fp32 [B, H, S rounded up to 128]) and rest (bf16 [B, S, H, D], what rounding took from out) are for the backward call, or nullptr. lengths: int32 [B] on the device, or nullptr. window 0: no window.
 int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int* lengths, const long long* strides, int B, int H, int KV,
                                  int S, int D, int window, int sinks, float scale, cudaStream_t s) {
   const auto tensor = [&](const void* p, int i) { return Tensor{(const __nv_bfloat16*)p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
@@ -149,15 +127,16 @@ int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, vo
   a.lengths = lengths;
   a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
   a.window = window == 0 ? S : window;
-  a.sinks = sinks;
+  a.sinks = sinks < S ? sinks : S;
   a.scale = scale;
   a.rest = packed(rest, a);
   if (!good(a) || !aligned(a.q) || !aligned(a.k) || !aligned(a.v) || !aligned(a.out) || ((uintptr_t)rest & 15)) return (int)cudaErrorInvalidValue;
   return (int)(D <= 64 ? forward<64>(a, s) : forward<128>(a, s));
 }
 
-// strides: of q, k, v, out, dout, dq, dk, dv in turn. lse and rest as the forward call left them; delta: fp32 [B, H, S] scratch.
-int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* rest, const void* dout, const float* lse, float* delta, void* dq, void* dk,
+// strides: of q, k, v, out, dout, dq, dk, dv in turn. lse and rest as the forward call left them; scratch: as many fp32
+// words as b200ops_window_attention_bwd_scratch says.
+int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* rest, const void* dout, const float* lse, float* scratch, void* dq, void* dk,
                                  void* dv, const int* lengths, const long long* strides, int B, int H, int KV, int S, int D, int window, int sinks, float scale,
                                  cudaStream_t s) {
   const auto tensor = [&](const void* p, int i) { return Tensor{(const __nv_bfloat16*)p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
@@ -171,19 +150,29 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
   a.dk = tensor(dk, 6);
   a.dv = tensor(dv, 7);
   a.lse = const_cast<float*>(lse);
-  a.delta = delta;
+  a.delta = scratch;
   a.lengths = lengths;
   a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
   a.window = window == 0 ? S : window;
-  a.sinks = sinks;
+  a.sinks = sinks < S ? sinks : S;
   a.scale = scale;
   a.rest = packed(rest, a);
-  if (!good(a) || !lse || !delta || !rest || ((uintptr_t)rest & 15)) return (int)cudaErrorInvalidValue;
+  if (!good(a) || !lse || !scratch || !rest || (((uintptr_t)rest | (uintptr_t)lse | (uintptr_t)scratch) & 15)) return (int)cudaErrorInvalidValue;
   for (const Tensor* t : {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv})
     if (!aligned(*t)) return (int)cudaErrorInvalidValue;
-  queryGradRows<<<rowCtas((long long)B * H * S), kThreads, 0, s>>>(a);
-  keyGradRows<<<rowCtas((long long)B * KV * S), kThreads, 0, s>>>(a);
-  return (int)cudaGetLastError();
+  float* partials = scratch + (size_t)B * H * a.padded();
+  return (int)(D <= 64 ? backward<64>(a, partials, s) : backward<128>(a, partials, s));
+}
+
+long long b200ops_window_attention_bwd_scratch(int B, int H, int KV, int S, int D, int window, int sinks) {
+  Args a{};
+  a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
+  a.window = window == 0 ? S : window;
+  a.sinks = sinks < S ? sinks : S;
+  if (!good(a)) return -1;
+  BwdParams p{};
+  splitSinks(a, p);
+  return (long long)B * H * a.padded() + partialWords(a, p);
 }
 
 }  // extern "C"

@@ -18,22 +18,20 @@ struct Tensor {
 struct Args {
   Tensor q, k, v, out, dout, dq, dk, dv;
   Tensor rest;         // what rounding took from out (bf16), kept for the backward pass, or nullptr
-  float* lse;          // [batch, heads, seq]: log2 of the sum of exp over a row's visible scores; rows that see nothing are not written
-  float* delta;        // [batch, heads, seq]: sum of dout * out over a row (backward)
+  float* lse;          // [batch, heads, padded()]: log2 of the sum of exp over a row's visible scores, infinity for a row behind the sequence's end
+  float* delta;        // the same shape: sum of dout * out over a row (backward)
   const int* lengths;  // [batch] or nullptr
   int B, H, KV, S, D;
   int window, sinks;   // window >= 1 (S or more: everything)
   float scale;
 
   __host__ __device__ int group() const { return H / KV; }
+  __host__ __device__ int padded() const { return (S + 127) / 128 * 128; }  // rows' statistics of a head, in whole tiles
 };
 
 __device__ __forceinline__ int lengthOf(const Args& a, int batch) {
   const int n = a.lengths ? a.lengths[batch] : a.S;
   return n < 0 ? 0 : n > a.S ? a.S : n;
 }
-// Key j is visible to query i of a sequence of L tokens.
-__device__ __forceinline__ bool visible(const Args& a, int i, int j) { return j <= i && (i - j < a.window || j < a.sinks); }
-
 }  // namespace wattn
 }  // namespace b200

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     if (ok) {
       tcFenceAfter();
       const bool live = row < L;
-      if (a.lse && live) a.lse[(size_t)bh * a.S + row] = m * p.c + log2f(l);
+      if (a.lse) a.lse[(size_t)bh * a.padded() + row] = live ? m * p.c + log2f(l) : INFINITY;
       const float inv = 1.f / l;
       uint8_t* stage = smemQ + t * C::kQBytes + q4 * 32 * 256;
       const auto rowsOf = [&](const Tensor& dst) {
@@ -326,6 +326,416 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   tcFenceBefore();
   __syncthreads();
   if (warp == 9) tmemDealloc(tmem, C::kTmemCols);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------
+// Two kernels of one shape, which both form the weights again instead of sharing them through memory, so that no gradient is summed by
+// atomics: a CTA owns 128 rows of two operands (X1, X2), streams 128-row tiles of two others (Y1, Y2) and has in tensor memory
+//   S = X1 Y1^T   and   dP = X2 Y2^T   (or their transposes),
+// from which 256 threads, two per row, make P = 2^(S c - lse) and dS = P (dP - delta) in bf16, in the place of what they were made of, as
+// the tensor-memory operands of the products that follow:
+//   queries: X = Q, dO;  Y = K, V;   dQ += dS Y1. Scores are double buffered. delta is formed here.
+//   keys:    X = K, V;   Y = Q, dO;  dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head.
+// In the keys' kernel dV of a tile and the next tile's S run while its dS is made, dK and the next dP while the next P is made.
+//
+// Y1 of tile n + 2 takes the slot of Y2 of tile n, which is through first, and the other way round.
+//
+// Keys that every later query sees (sinks) would keep their CTAs far longer than the others: the queries behind the window are split over
+// further CTAs, whose fp32 sums joinSinks adds up in a fixed order.
+enum Side { kQueries, kKeys };
+
+struct BwdParams {
+  CUtensorMap x1, x2, y1, y2;
+  Args a;
+  float c;
+  int tiles;      // 128-row tiles of a sequence
+  int sinkTiles;  // key tiles whose far queries are split off; 0: none
+  int farChunk, farCount;  // query tiles per split, splits per sink tile
+  float* partials;         // [B * KV][sinkTiles][1 + farCount][dK, dV][min(sinks, 128)][D]
+  int* err;
+};
+
+template <int HD> struct BwdCfg {
+  static constexpr int kThreads = 384;                // split as in the forward kernel
+  static constexpr int kMathRegs = 216, kOtherRegs = 64;
+  static constexpr int kBoxes = HD / 64;
+  static constexpr uint32_t kTileBytes = kBoxes * kBox;
+  static constexpr uint32_t kXBytes = 8 * 32 * 256;  // X1 and X2, later the staging buffers of eight warps
+  static constexpr size_t kSmem = 1024 + kXBytes + 4 * kTileBytes + 2 * 2 * kTile * 4 + 2 * kTile * 4 + 256;
+  static constexpr uint32_t kTmemCols = 512;
+};
+
+template <int HD, Side SIDE>
+__global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const __grid_constant__ BwdParams p) {
+  using C = BwdCfg<HD>;
+  using namespace sm100;
+  extern __shared__ uint8_t smemRaw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* smemX = smem;                    // X1, X2
+  uint8_t* ring = smem + C::kXBytes;        // 4 slots
+  float* stats = reinterpret_cast<float*>(ring + 4 * C::kTileBytes);  // keys: [2][lse, delta][128]
+  float* half = stats + 4 * kTile;          // queries: [2][128] halves of delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(half + 2 * kTile);
+  uint64_t *xFull = bars, *full = bars + 1, *empty = bars + 5, *sFull = bars + 9 /*[2]*/, *dpFull = bars + 11, *pReady = bars + 12, *dsReady = bars + 13,
+           *statFull = bars + 14 /*[2]*/, *statEmpty = bars + 16 /*[2]*/, *done = bars + 18;
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 19);
+  // tensor memory: queries S0, S1, dP, dQ; keys S, dP, dV, dK
+  constexpr uint32_t kS = 0, kDp = SIDE == kQueries ? 256 : 128, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
+
+  const Args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* err = p.err;
+
+  // ---- what this CTA does: rows [x0, x0 + 128) of head xh against tiles [yFirst, yFirst + yTiles) (queries: keys, sinks first) of `group` heads from yh on
+  const int xHeads = SIDE == kQueries ? a.H : a.KV, all = a.B * xHeads;
+  const int bh = blockIdx.x % all, xh = bh % xHeads, b = bh / xHeads;
+  const int L = lengthOf(a, b);
+  int item = blockIdx.x / all, xTile, far = -1;
+  if constexpr (SIDE == kQueries) {
+    xTile = p.tiles - 1 - item;  // the longest rows first
+  } else {
+    xTile = item < p.tiles ? item : (item - p.tiles) / p.farCount;
+    if (item >= p.tiles) far = (item - p.tiles) % p.farCount;
+  }
+  const int x0 = xTile * kTile;
+  int yFirst, yTiles, sinkTiles = 0;
+  if constexpr (SIDE == kQueries) {
+    const KeyRange r(a, x0, min(x0 + kTile, L) - 1);
+    yFirst = r.first;
+    sinkTiles = min(r.sinkTiles, r.first);
+    yTiles = x0 < L ? sinkTiles + r.last - r.first + 1 : 0;
+  } else {
+    const int lastTile = (L - 1) / kTile;  // of the sequence
+    const int reach = a.window > a.S - x0 ? a.S : x0 + kTile + a.window - 1;  // first query that sees none of the tile's keys through the window
+    const int nearLast = x0 < a.sinks && p.sinkTiles == 0 ? lastTile : min(lastTile, (reach - 1) / kTile);
+    if (far < 0) {
+      yFirst = xTile;
+      yTiles = nearLast - xTile + 1;
+    } else {
+      yFirst = (reach - 1) / kTile + 1 + far * p.farChunk;
+      yTiles = min(p.farChunk, lastTile - yFirst + 1);
+    }
+    if (x0 >= L || yTiles < 0) yTiles = 0;
+  }
+  const int group = SIDE == kQueries ? 1 : a.group(), yh = SIDE == kQueries ? xh / a.group() : xh * a.group();
+  const int count = yTiles * group;
+  const auto tileOf = [&](int n) {
+    if constexpr (SIDE == kQueries) return n < sinkTiles ? n : yFirst + n - sinkTiles;
+    else return yFirst + n % yTiles;
+  };
+  const auto headOf = [&](int n) { return SIDE == kQueries ? yh : yh + n / yTiles; };
+  const bool sinkRows = SIDE == kKeys && xTile < p.sinkTiles;  // some rows' sums go through `partials`
+  const int partRows = sinkRows ? min(kTile, a.sinks - x0) : 0, partPitch = min(a.sinks, kTile);
+  float* part = sinkRows ? p.partials + ((size_t)(bh * p.sinkTiles + xTile) * (1 + p.farCount) + 1 + far) * 2 * partPitch * a.D : nullptr;
+
+  if (count == 0) {
+    if (warp < 8) {
+      const int tid = threadIdx.x & 127, which = warp >> 2;
+      if constexpr (SIDE == kQueries) {
+        if (which == 0) zeroOut(a.dq, b, xh, x0, a.S, a.D, tid);
+      } else {
+        if (far < 0) zeroOut(which ? a.dk : a.dv, b, xh, x0, a.S, a.D, tid);
+        for (int n = tid; n < partRows * a.D; n += 128) part[(which ? 0 : partPitch * a.D) + n] = 0.f;
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    prefetchTensorMap(&p.x1);
+    prefetchTensorMap(&p.x2);
+    prefetchTensorMap(&p.y1);
+    prefetchTensorMap(&p.y2);
+    mbarInit(xFull, 1);
+    for (int s = 0; s < 4; s++) {
+      mbarInit(&full[s], 1);
+      mbarInit(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; s++) {
+      mbarInit(&sFull[s], 1);
+      mbarInit(&statFull[s], 1);
+      mbarInit(&statEmpty[s], 8);
+    }
+    mbarInit(dpFull, 1);
+    mbarInit(pReady, 8);
+    mbarInit(dsReady, 8);
+    mbarInit(done, 1);
+    fenceBarrierInit();
+  }
+  if (warp == 9) {
+    tmemAlloc(tmemSlot, C::kTmemCols);
+    tmemRelinquish();
+  }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = *tmemSlot;
+  const auto slot1 = [](int n) { return 2 * (n & 1) + ((n >> 1) & 1); };
+  const auto slot2 = [](int n) { return 2 * (n & 1) + 1 - ((n >> 1) & 1); };
+
+  if (warp == 8) {
+    setMaxRegsDown<C::kOtherRegs>();
+    if (lane == 0) {
+      mbarArriveExpectTx(xFull, 2 * C::kTileBytes);
+      for (int x = 0; x < C::kBoxes; x++) {
+        tmaLoad4d(smemX + x * kBox, &p.x1, x * 64, x0, xh, b, xFull);
+        tmaLoad4d(smemX + C::kTileBytes + x * kBox, &p.x2, x * 64, x0, xh, b, xFull);
+      }
+      bool ok = true;
+      for (int n = 0; n < count && ok; n++) {
+        const int y0 = tileOf(n) * kTile, h = headOf(n);
+        const uint32_t turn = ((n >> 1) & 1) ^ 1;
+        for (int w = 0; w < 2 && ok; w++) {
+          const int s = w ? slot2(n) : slot1(n);
+          if (!(ok = mbarWait(&empty[s], turn, err, ERR_BWD_LOAD))) break;
+          mbarArriveExpectTx(&full[s], C::kTileBytes);
+          for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * kBox, w ? &p.y2 : &p.y1, x * 64, y0, h, b, &full[s]);
+        }
+        if constexpr (SIDE == kKeys) {
+          if (!ok || !(ok = mbarWait(&statEmpty[n & 1], turn, err, ERR_BWD_LOAD))) break;
+          const size_t at = ((size_t)b * a.H + h) * a.padded() + y0;
+          mbarArriveExpectTx(&statFull[n & 1], 2 * kTile * 4);
+          bulkLoad(stats + (n & 1) * 2 * kTile, a.lse + at, kTile * 4, &statFull[n & 1]);
+          bulkLoad(stats + (n & 1) * 2 * kTile + kTile, a.delta + at, kTile * 4, &statFull[n & 1]);
+        }
+      }
+      if (!ok) {  // let loads in flight land
+        mbarWait(xFull, 0, err, 0, 2000u);
+        for (int s = 0; s < 4; s++) mbarWait(&full[s], 0, err, 0, 2000u);
+      }
+    }
+  } else if (warp == 9) {
+    setMaxRegsDown<C::kOtherRegs>();
+    constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescAcc = instrDescMajor(kTile, HD, 1, 0, 1);
+    const auto wait = [&](int s, int n) { return mbarWait(&full[s], (n >> 1) & 1, err, ERR_BWD_MMA); };
+    // Rows behind the sequence's end are zeroed where they are summed over: a weight of zero does not silence what may lie there.
+    const auto clear = [&](int s, int n) {
+      const int beyond = L - tileOf(n) * kTile;
+      if (beyond < kTile) zeroRows<C::kBoxes>(ring + s * C::kTileBytes, beyond, lane);
+    };
+    const auto product = [&](uint32_t d, int x, int s) {  // d = X Y^T
+      const uint32_t xa = smemAddr(smemX + x * C::kTileBytes), ya = smemAddr(ring + s * C::kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; kk++) {
+        const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
+        mmaF16(tmem + d, smemDescSw128(xa + o), smemDescSw128(ya + o), idescS, kk != 0);
+      }
+    };
+    const auto gather = [&](uint32_t acc, uint32_t w, int s, bool first) {  // acc += W Y, W: two halves of 64 columns, each packed into 32
+      const uint32_t ya = smemAddr(ring + s * C::kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; kk++)
+        mmaF16FromTmem(tmem + acc, tmem + w + (kk / 4) * 64 + (kk % 4) * 8, smemDescSw128Mn(ya + kk * 2048, kBox), idescAcc, !first || kk != 0);
+    };
+    bool ok = mbarWait(xFull, 0, err, ERR_BWD_MMA);
+    const auto scores = [&](int n) {
+      if (!wait(slot1(n), n)) return false;
+      clear(slot1(n), n);
+      if (lane == 0) {
+        const int buf = SIDE == kQueries ? n & 1 : 0;
+        product(kS + buf * kTile, 0, slot1(n));
+        mmaCommit(&sFull[buf]);
+      }
+      __syncwarp();
+      return true;
+    };
+    const auto grads = [&](int n) {
+      if (!wait(slot2(n), n)) return false;
+      if (SIDE == kKeys) clear(slot2(n), n);
+      if (lane == 0) {
+        product(kDp, 1, slot2(n));
+        mmaCommit(dpFull);
+        if (SIDE == kQueries) mmaCommit(&empty[slot2(n)]);
+      }
+      __syncwarp();
+      return true;
+    };
+    ok = ok && scores(0) && grads(0);
+    if (SIDE == kQueries && count > 1) ok = ok && scores(1);
+    for (int n = 0; n < count && ok; n++) {
+      if constexpr (SIDE == kKeys) {
+        if (!(ok = mbarWait(pReady, n & 1, err, ERR_BWD_MMA))) break;
+        tcFenceAfter();
+        if (lane == 0) {
+          gather(kAcc1, kS, slot2(n), n == 0);
+          mmaCommit(&empty[slot2(n)]);
+        }
+        __syncwarp();
+        if (n + 1 < count && !(ok = scores(n + 1))) break;
+      }
+      if (!(ok = mbarWait(dsReady, n & 1, err, ERR_BWD_MMA))) break;
+      tcFenceAfter();
+      if (lane == 0) {
+        gather(SIDE == kQueries ? kAcc1 : kAcc2, kDp, slot1(n), n == 0);
+        mmaCommit(&empty[slot1(n)]);
+        if (n + 1 == count) mmaCommit(done);
+      }
+      __syncwarp();
+      if (n + 1 < count && !(ok = grads(n + 1))) break;
+      if (SIDE == kQueries && n + 2 < count && !(ok = scores(n + 2))) break;
+    }
+  } else if (warp >= 10) {
+    setMaxRegsDown<C::kOtherRegs>();
+  } else {
+    setMaxRegsUp<C::kMathRegs>();
+    const int q4 = warp & 3, side = warp >> 2, r = q4 * 32 + lane, row = x0 + r;
+    const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16), cols = side * 64;
+    const bool live = row < L;
+    float lse = 0.f, delta = 0.f;
+    if constexpr (SIDE == kQueries) {
+      if (live) {
+        lse = a.lse[(size_t)bh * a.padded() + row];
+        const uint4* o = reinterpret_cast<const uint4*>(a.out.at(b, xh, row));
+        const uint4* e = reinterpret_cast<const uint4*>(a.rest.at(b, xh, row));
+        const uint4* g = reinterpret_cast<const uint4*>(a.dout.at(b, xh, row));
+        for (int n = side * (HD / 16); n < min(a.D / 8, (side + 1) * (HD / 16)); n++) {
+          float x[8], y[8], z[8];
+          unpack8(o[n], x);
+          unpack8(e[n], y);
+          unpack8(g[n], z);
+#pragma unroll
+          for (int i = 0; i < 8; i++) delta += (x[i] + y[i]) * z[i];
+        }
+      }
+      half[side * kTile + r] = delta;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      delta = half[r] + half[kTile + r];
+      if (side == 0) a.delta[(size_t)bh * a.padded() + row] = delta;
+    }
+    bool ok = true;
+    for (int n = 0; n < count && ok; n++) {
+      const int y0 = tileOf(n) * kTile;
+      const float* st = stats + (n & 1) * 2 * kTile + cols;
+      if (SIDE == kKeys && !(ok = mbarWait(&statFull[n & 1], (n >> 1) & 1, err, ERR_BWD_MATH))) break;
+      const int buf = SIDE == kQueries ? n & 1 : 0;
+      if (!(ok = mbarWait(&sFull[buf], SIDE == kQueries ? (n >> 1) & 1 : n & 1, err, ERR_BWD_MATH))) break;
+      tcFenceAfter();
+      uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+      const bool every = SIDE == kQueries ? x0 + kTile <= L && seesAll(a, x0, x0 + kTile - 1, y0) : y0 + kTile <= L && seesAll(a, y0, y0 + kTile - 1, x0);
+      if (!every) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const int y = y0 + cols + x * 32;
+          if constexpr (SIDE == kQueries) {
+            bits[x] = live ? maskBits(a, row, y) : 0u;
+          } else {  // queries [row, end) see key `row`
+            const auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
+            const int end = row < a.sinks || a.window > L - row ? L : row + a.window;
+            bits[x] = below(end - y) & ~below(row - y);
+          }
+        }
+      }
+      float w[64];
+      {
+        uint32_t s[2][32];
+        tmemLoad32(base + kS + buf * kTile + cols, s[0]);
+        tmemLoad32(base + kS + buf * kTile + cols + 32, s[1]);
+        tmemLoadWait();
+#pragma unroll
+        for (int e = 0; e < 64; e++) {
+          const float off = SIDE == kQueries ? lse : st[e];
+          const float v = exp2Fast(fmaf(__uint_as_float(s[e / 32][e % 32]), p.c, -off));
+          w[e] = (bits[e / 32] >> (e % 32)) & 1 ? v : 0.f;
+        }
+      }
+      if constexpr (SIDE == kKeys) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          uint32_t o[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 32 + 2 * e], w[x * 32 + 2 * e + 1]);
+          tmemStore16(base + kS + cols + x * 16, o);
+        }
+        tmemStoreWait();
+        tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArrive(pReady);
+      }
+      if (!(ok = mbarWait(dpFull, n & 1, err, ERR_BWD_MATH))) break;
+      tcFenceAfter();
+      {
+        uint32_t d[2][32];
+        tmemLoad32(base + kDp + cols, d[0]);
+        tmemLoad32(base + kDp + cols + 32, d[1]);
+        tmemLoadWait();
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          uint32_t o[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            float v[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int i = x * 32 + 2 * e + k;
+              v[k] = w[i] * (__uint_as_float(d[x][2 * e + k]) - (SIDE == kQueries ? delta : st[kTile + i]));
+              if (!((bits[x] >> (2 * e + k)) & 1)) v[k] = 0.f;  // what is masked may be anything
+            }
+            o[e] = pack2(v[0], v[1]);
+          }
+          tmemStore16(base + kDp + cols + x * 16, o);
+        }
+      }
+      tmemStoreWait();
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) {
+        mbarArrive(dsReady);
+        if (SIDE == kKeys) mbarArrive(&statEmpty[n & 1]);
+      }
+    }
+    ok = ok && mbarWait(done, 0, err, ERR_BWD_MATH);
+    if (ok) {
+      tcFenceAfter();
+      uint8_t* stage = smemX + warp * 32 * 256;
+      const float f = SIDE == kKeys && side == 0 ? 1.f : a.scale;
+      // queries: each of a row's two threads has half of dQ's columns; keys: one has dV, the other dK
+      const uint32_t acc = base + (SIDE == kQueries ? kAcc1 + side * (HD / 2) : side ? kAcc2 : kAcc1);
+      const int width = SIDE == kQueries ? HD / 2 : HD, col0 = SIDE == kQueries ? side * (HD / 2) : 0;
+      const Tensor& dst = SIDE == kQueries ? a.dq : side ? a.dk : a.dv;
+      if (far < 0)
+        gemm::drainStaged(
+            stage, lane, width, a.D - col0,
+            [&](int x, uint32_t(&v)[32]) {
+              tmemLoad32(acc + x * 32, v);
+              tmemLoadWait();
+#pragma unroll
+              for (int e = 0; e < 32; e++) v[e] = live ? __float_as_uint(__uint_as_float(v[e]) * f) : 0u;
+            },
+            [&](int k) -> __nv_bfloat16* {
+              const int out = row - lane + k;
+              return out < a.S && q4 * 32 + k >= partRows ? dst.at(b, xh, out) + col0 : nullptr;
+            });
+      if (q4 * 32 < partRows)
+        for (int x = 0; x < HD / 32; x++) {
+          uint32_t v[32];
+          tmemLoad32(acc + x * 32, v);
+          tmemLoadWait();
+          float* to = part + (size_t)(side ? 0 : partPitch + 0) * a.D + (size_t)r * a.D + x * 32;
+          if (r < partRows)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (x * 32 + e < a.D)
+                *reinterpret_cast<float4*>(to + e) = live ? make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]))
+                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+  }
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == 9) tmemDealloc(tmem, C::kTmemCols);
+}
+
+// dK and dV of the sinks from the sums of their CTAs.
+__global__ void __launch_bounds__(128) joinSinks(const __grid_constant__ BwdParams p) {
+  const Args& a = p.a;
+  const int j = blockIdx.x, bh = blockIdx.y, h = bh % a.KV, b = bh / a.KV, tile = j / kTile, pitch = min(a.sinks, kTile);
+  const float* from = p.partials + (size_t)(bh * p.sinkTiles + tile) * (1 + p.farCount) * 2 * pitch * a.D + (size_t)(j % kTile) * a.D;
+  for (int n = threadIdx.x; n < 2 * a.D; n += blockDim.x) {
+    const int d = n % a.D, which = n / a.D;
+    float v = 0.f;
+    for (int x = 0; x <= p.farCount; x++) v += from[((size_t)2 * x + which) * pitch * a.D + d];
+    (which ? a.dv : a.dk).at(b, h, j)[d] = __float2bfloat16(which ? v : v * a.scale);
+  }
 }
 
 }  // namespace wattn

@@ -29,6 +29,8 @@ def _lib_attn():
         lib.b200ops_qk_norm_rope_bwd.argtypes = [vp] * 7 + [i32] + [vp] * 5 + [ll] + [i32] * 4 + [f32, vp]
         lib.b200ops_window_attention_fwd.argtypes = [vp] * 8 + [i32] * 7 + [f32, vp]
         lib.b200ops_window_attention_bwd.argtypes = [vp] * 13 + [i32] * 7 + [f32, vp]
+        lib.b200ops_window_attention_bwd_scratch.argtypes = [i32] * 7
+        lib.b200ops_window_attention_bwd_scratch.restype = ll
         _sigs_done = True
     return lib
 
@@ -112,7 +114,7 @@ class _WindowAttention(torch.autograd.Function):
         B, H, S, D = q.shape
         KV = k.shape[1]
         out = _by_token(B, H, S, D, q.device)
-        lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if keep else None
+        lse = torch.empty(B, H, (S + 127) // 128 * 128, dtype=torch.float32, device=q.device) if keep else None
         rest = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device) if keep else None  # what rounding took from the answer
         with _on(q):
             _ck(_lib_attn().b200ops_window_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if keep else None, rest.data_ptr() if keep else None,
@@ -131,9 +133,10 @@ class _WindowAttention(torch.autograd.Function):
         B, H, S, D = q.shape
         KV = k.shape[1]
         dq, dk, dv = (_by_token(B, n, S, D, q.device) for n in (H, KV, KV))
-        delta = torch.empty_like(lse)
+        lib = _lib_attn()
         with _on(q):
-            _ck(_lib_attn().b200ops_window_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+            scratch = torch.empty(int(lib.b200ops_window_attention_bwd_scratch(B, H, KV, S, D, window, sinks)), dtype=torch.float32, device=q.device)
+            _ck(lib.b200ops_window_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), scratch.data_ptr(),
                                                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if lengths is None else lengths.data_ptr(),
                                                          _strides(q, k, v, out, dout, dq, dk, dv), B, H, KV, S, D, window, sinks, scale, _s()),
                 "window_attention_bwd")
