@@ -4,6 +4,14 @@
 //   dz   = [(1 - a) (c - onehot_t) + a tau (q - sum_{k: id k = v} p_k)] * gradScale
 // An entry whose id lies outside [0, V) does not exist; a row without entries has no distillation term. A row whose target lies outside
 // [0, V) counts nothing: zero loss, zero gradient.
+//
+// A row is read once and its gradient written once: a cluster of 1 to 8 CTAs holds it in shared memory, a slice each (64 KB if that is
+// enough, so that three CTAs share an SM and one row's loads and stores run beside another's arithmetic). Maximum and sums meet through
+// the cluster's shared memory, the gradient takes the logits' place there and leaves by a bulk store. Each pass then costs one power of two
+// per element where one exponent serves both softmaxes, or where the temperature is a small whole number and c is a power of q by
+// multiplication (kPower); two otherwise.
+#include "gemm_host.h"
+#include "sm100.cuh"
 #include "rows.cuh"
 
 namespace b200 {
@@ -11,8 +19,12 @@ namespace distill {
 
 using namespace rows;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kMaxEntries = 1024;
+constexpr int kMaxCluster = 8;
+constexpr int kSlice = 32768;      // elements of a slice, as long as a cluster of eight can hold the row
+constexpr int kMaxSlice = 104 * 1024;
+constexpr int kErrLoad = 31;
 
 struct Args {
   const __nv_bfloat16* z;
@@ -22,97 +34,231 @@ struct Args {
   const void* values;    // [T, K] fp32 or bf16
   float* loss;
   long long zStride, gradStride;
-  int V, K;
+  int V, K, idBytes, valueBytes, slice, power;
+  bool zBulk, gradBulk;  // rows start on 16-byte boundaries
   float a, tau, gradScale;
+  int* err;
 };
 
-template <int NT> __device__ __forceinline__ float blockReduce(float v, float* sh, bool maximum) {
+// One: a single exponent (temperature one, or one of the two losses alone). Power: c = q^power. Two: both.
+enum Mode { kOne, kPower, kTwo };
+
+__device__ __forceinline__ float blockReduce(float v, float* sh, bool maximum) {
+  constexpr int kWarps = kThreads / 32;
   v = maximum ? laneMax<32>(v) : laneSum<32>(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = (threadIdx.x & 31) < NT / 32 ? sh[threadIdx.x & 31] : maximum ? -INFINITY : 0.f;
+  v = (threadIdx.x & 31) < kWarps ? sh[threadIdx.x & 31] : maximum ? -INFINITY : 0.f;
   return maximum ? laneMax<32>(v) : laneSum<32>(v);
 }
 
-// One CTA per row, three passes over it: maximum, sums, gradient.
-template <typename I, typename W>
-__global__ void __launch_bounds__(kThreads) distillKernel(const Args p) {
-  __shared__ float sh[32];
-  __shared__ int id[kMaxEntries];
-  __shared__ float prob[kMaxEntries], logProb[kMaxEntries], zAt[kMaxEntries];
-  const size_t row = blockIdx.x;
+__device__ __forceinline__ void storeCluster(uint32_t clusterAddr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(clusterAddr), "f"(v) : "memory"); }
+
+template <Mode MODE>
+__global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int ctas) {
+  using namespace sm100;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(smem);
+  int* id = reinterpret_cast<int*>(smem + (size_t)p.slice * 2);
+  float* prob = reinterpret_cast<float*>(id + p.K);
+  float* zAt = prob + p.K;
+  __shared__ float sh[32], meet[3][kMaxCluster];  // of the cluster's CTAs: maximum, sums
+  __shared__ uint64_t bar;
+
+  const size_t row = blockIdx.x / ctas;
+  const int rank = blockIdx.x % ctas;
+  const int first = rank * p.slice, n = max(0, min(p.slice, p.V - first)), nvec = n >> 3;
   const __nv_bfloat16* z = p.z + row * p.zStride;
   __nv_bfloat16* grad = p.grad + row * p.gradStride;
   const long long target = p.targets[row];
-  if (target < 0 || target >= p.V) {
-    if (threadIdx.x == 0) p.loss[row] = 0.f;
-    for (int v = threadIdx.x; v < p.V; v += kThreads) grad[v] = __float2bfloat16(0.f);
+  if (target < 0 || target >= p.V) {  // all CTAs of the cluster alike
+    if (rank == 0 && threadIdx.x == 0) p.loss[row] = 0.f;
+    if (p.gradBulk) {
+      for (int j = threadIdx.x; j < nvec; j += kThreads) reinterpret_cast<uint4*>(grad + first)[j] = make_uint4(0, 0, 0, 0);
+      for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) grad[first + j] = __float2bfloat16(0.f);
+    } else {
+      for (int j = threadIdx.x; j < n; j += kThreads) grad[first + j] = __float2bfloat16(0.f);
+    }
     return;
   }
-  float m = -INFINITY;
-  for (int v = threadIdx.x; v < p.V; v += kThreads) m = fmaxf(m, __bfloat162float(z[v]));
-  m = blockReduce<kThreads>(m, sh, true);
-  const float one = kLog2e, soft = kLog2e / p.tau;
-  float sumOne = 0.f, sumSoft = 0.f;
-  for (int v = threadIdx.x; v < p.V; v += kThreads) {
-    const float d = __bfloat162float(z[v]) - m;
-    sumOne += exp2Fast(d * one);
-    sumSoft += exp2Fast(d * soft);
+  if (threadIdx.x == 0) {
+    mbarInit(&bar, 1);
+    fenceBarrierInit();
+    if (p.zBulk && nvec > 0) {
+      mbarArriveExpectTx(&bar, nvec * 16);
+      bulkLoad(x, z + first, nvec * 16, &bar);
+    }
   }
-  sumOne = blockReduce<kThreads>(sumOne, sh, false);
-  sumSoft = blockReduce<kThreads>(sumSoft, sh, false);
+  __syncthreads();
+  clusterArrive();  // waited for before the first store into another CTA
+  for (int j = (p.zBulk ? nvec * 8 : 0) + threadIdx.x; j < n; j += kThreads) x[j] = z[first + j];
 
-  // the teacher's entries
+  // The teacher's entries, in every CTA, while the slice is on its way.
   float best = -INFINITY;
   for (int k = threadIdx.x; k < p.K; k += kThreads) {
-    const long long i = (long long)reinterpret_cast<const I*>(p.ids)[row * p.K + k];
-    const bool exists = i >= 0 && i < p.V;
-    const float y = exists ? toFloat(reinterpret_cast<const W*>(p.values)[row * p.K + k]) / p.tau : -INFINITY;
+    const long long i = p.idBytes == 8 ? reinterpret_cast<const long long*>(p.ids)[row * p.K + k] : (long long)reinterpret_cast<const int*>(p.ids)[row * p.K + k];
+    const bool exists = i >= 0 && i < p.V && p.a > 0.f;
+    float y = -INFINITY;
+    if (exists) y = (p.valueBytes == 4 ? reinterpret_cast<const float*>(p.values)[row * p.K + k] : toFloat(reinterpret_cast<const __nv_bfloat16*>(p.values)[row * p.K + k])) / p.tau;
     id[k] = exists ? (int)i : -1;
-    logProb[k] = y;
+    prob[k] = y;
     zAt[k] = exists ? __bfloat162float(z[i]) : 0.f;
     best = fmaxf(best, y);
   }
-  best = blockReduce<kThreads>(best, sh, true);
+  const float zt = __bfloat162float(z[target]);
+  best = blockReduce(best, sh, true);
   float norm = 0.f;
   if (best > -INFINITY)
     for (int k = threadIdx.x; k < p.K; k += kThreads)
-      if (id[k] >= 0) norm += exp2Fast((logProb[k] - best) * kLog2e);
-  norm = blockReduce<kThreads>(norm, sh, false);
+      if (id[k] >= 0) norm += exp2Fast((prob[k] - best) * kLog2e);
+  norm = blockReduce(norm, sh, false);  // its barriers also make the plainly loaded elements visible
   const float a = norm == 0.f ? 0.f : p.a;
+
+  // ---- the row's maximum
+  if (p.zBulk && nvec > 0) mbarWait(&bar, 0, p.err, kErrLoad);  // given up or not, the CTA stays: its cluster writes into it
+  __nv_bfloat162 top2 = __float2bfloat162_rn(-INFINITY);
+  const uint4* xv = reinterpret_cast<const uint4*>(x);
+  for (int j = threadIdx.x; j < nvec; j += kThreads) {
+    const uint4 raw = xv[j];
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    top2 = __hmax2(top2, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  }
+  float m = fmaxf(__low2float(top2), __high2float(top2));
+  for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) m = fmaxf(m, __bfloat162float(x[j]));
+  m = blockReduce(m, sh, true);
+  clusterWait();
+  if (threadIdx.x < ctas) storeCluster(mapToCta(smemAddr(&meet[0][rank]), threadIdx.x), m);
+  clusterArrive();
+  clusterWait();
+  for (int r = 0; r < ctas; r++) m = fmaxf(m, meet[0][r]);
+
+  // ---- the sums
+  const float soft = MODE == kOne && p.a == 0.f ? kLog2e : kLog2e / p.tau, one = kLog2e;
+  const float offSoft = m * soft, offOne = m * one;
+  const auto powers = [&](float v, float& q, float& c) {
+    q = exp2Fast(fmaf(v, soft, -offSoft));
+    if constexpr (MODE == kPower) {
+      c = q * q;
+      if (p.power >= 3) c *= p.power == 3 ? q : c;
+    } else if constexpr (MODE == kTwo) {
+      c = exp2Fast(fmaf(v, one, -offOne));
+    } else {
+      c = q;
+    }
+  };
+  float sumSoft = 0.f, sumOne = 0.f;
+  for (int j = threadIdx.x; j < nvec; j += kThreads) {
+    float f[8], q[8], c[8];
+    unpack8(xv[j], f);
+#pragma unroll
+    for (int e = 0; e < 8; e++) powers(f[e], q[e], c[e]);
+    sumSoft += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    if (MODE != kOne) sumOne += ((c[0] + c[1]) + (c[2] + c[3])) + ((c[4] + c[5]) + (c[6] + c[7]));
+  }
+  for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) {
+    float q, c;
+    powers(__bfloat162float(x[j]), q, c);
+    sumSoft += q;
+    sumOne += c;
+  }
+  sumSoft = blockReduce(sumSoft, sh, false);
+  if (MODE != kOne) sumOne = blockReduce(sumOne, sh, false);
+  if (threadIdx.x < ctas) {
+    storeCluster(mapToCta(smemAddr(&meet[1][rank]), threadIdx.x), sumSoft);
+    storeCluster(mapToCta(smemAddr(&meet[2][rank]), threadIdx.x), sumOne);
+  }
+  clusterArrive();  // also: no CTA writes its part of the gradient before every CTA has read the logits that it looks up
+  clusterWait();
+  sumSoft = sumOne = 0.f;
+  for (int r = 0; r < ctas; r++) {
+    sumSoft += meet[1][r];
+    sumOne += meet[2][r];
+  }
+  if (MODE == kOne) sumOne = sumSoft;
+
+  // ---- the loss
   const float logNorm = logf(norm), logSoft = logf(sumSoft);
   float kl = 0.f;
   for (int k = threadIdx.x; k < p.K; k += kThreads) {
-    const float lp = logProb[k] - best - logNorm;
+    const float lp = prob[k] - best - logNorm;
     const float pk = id[k] >= 0 && norm != 0.f ? exp2Fast(lp * kLog2e) : 0.f;
     prob[k] = pk;
     if (pk != 0.f) kl += pk * (lp - ((zAt[k] - m) / p.tau - logSoft));
   }
-  kl = blockReduce<kThreads>(kl, sh, false);
-  const float zt = __bfloat162float(z[target]);
-  if (threadIdx.x == 0) p.loss[row] = (1.f - p.a) * (m + logf(sumOne) - zt) + a * p.tau * p.tau * kl;
-  __syncthreads();
+  if (rank == 0) {
+    kl = blockReduce(kl, sh, false);
+    if (threadIdx.x == 0) {
+      float loss = a == 0.f ? 0.f : a * p.tau * p.tau * kl;
+      if (p.a < 1.f) loss += (1.f - p.a) * (m + logf(sumOne) - zt);
+      p.loss[row] = loss;
+    }
+  }
 
-  const float fOne = (1.f - p.a) / sumOne * p.gradScale, fSoft = a * p.tau / sumSoft * p.gradScale;
-  const auto dense = [&](float x) { return fOne * exp2Fast((x - m) * one) + fSoft * exp2Fast((x - m) * soft); };
-  for (int v = threadIdx.x; v < p.V; v += kThreads) grad[v] = __float2bfloat16(dense(__bfloat162float(z[v])));
+  // ---- the gradient, in the logits' place
+  const float fOne = p.a < 1.f ? (1.f - p.a) / sumOne * p.gradScale : 0.f, fSoft = a == 0.f ? 0.f : a * p.tau / sumSoft * p.gradScale;
+  const auto dense = [&](float v) {
+    float q, c;
+    powers(v, q, c);
+    return MODE == kOne ? (fOne + fSoft) * q : fOne * c + fSoft * q;
+  };
+  for (int j = threadIdx.x; j < nvec; j += kThreads) {
+    float f[8];
+    unpack8(xv[j], f);
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = dense(f[e]);
+    reinterpret_cast<uint4*>(x)[j] = pack8(f);
+  }
+  for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) x[j] = __float2bfloat16(dense(__bfloat162float(x[j])));
   __syncthreads();
   // The teacher's entries and the target once more, from their logits in 32 bits. An id's first entry writes for all of them.
   for (int k = threadIdx.x; k <= p.K; k += kThreads) {
     const int v = k < p.K ? id[k] : (int)target;
-    if (v < 0) continue;
+    if (v < first || v >= first + n) continue;
     float mass = 0.f;
-    bool first = true;
+    bool again = false;
     for (int o = 0; o < p.K; o++)
       if (id[o] == v) {
         mass += prob[o];
-        first = first && o >= k;
+        again = again || o < k;
       }
-    if (!first) continue;
-    const float x = k < p.K ? zAt[k] : zt;
-    grad[v] = __float2bfloat16(dense(x) - p.gradScale * (a * p.tau * mass + (v == target ? 1.f - p.a : 0.f)));
+    if (!again) x[v - first] = __float2bfloat16(dense(k < p.K ? zAt[k] : zt) - p.gradScale * (a * p.tau * mass + (v == target ? 1.f - p.a : 0.f)));
   }
+  fenceProxyAsync();
+  __syncthreads();
+  if (p.gradBulk) {
+    for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) grad[first + j] = x[j];
+    if (threadIdx.x == 0 && nvec > 0) {
+      bulkStore(grad + first, x, nvec * 16);
+      tmaStoreCommit();
+      tmaStoreWaitRead0();
+    }
+  } else {
+    for (int j = threadIdx.x; j < n; j += kThreads) grad[first + j] = x[j];
+  }
+}
+
+template <Mode MODE> cudaError_t launch(const Args& p, long long T, int ctas, size_t smem, cudaStream_t s) {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(distillKernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxSlice + 12 * kMaxEntries);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(T * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = ctas;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, distillKernel<MODE>, p, ctas);
 }
 
 }  // namespace distill
@@ -121,19 +267,37 @@ __global__ void __launch_bounds__(kThreads) distillKernel(const Args p) {
 extern "C" {
 
 // Rows of logits [T, V] bf16 (row stride in elements) and of grad (the same buffer and stride, or another); targets int64 [T];
-// ids [T, K] int64 (idBytes 8) or int32 (4); values [T, K] fp32 (valueBytes 4) or bf16 (2); loss fp32 [T].
+// ids [T, K] int64 (idBytes 8) or int32 (4); values [T, K] fp32 (valueBytes 4) or bf16 (2); loss fp32 [T]. V up to 851,968, K up to 1024.
 int b200ops_distill_loss(const void* logits, void* grad, const long long* targets, const void* ids, int idBytes, const void* values, int valueBytes, float* loss,
                          long long T, int V, int K, long long stride, long long gradStride, float a, float tau, float gradScale, cudaStream_t s) {
   using namespace b200::distill;
-  if (T < 0 || T > 0x7fffffffLL || V <= 0 || K <= 0 || K > kMaxEntries || !(tau > 0.f) || stride < V || gradStride < V || (idBytes != 4 && idBytes != 8) ||
-      (valueBytes != 2 && valueBytes != 4))
+  if (T < 0 || V <= 0 || V > kMaxCluster * kMaxSlice || K <= 0 || K > kMaxEntries || !(tau > 0.f) || !(a >= 0.f && a <= 1.f) || stride < V || gradStride < V ||
+      (idBytes != 4 && idBytes != 8) || (valueBytes != 2 && valueBytes != 4) || (((uintptr_t)logits | (uintptr_t)grad) & 1))
     return (int)cudaErrorInvalidValue;
   if (T == 0) return 0;
-  const Args p{(const __nv_bfloat16*)logits, (__nv_bfloat16*)grad, targets, ids, values, loss, stride, gradStride, V, K, a, tau, gradScale};
-  const auto go = [&](auto kernel) { kernel<<<(unsigned)T, kThreads, 0, s>>>(p); };
-  if (idBytes == 8) go(valueBytes == 4 ? distillKernel<long long, float> : distillKernel<long long, __nv_bfloat16>);
-  else go(valueBytes == 4 ? distillKernel<int, float> : distillKernel<int, __nv_bfloat16>);
-  return (int)cudaGetLastError();
+  int ctas = 1;
+  while (ctas < kMaxCluster && (long long)ctas * kSlice < V) ctas *= 2;
+  if (T * ctas > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  Args p{};
+  p.z = (const __nv_bfloat16*)logits;
+  p.grad = (__nv_bfloat16*)grad;
+  p.targets = targets;
+  p.ids = ids;
+  p.values = values;
+  p.loss = loss;
+  p.zStride = stride;
+  p.gradStride = gradStride;
+  p.V = V, p.K = K, p.idBytes = idBytes, p.valueBytes = valueBytes;
+  p.slice = ((V + ctas - 1) / ctas + 63) / 64 * 64;
+  p.zBulk = ((uintptr_t)logits & 15) == 0 && (stride % 8 == 0 || T == 1);
+  p.gradBulk = ((uintptr_t)grad & 15) == 0 && (gradStride % 8 == 0 || T == 1);
+  p.a = a, p.tau = tau, p.gradScale = gradScale;
+  p.err = b200::gemm::errWord();
+  if (!p.err) return (int)cudaErrorMemoryAllocation;
+  p.power = tau == 2.f || tau == 3.f || tau == 4.f ? (int)tau : 0;
+  const size_t smem = (size_t)p.slice * 2 + (size_t)K * 12;
+  if (tau == 1.f || a == 0.f || a == 1.f) return (int)launch<kOne>(p, T, ctas, smem, s);
+  return (int)(p.power ? launch<kPower>(p, T, ctas, smem, s) : launch<kTwo>(p, T, ctas, smem, s));
 }
 
 }  // extern "C"

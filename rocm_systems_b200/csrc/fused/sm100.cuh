@@ -87,6 +87,9 @@ __device__ __forceinline__ void bulkLoad(void* smemDst, const void* src, uint32_
                "r"(smemAddr(bar))
                : "memory");
 }
+__device__ __forceinline__ void bulkStore(void* dst, const void* smemSrc, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smemAddr(smemSrc)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void tmaStore2d(const CUtensorMap* map, const void* smemSrc, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smemAddr(smemSrc)), "r"(x), "r"(y)
                : "memory");

@@ -197,7 +197,7 @@ def distill_loss(logits: torch.Tensor, targets: torch.Tensor, teacher_ids: torch
 
     ``loss = (1 - weight) * cross_entropy(z, target) + weight * t^2 * KL(softmax(teacher_logits / t) || softmax(z / t))`` with the temperature
     ``t``; the first softmax runs over the row's stored entries, the second over the whole vocabulary. ``logits`` [T, V] bf16 with dense rows;
-    ``targets`` int64 [T]; ``teacher_ids`` [T, K] int64 or int32, ``teacher_logits`` [T, K] fp32 or bf16, K at most 1024, in any order. Entries of
+    V at most 851,968; ``targets`` int64 [T]; ``teacher_ids`` [T, K] int64 or int32, ``teacher_logits`` [T, K] fp32 or bf16, K at most 1024, in any order. Entries of
     one id add up; an entry whose id is outside [0, V) counts nothing, and a row without entries has no second term. A row whose target is
     outside [0, V) (padding) has zero loss and zero gradient. The gradient, times ``grad_scale``, goes to ``grad`` (``logits`` itself: in
     place), by default a new tensor."""
@@ -207,6 +207,7 @@ def distill_loss(logits: torch.Tensor, targets: torch.Tensor, teacher_ids: torch
     assert targets.shape == (T,) and targets.dtype == torch.int64 and targets.is_contiguous(), "targets: contiguous int64 [T]"
     assert teacher_ids.dim() == 2 and teacher_ids.shape == teacher_logits.shape and teacher_ids.shape[0] == T, "teacher_ids and teacher_logits: [T, K]"
     K = teacher_ids.shape[1]
+    assert V <= 851968, "a vocabulary of up to 851,968"
     assert 1 <= K <= 1024, "1 to 1024 teacher entries per row"
     assert teacher_ids.dtype in (torch.int64, torch.int32) and teacher_logits.dtype in (torch.float32, torch.bfloat16), "int64 or int32 ids, fp32 or bf16 logits"
     assert 0.0 <= weight <= 1.0 and 0.0 < temperature < math.inf and math.isfinite(grad_scale), "0 <= weight <= 1, temperature above 0"

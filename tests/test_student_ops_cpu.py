@@ -85,6 +85,7 @@ def _loss_args(T=4, V=64, K=3, **over):
     ("targets", _loss_args(targets=torch.zeros(4, dtype=torch.int32))),
     ("targets", _loss_args(targets=torch.zeros(5, dtype=torch.int64))),
     ("teacher_ids and teacher_logits", _loss_args(teacher_logits=torch.zeros(4, 2))),
+    ("vocabulary", _loss_args(T=1, V=851969)),
     ("teacher entries", _loss_args(K=0)),
     ("teacher entries", _loss_args(K=1025)),
     ("int64 or int32 ids", _loss_args(teacher_ids=torch.zeros(4, 3, dtype=torch.int16))),
@@ -126,7 +127,7 @@ def test_c_entries_refuse_what_they_cannot_run():
         assert lib.b200ops_qk_norm_rope_bwd(p, p, p, none, p, p, p, 1, p, p, p, p, p, 8, seq, heads, kv, D, 1e-5, None) == invalid
     t = train_ops._lib_ops()
     loss = lambda T=4, V=64, K=3, st=64, gst=64, ib=8, vb=4, tau=1.0: t.b200ops_distill_loss(p, p, p, p, ib, p, vb, p, T, V, K, st, gst, 1.0, tau, 1.0, None)
-    for bad in ({"T": -1}, {"V": 0}, {"K": 0}, {"K": 1025}, {"st": 63}, {"gst": 8}, {"ib": 2}, {"vb": 8}, {"tau": 0.0}, {"tau": float("nan")}):
+    for bad in ({"T": -1}, {"V": 0}, {"V": 851969, "st": 851976, "gst": 851976}, {"K": 0}, {"K": 1025}, {"st": 63}, {"gst": 8}, {"ib": 2}, {"vb": 8}, {"tau": 0.0}, {"tau": float("nan")}):
         assert loss(**bad) == invalid, bad
 
 

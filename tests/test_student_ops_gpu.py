@@ -211,8 +211,8 @@ def _check_distill(logits, tgt, ids, values, weight, tau, scale, grad=None):
 
 
 @pytest.mark.parametrize("T, V, K", [(1, 1, 1), (1, 8, 3), (5, 7, 7), (3, 1000, 16), (9, 1003, 5), (4, 4096, 1), (6, 32000, 64), (4, 50257, 33), (5, 128256, 64), (2, 300000, 200),
-                                     (3, 5000, 1024)])
-@pytest.mark.parametrize("weight, tau", [(0.5, 2.0), (1.0, 1.0), (0.0, 3.0)])
+                                     (3, 5000, 1024), (3, 32768, 9), (3, 32776, 9), (2, 65600, 9), (1, 262145, 5), (1, 851968, 5)])
+@pytest.mark.parametrize("weight, tau", [(0.5, 2.0), (1.0, 1.0), (0.0, 3.0), (0.3, 3.0), (0.6, 4.0), (0.4, 1.0), (1.0, 2.5), (0.7, 2.5)])
 def test_distill_loss(T, V, K, weight, tau):
     _check_distill(*_distill_inputs(T + V, T, V, K), weight, tau, 1 / T)
 
