@@ -14,6 +14,8 @@ Cases (inputs are larger than the 126 MB L2 where the kernel streams memory, and
     ep          expert-parallel route / dispatch / grouped expert GEMMs / combine on one rank (32 experts)
     train       RMSNorm forward + backward, RoPE, SwiGLU forward + backward, cross-entropy, embedding, AdamW at the shapes
                 of the 8B model's step
+    student     per-head norms with the rotation, windowed attention with sinks (both ways, with and without a window) and the
+                distillation loss at the 8B model's shapes, 4096 tokens (1024 in the loss)
     emu         the collective kernels' multi-rank paths (flag-in-data all-reduce, pipelined staged reduce with bulk loads,
                 staged copy, FIFO send/recv, fused reduce-scatter+cast) as 4 emulated ranks in one cooperative kernel;
                 must be started with B200COLL_EMULATE_RANKS=1 B200COLL_NVLS_ENABLE=0 in the environment
@@ -181,6 +183,38 @@ def case_train(iters: int) -> dict:
     return res
 
 
+def case_student(iters: int) -> dict:
+    from ..ops import attention, train_ops as ops
+
+    S, H, KV, D, V = 4096, 32, 8, 128, 128256
+    res = {}
+
+    def both(name, fwd, leaves, grads):
+        """Times of the forward call alone and of the backward call alone (its graph is kept)."""
+        with torch.no_grad():
+            res[name + "_eval_ms"] = _time(fwd, iters)
+        res[name + "_fwd_ms"] = _time(fwd, iters)
+        out = fwd()
+        res[name + "_bwd_ms"] = _time(lambda: torch.autograd.grad(out, leaves, grads, retain_graph=True), iters)
+
+    qkv = torch.randn(1, S, H + 2 * KV, D, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    wq, wk = (torch.ones(D, device="cuda", dtype=torch.bfloat16).requires_grad_(True) for _ in range(2))
+    table = ops.rope_table(S, D, 500000.0, "cuda")
+    dq, dk, dv = (torch.randn(1, S, n, D, device="cuda").to(torch.bfloat16).transpose(1, 2) for n in (H, KV, KV))
+    both("qk_norm_rope", lambda: attention.qk_norm_rope(qkv, wq, wk, table, H, KV), (qkv, wq, wk), (dq, dk, dv))
+    q, k, v = (t.detach().requires_grad_(True) for t in attention.qk_norm_rope(qkv, wq, wk, table, H, KV))
+    both("attention_window", lambda: attention.window_attention(q, k, v, 1024, 4), (q, k, v), dq)
+    both("attention_full", lambda: attention.window_attention(q, k, v), (q, k, v), dq)
+    T, K = 1024, 64
+    logits = torch.randn(T, V, device="cuda").to(torch.bfloat16)
+    tgt = torch.randint(0, V, (T,), device="cuda")
+    ids, values, grad = torch.randint(0, V, (T, K), device="cuda"), torch.randn(T, K, device="cuda"), torch.empty_like(logits)
+    for name, weight, tau in (("", 0.75, 2.0), ("_alone", 1.0, 2.0), ("_two_exponents", 0.75, 2.5)):
+        res["distill" + name + "_ms"] = _time(lambda: ops.distill_loss(logits, tgt, ids, values, weight, tau, 1.0 / T, grad=grad), iters)
+    res["gemm_error"] = ops.gemm_take_error()
+    return res
+
+
 def case_emu(iters: int) -> dict:
     if os.environ.get("B200COLL_EMULATE_RANKS") != "1":
         raise SystemExit("the emu case needs B200COLL_EMULATE_RANKS=1 B200COLL_NVLS_ENABLE=0 in the environment")
@@ -198,7 +232,7 @@ def case_emu(iters: int) -> dict:
     return res
 
 
-CASES = {"gemm": case_gemm, "fp8": case_fp8, "decode": case_decode, "tp": case_tp, "ep": case_ep, "train": case_train, "emu": case_emu}
+CASES = {"gemm": case_gemm, "fp8": case_fp8, "decode": case_decode, "tp": case_tp, "ep": case_ep, "train": case_train, "student": case_student, "emu": case_emu}
 
 
 def main() -> int:

@@ -53,6 +53,10 @@ __device__ __forceinline__ float blockReduce(float v, float* sh, bool maximum) {
   return maximum ? laneMax<32>(v) : laneSum<32>(v);
 }
 
+__device__ __forceinline__ float teacherValue(const Args& p, size_t row, int k) {
+  return (p.valueBytes == 4 ? reinterpret_cast<const float*>(p.values)[row * p.K + k] : toFloat(reinterpret_cast<const __nv_bfloat16*>(p.values)[row * p.K + k])) / p.tau;
+}
+
 __device__ __forceinline__ void storeCluster(uint32_t clusterAddr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(clusterAddr), "f"(v) : "memory"); }
 
 template <Mode MODE>
@@ -63,62 +67,55 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
   int* id = reinterpret_cast<int*>(smem + (size_t)p.slice * 2);
   float* prob = reinterpret_cast<float*>(id + p.K);
   float* zAt = prob + p.K;
-  __shared__ float sh[32], meet[3][kMaxCluster];  // of the cluster's CTAs: maximum, sums
+  __shared__ float sh[32], meet[3][kMaxCluster];  // of the cluster's CTAs: maximum, sums relative to it
+  __shared__ float teacher[4];                    // largest value, logarithm of the sum, 1 if there are entries; the target's logit
   __shared__ uint64_t bar;
 
   const size_t row = blockIdx.x / ctas;
-  const int rank = blockIdx.x % ctas;
+  const int rank = blockIdx.x % ctas, lane = threadIdx.x & 31;
   const int first = rank * p.slice, n = max(0, min(p.slice, p.V - first)), nvec = n >> 3;
   const __nv_bfloat16* z = p.z + row * p.zStride;
   __nv_bfloat16* grad = p.grad + row * p.gradStride;
-  const long long target = p.targets[row];
-  if (target < 0 || target >= p.V) {  // all CTAs of the cluster alike
-    if (rank == 0 && threadIdx.x == 0) p.loss[row] = 0.f;
-    if (p.gradBulk) {
-      for (int j = threadIdx.x; j < nvec; j += kThreads) reinterpret_cast<uint4*>(grad + first)[j] = make_uint4(0, 0, 0, 0);
-      for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) grad[first + j] = __float2bfloat16(0.f);
-    } else {
-      for (int j = threadIdx.x; j < n; j += kThreads) grad[first + j] = __float2bfloat16(0.f);
-    }
-    return;
-  }
+  const bool bulk = p.zBulk && nvec > 0;
   if (threadIdx.x == 0) {
     mbarInit(&bar, 1);
     fenceBarrierInit();
-    if (p.zBulk && nvec > 0) {
+    if (bulk) {
       mbarArriveExpectTx(&bar, nvec * 16);
       bulkLoad(x, z + first, nvec * 16, &bar);
     }
   }
   __syncthreads();
   clusterArrive();  // waited for before the first store into another CTA
+  const long long target = p.targets[row];
+  const bool counts = target >= 0 && target < p.V;  // for all CTAs of the cluster alike
   for (int j = (p.zBulk ? nvec * 8 : 0) + threadIdx.x; j < n; j += kThreads) x[j] = z[first + j];
 
-  // The teacher's entries, in every CTA, while the slice is on its way.
-  float best = -INFINITY;
-  for (int k = threadIdx.x; k < p.K; k += kThreads) {
-    const long long i = p.idBytes == 8 ? reinterpret_cast<const long long*>(p.ids)[row * p.K + k] : (long long)reinterpret_cast<const int*>(p.ids)[row * p.K + k];
-    const bool exists = i >= 0 && i < p.V && p.a > 0.f;
-    float y = -INFINITY;
-    if (exists) y = (p.valueBytes == 4 ? reinterpret_cast<const float*>(p.values)[row * p.K + k] : toFloat(reinterpret_cast<const __nv_bfloat16*>(p.values)[row * p.K + k])) / p.tau;
-    id[k] = exists ? (int)i : -1;
-    prob[k] = y;
-    zAt[k] = exists ? __bfloat162float(z[i]) : 0.f;
-    best = fmaxf(best, y);
+  // What the teacher says, in every CTA, while the slice is on its way.
+  if (counts) {
+    for (int k = threadIdx.x; k < p.K; k += kThreads) {
+      const long long i = p.idBytes == 8 ? reinterpret_cast<const long long*>(p.ids)[row * p.K + k] : (long long)reinterpret_cast<const int*>(p.ids)[row * p.K + k];
+      const bool exists = i >= 0 && i < p.V && p.a > 0.f;
+      id[k] = exists ? (int)i : -1;
+      prob[k] = exists ? teacherValue(p, row, k) : -INFINITY;
+      zAt[k] = exists ? __bfloat162float(z[i]) : 0.f;
+    }
+    if (threadIdx.x == kThreads - 1) teacher[3] = __bfloat162float(z[target]);
   }
-  const float zt = __bfloat162float(z[target]);
-  best = blockReduce(best, sh, true);
-  float norm = 0.f;
-  if (best > -INFINITY)
-    for (int k = threadIdx.x; k < p.K; k += kThreads)
-      if (id[k] >= 0) norm += exp2Fast((prob[k] - best) * kLog2e);
-  norm = blockReduce(norm, sh, false);  // its barriers also make the plainly loaded elements visible
-  const float a = norm == 0.f ? 0.f : p.a;
+  if (bulk) mbarWait(&bar, 0, p.err, kErrLoad);  // given up or not, the CTA stays: its cluster writes into it
+  if (!counts) {
+    if (rank == 0 && threadIdx.x == 0) p.loss[row] = 0.f;
+    if (p.gradBulk)
+      for (int j = threadIdx.x; j < nvec; j += kThreads) reinterpret_cast<uint4*>(grad + first)[j] = make_uint4(0, 0, 0, 0);
+    for (int j = (p.gradBulk ? nvec * 8 : 0) + threadIdx.x; j < n; j += kThreads) grad[first + j] = __float2bfloat16(0.f);
+    clusterWait();
+    return;
+  }
+  __syncthreads();  // plainly loaded elements and the teacher's entries are in shared memory
 
-  // ---- the row's maximum
-  if (p.zBulk && nvec > 0) mbarWait(&bar, 0, p.err, kErrLoad);  // given up or not, the CTA stays: its cluster writes into it
+  // ---- the slice's maximum
+  uint4* xv = reinterpret_cast<uint4*>(x);
   __nv_bfloat162 top2 = __float2bfloat162_rn(-INFINITY);
-  const uint4* xv = reinterpret_cast<const uint4*>(x);
   for (int j = threadIdx.x; j < nvec; j += kThreads) {
     const uint4 raw = xv[j];
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
@@ -127,89 +124,102 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
   float m = fmaxf(__low2float(top2), __high2float(top2));
   for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) m = fmaxf(m, __bfloat162float(x[j]));
   m = blockReduce(m, sh, true);
-  clusterWait();
-  if (threadIdx.x < ctas) storeCluster(mapToCta(smemAddr(&meet[0][rank]), threadIdx.x), m);
-  clusterArrive();
-  clusterWait();
-  for (int r = 0; r < ctas; r++) m = fmaxf(m, meet[0][r]);
 
-  // ---- the sums
+  if (threadIdx.x < 32) {  // the teacher's softmax, by one warp from shared memory
+    float best = -INFINITY, norm = 0.f;
+    for (int k = lane; k < p.K; k += 32) best = fmaxf(best, prob[k]);
+    best = laneMax<32>(best);
+    if (best > -INFINITY)
+      for (int k = lane; k < p.K; k += 32)
+        if (id[k] >= 0) norm += exp2Fast((prob[k] - best) * kLog2e);
+    norm = laneSum<32>(norm);
+    const float logNorm = logf(norm);
+    for (int k = lane; k < p.K; k += 32) prob[k] = id[k] >= 0 && norm != 0.f ? exp2Fast((prob[k] - best - logNorm) * kLog2e) : 0.f;
+    if (lane == 0) teacher[0] = best, teacher[1] = logNorm, teacher[2] = norm == 0.f ? 0.f : 1.f;
+  }
+
+  // ---- the slice's sums, relative to its own maximum: one exchange with the cluster is enough
   const float soft = MODE == kOne && p.a == 0.f ? kLog2e : kLog2e / p.tau, one = kLog2e;
-  const float offSoft = m * soft, offOne = m * one;
-  const auto powers = [&](float v, float& q, float& c) {
-    q = exp2Fast(fmaf(v, soft, -offSoft));
+  const F2 soft2 = makeF2(soft, soft), one2 = makeF2(one, one);
+  F2 offSoft, offOne;
+  const auto relativeTo = [&](float top) {
+    offSoft = makeF2(-top * soft, -top * soft);
+    offOne = makeF2(-top * one, -top * one);
+  };
+  const auto powers = [&](F2 v, F2& q, F2& c) {
+    q = exp2F2(fmaF2(v, soft2, offSoft));
     if constexpr (MODE == kPower) {
-      c = q * q;
-      if (p.power >= 3) c *= p.power == 3 ? q : c;
+      c = mulF2(q, q);
+      if (p.power >= 3) c = mulF2(c, p.power == 3 ? q : c);
     } else if constexpr (MODE == kTwo) {
-      c = exp2Fast(fmaf(v, one, -offOne));
+      c = exp2F2(fmaF2(v, one2, offOne));
     } else {
       c = q;
     }
   };
-  float sumSoft = 0.f, sumOne = 0.f;
+  relativeTo(m == -INFINITY ? 0.f : m);  // nothing but minus infinity in this slice: sums of zero
+  F2 partSoft = makeF2(0.f, 0.f), partOne = partSoft;
   for (int j = threadIdx.x; j < nvec; j += kThreads) {
-    float f[8], q[8], c[8];
-    unpack8(xv[j], f);
-#pragma unroll
-    for (int e = 0; e < 8; e++) powers(f[e], q[e], c[e]);
-    sumSoft += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
-    if (MODE != kOne) sumOne += ((c[0] + c[1]) + (c[2] + c[3])) + ((c[4] + c[5]) + (c[6] + c[7]));
+    const uint4 raw = xv[j];
+    F2 q[4], c[4];
+    powers(unpackF2(raw.x), q[0], c[0]);
+    powers(unpackF2(raw.y), q[1], c[1]);
+    powers(unpackF2(raw.z), q[2], c[2]);
+    powers(unpackF2(raw.w), q[3], c[3]);
+    partSoft = addF2(partSoft, addF2(addF2(q[0], q[1]), addF2(q[2], q[3])));
+    if (MODE != kOne) partOne = addF2(partOne, addF2(addF2(c[0], c[1]), addF2(c[2], c[3])));
   }
   for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) {
-    float q, c;
-    powers(__bfloat162float(x[j]), q, c);
-    sumSoft += q;
-    sumOne += c;
+    F2 q, c;
+    powers(makeF2(__bfloat162float(x[j]), -INFINITY), q, c);
+    partSoft = addF2(partSoft, q);
+    partOne = addF2(partOne, c);
   }
-  sumSoft = blockReduce(sumSoft, sh, false);
-  if (MODE != kOne) sumOne = blockReduce(sumOne, sh, false);
+  float sumSoft, sumOne, upper;
+  splitF2(partSoft, sumSoft, upper);
+  sumSoft = blockReduce(sumSoft + upper, sh, false);
+  splitF2(partOne, sumOne, upper);
+  if (MODE != kOne) sumOne = blockReduce(sumOne + upper, sh, false);
+  clusterWait();
   if (threadIdx.x < ctas) {
+    storeCluster(mapToCta(smemAddr(&meet[0][rank]), threadIdx.x), m);
     storeCluster(mapToCta(smemAddr(&meet[1][rank]), threadIdx.x), sumSoft);
     storeCluster(mapToCta(smemAddr(&meet[2][rank]), threadIdx.x), sumOne);
   }
+  __syncthreads();
   clusterArrive();  // also: no CTA writes its part of the gradient before every CTA has read the logits that it looks up
   clusterWait();
+  m = -INFINITY;
+  for (int r = 0; r < ctas; r++) m = fmaxf(m, meet[0][r]);
   sumSoft = sumOne = 0.f;
   for (int r = 0; r < ctas; r++) {
-    sumSoft += meet[1][r];
-    sumOne += meet[2][r];
+    const float d = meet[0][r] - m;
+    if (meet[1][r] == 0.f) continue;  // nothing but minus infinity in this slice
+    sumSoft += meet[1][r] * exp2Fast(d * soft);
+    sumOne += meet[2][r] * exp2Fast(d * one);
   }
   if (MODE == kOne) sumOne = sumSoft;
-
-  // ---- the loss
-  const float logNorm = logf(norm), logSoft = logf(sumSoft);
-  float kl = 0.f;
-  for (int k = threadIdx.x; k < p.K; k += kThreads) {
-    const float lp = prob[k] - best - logNorm;
-    const float pk = id[k] >= 0 && norm != 0.f ? exp2Fast(lp * kLog2e) : 0.f;
-    prob[k] = pk;
-    if (pk != 0.f) kl += pk * (lp - ((zAt[k] - m) / p.tau - logSoft));
-  }
-  if (rank == 0) {
-    kl = blockReduce(kl, sh, false);
-    if (threadIdx.x == 0) {
-      float loss = a == 0.f ? 0.f : a * p.tau * p.tau * kl;
-      if (p.a < 1.f) loss += (1.f - p.a) * (m + logf(sumOne) - zt);
-      p.loss[row] = loss;
-    }
-  }
+  relativeTo(m);
+  const float a = teacher[2] == 0.f ? 0.f : p.a;
 
   // ---- the gradient, in the logits' place
   const float fOne = p.a < 1.f ? (1.f - p.a) / sumOne * p.gradScale : 0.f, fSoft = a == 0.f ? 0.f : a * p.tau / sumSoft * p.gradScale;
-  const auto dense = [&](float v) {
-    float q, c;
+  const F2 fOne2 = makeF2(fOne, fOne), fSoft2 = MODE == kOne ? makeF2(fOne + fSoft, fOne + fSoft) : makeF2(fSoft, fSoft);
+  const auto dense = [&](F2 v) {
+    F2 q, c;
     powers(v, q, c);
-    return MODE == kOne ? (fOne + fSoft) * q : fOne * c + fSoft * q;
+    return MODE == kOne ? mulF2(fSoft2, q) : fmaF2(fOne2, c, mulF2(fSoft2, q));
   };
   for (int j = threadIdx.x; j < nvec; j += kThreads) {
-    float f[8];
-    unpack8(xv[j], f);
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = dense(f[e]);
-    reinterpret_cast<uint4*>(x)[j] = pack8(f);
+    const uint4 raw = xv[j];
+    xv[j] = make_uint4(pack2(dense(unpackF2(raw.x))), pack2(dense(unpackF2(raw.y))), pack2(dense(unpackF2(raw.z))), pack2(dense(unpackF2(raw.w))));
   }
-  for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) x[j] = __float2bfloat16(dense(__bfloat162float(x[j])));
+  const auto denseOne = [&](float v) {
+    float lo, hi;
+    splitF2(dense(makeF2(v, v)), lo, hi);
+    return lo;
+  };
+  for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) x[j] = __float2bfloat16(denseOne(__bfloat162float(x[j])));
   __syncthreads();
   // The teacher's entries and the target once more, from their logits in 32 bits. An id's first entry writes for all of them.
   for (int k = threadIdx.x; k <= p.K; k += kThreads) {
@@ -222,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
         mass += prob[o];
         again = again || o < k;
       }
-    if (!again) x[v - first] = __float2bfloat16(dense(k < p.K ? zAt[k] : zt) - p.gradScale * (a * p.tau * mass + (v == target ? 1.f - p.a : 0.f)));
+    const float at = k < p.K ? zAt[k] : teacher[3];
+    if (!again) x[v - first] = __float2bfloat16(denseOne(at) - p.gradScale * (a * p.tau * mass + (v == target ? 1.f - p.a : 0.f)));
   }
   fenceProxyAsync();
   __syncthreads();
@@ -231,11 +242,25 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
     if (threadIdx.x == 0 && nvec > 0) {
       bulkStore(grad + first, x, nvec * 16);
       tmaStoreCommit();
-      tmaStoreWaitRead0();
     }
   } else {
     for (int j = threadIdx.x; j < n; j += kThreads) grad[first + j] = x[j];
   }
+
+  // ---- the loss, while the gradient leaves
+  if (rank == 0 && threadIdx.x < 32) {
+    const float logSoft = logf(sumSoft);
+    float kl = 0.f;
+    for (int k = lane; k < p.K; k += 32)
+      if (prob[k] != 0.f) kl += prob[k] * ((teacherValue(p, row, k) - teacher[0] - teacher[1]) - ((zAt[k] - m) / p.tau - logSoft));
+    kl = laneSum<32>(kl);
+    if (lane == 0) {
+      float loss = a == 0.f ? 0.f : a * p.tau * p.tau * kl;
+      if (p.a < 1.f) loss += (1.f - p.a) * (m + logf(sumOne) - teacher[3]);
+      p.loss[row] = loss;
+    }
+  }
+  if (threadIdx.x == 0) tmaStoreWaitRead0();
 }
 
 template <Mode MODE> cudaError_t launch(const Args& p, long long T, int ctas, size_t smem, cudaStream_t s) {

@@ -17,6 +17,37 @@ __device__ __forceinline__ float exp2Fast(float x) {
   return y;
 }
 
+// Two fp32 values in a 64-bit register: one instruction for both.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 makeF2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void splitF2(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fmaF2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mulF2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 addF2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 exp2F2(F2 x) {
+  float a, b;
+  splitF2(x, a, b);
+  return makeF2(exp2Fast(a), exp2Fast(b));
+}
+// Two bf16 values of a 32-bit word.
+__device__ __forceinline__ F2 unpackF2(uint32_t w) { return makeF2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
 // Sum / maximum over groups of N consecutive lanes (N a power of two); every lane gets the result.
 template <int N> __device__ __forceinline__ float laneSum(float v) {
 #pragma unroll
@@ -40,6 +71,11 @@ __device__ __forceinline__ void unpack4(const uint2& p, float (&f)[4]) {
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(F2 v) {
+  float a, b;
+  splitF2(v, a, b);
+  return pack2(a, b);
 }
 __device__ __forceinline__ uint2 pack4(const float (&f)[4]) { return make_uint2(pack2(f[0], f[1]), pack2(f[2], f[3])); }
 __device__ __forceinline__ void unpack8(const uint4& p, float (&f)[8]) {
