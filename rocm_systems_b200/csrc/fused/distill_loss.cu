@@ -19,12 +19,13 @@ namespace distill {
 
 using namespace rows;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxEntries = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kSlice = 32768;      // elements of a slice, as long as a cluster of eight can hold the row
+constexpr int kSlice = 16384;      // elements of a slice, as long as a cluster of eight can hold the row
 constexpr int kMaxSlice = 104 * 1024;
-constexpr int kErrLoad = 31;
+constexpr int kErrLoad = 31, kErrMeet = 32;
 
 struct Args {
   const __nv_bfloat16* z;
@@ -43,33 +44,39 @@ struct Args {
 // One: a single exponent (temperature one, or one of the two losses alone). Power: c = q^power. Two: both.
 enum Mode { kOne, kPower, kTwo };
 
-__device__ __forceinline__ float blockReduce(float v, float* sh, bool maximum) {
-  constexpr int kWarps = kThreads / 32;
-  v = maximum ? laneMax<32>(v) : laneSum<32>(v);
-  __syncthreads();
+// Over the block; `sh` (a float per warp) is used once in a kernel.
+__device__ __forceinline__ float blockMax(float v, float* sh) {
+  v = laneMax<32>(v);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = (threadIdx.x & 31) < kWarps ? sh[threadIdx.x & 31] : maximum ? -INFINITY : 0.f;
-  return maximum ? laneMax<32>(v) : laneSum<32>(v);
+  return laneMax<32>(sh[(threadIdx.x & 31) % kWarps]);
+}
+__device__ __forceinline__ float2 blockSum(float2 v, float2* sh) {
+  v.x = laneSum<32>(v.x);
+  v.y = laneSum<32>(v.y);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = (threadIdx.x & 31) < kWarps ? sh[threadIdx.x & 31] : make_float2(0.f, 0.f);
+  return make_float2(laneSum<32>(v.x), laneSum<32>(v.y));
 }
 
 __device__ __forceinline__ float teacherValue(const Args& p, size_t row, int k) {
   return (p.valueBytes == 4 ? reinterpret_cast<const float*>(p.values)[row * p.K + k] : toFloat(reinterpret_cast<const __nv_bfloat16*>(p.values)[row * p.K + k])) / p.tau;
 }
 
-__device__ __forceinline__ void storeCluster(uint32_t clusterAddr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(clusterAddr), "f"(v) : "memory"); }
-
 template <Mode MODE>
-__global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int ctas) {
+__global__ void __launch_bounds__(kThreads, 6) distillKernel(const Args p, int ctas) {
   using namespace sm100;
   extern __shared__ __align__(128) uint8_t smem[];
   __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(smem);
   int* id = reinterpret_cast<int*>(smem + (size_t)p.slice * 2);
   float* prob = reinterpret_cast<float*>(id + p.K);
   float* zAt = prob + p.K;
-  __shared__ float sh[32], meet[3][kMaxCluster];  // of the cluster's CTAs: maximum, sums relative to it
+  __shared__ float tops[kWarps];
+  __shared__ float2 sums[kWarps];
+  __shared__ float4 meet[kMaxCluster];            // of the cluster's CTAs: maximum, sums relative to it
   __shared__ float teacher[4];                    // largest value, logarithm of the sum, 1 if there are entries; the target's logit
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bar, met;
 
   const size_t row = blockIdx.x / ctas;
   const int rank = blockIdx.x % ctas, lane = threadIdx.x & 31;
@@ -79,14 +86,16 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
   const bool bulk = p.zBulk && nvec > 0;
   if (threadIdx.x == 0) {
     mbarInit(&bar, 1);
+    mbarInit(&met, 1);
     fenceBarrierInit();
+    mbarArriveExpectTx(&met, ctas * sizeof(float4));
     if (bulk) {
       mbarArriveExpectTx(&bar, nvec * 16);
       bulkLoad(x, z + first, nvec * 16, &bar);
     }
   }
   __syncthreads();
-  clusterArrive();  // waited for before the first store into another CTA
+  clusterArriveRelaxed();  // waited for before the first store into another CTA
   const long long target = p.targets[row];
   const bool counts = target >= 0 && target < p.V;  // for all CTAs of the cluster alike
   for (int j = (p.zBulk ? nvec * 8 : 0) + threadIdx.x; j < n; j += kThreads) x[j] = z[first + j];
@@ -123,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
   }
   float m = fmaxf(__low2float(top2), __high2float(top2));
   for (int j = nvec * 8 + threadIdx.x; j < n; j += kThreads) m = fmaxf(m, __bfloat162float(x[j]));
-  m = blockReduce(m, sh, true);
+  m = blockMax(m, tops);
 
   if (threadIdx.x < 32) {  // the teacher's softmax, by one warp from shared memory
     float best = -INFINITY, norm = 0.f;
@@ -175,28 +184,23 @@ __global__ void __launch_bounds__(kThreads, 3) distillKernel(const Args p, int c
     partSoft = addF2(partSoft, q);
     partOne = addF2(partOne, c);
   }
-  float sumSoft, sumOne, upper;
+  float sumSoft, sumOne, upper, upperOne;
   splitF2(partSoft, sumSoft, upper);
-  sumSoft = blockReduce(sumSoft + upper, sh, false);
-  splitF2(partOne, sumOne, upper);
-  if (MODE != kOne) sumOne = blockReduce(sumOne + upper, sh, false);
+  splitF2(partOne, sumOne, upperOne);
+  const float2 both = blockSum(make_float2(sumSoft + upper, sumOne + upperOne), sums);
+  // Each CTA tells all of them, and goes on when all have told it: then they have also read the logits that they look up, which the gradient
+  // may be about to take the place of.
   clusterWait();
-  if (threadIdx.x < ctas) {
-    storeCluster(mapToCta(smemAddr(&meet[0][rank]), threadIdx.x), m);
-    storeCluster(mapToCta(smemAddr(&meet[1][rank]), threadIdx.x), sumSoft);
-    storeCluster(mapToCta(smemAddr(&meet[2][rank]), threadIdx.x), sumOne);
-  }
-  __syncthreads();
-  clusterArrive();  // also: no CTA writes its part of the gradient before every CTA has read the logits that it looks up
-  clusterWait();
+  if (threadIdx.x < ctas) storeAsync4(mapToCta(smemAddr(&meet[rank]), threadIdx.x), m, both.x, both.y, 0.f, mapToCta(smemAddr(&met), threadIdx.x));
+  mbarWait(&met, 0, p.err, kErrMeet);
   m = -INFINITY;
-  for (int r = 0; r < ctas; r++) m = fmaxf(m, meet[0][r]);
+  for (int r = 0; r < ctas; r++) m = fmaxf(m, meet[r].x);
   sumSoft = sumOne = 0.f;
   for (int r = 0; r < ctas; r++) {
-    const float d = meet[0][r] - m;
-    if (meet[1][r] == 0.f) continue;  // nothing but minus infinity in this slice
-    sumSoft += meet[1][r] * exp2Fast(d * soft);
-    sumOne += meet[2][r] * exp2Fast(d * one);
+    const float d = meet[r].x - m;
+    if (meet[r].y == 0.f) continue;  // nothing but minus infinity in this slice
+    sumSoft += meet[r].y * exp2Fast(d * soft);
+    sumOne += meet[r].z * exp2Fast(d * one);
   }
   if (MODE == kOne) sumOne = sumSoft;
   relativeTo(m);

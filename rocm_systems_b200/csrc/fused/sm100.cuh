@@ -212,6 +212,14 @@ __device__ __forceinline__ uint32_t mapToCta(uint32_t smemByteAddr, uint32_t ran
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smemByteAddr), "r"(rank));
   return r;
 }
+// The same arrival without the wait for this thread's earlier writes: for a barrier that hands no data over.
+__device__ __forceinline__ void clusterArriveRelaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+// Four fp32 values into another CTA's shared memory (16-byte aligned), counted in bytes on a barrier of that CTA.
+__device__ __forceinline__ void storeAsync4(uint32_t clusterAddr, float a, float b, float c, float d, uint32_t barClusterAddr) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(clusterAddr), "f"(a), "f"(b), "f"(c), "f"(d),
+               "r"(barClusterAddr)
+               : "memory");
+}
 __device__ __forceinline__ void clusterArrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void clusterWait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Arrive on a barrier of any CTA of the cluster. What it orders are tensor-memory accesses, through the tcgen05 fences on both sides,
