@@ -447,8 +447,11 @@ c10::intrusive_ptr<c10d::Backend> createBackend(const c10::intrusive_ptr<c10d::S
 
 }  // namespace
 
+void bindStudentOps(py::module_& m);  // student_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "c10d backend of the b200coll collective library";
+  m.doc() = "c10d backend of the b200coll collective library, and operators with autograd";
+  bindStudentOps(m);
   m.def("create_backend", &createBackend, py::arg("store"), py::arg("rank"), py::arg("size"), py::arg("timeout"));
   m.def("comm_handle", [](const c10::intrusive_ptr<c10d::Backend>& b) -> int64_t { return b->getID(); });
 }

@@ -6,9 +6,7 @@ library raises at import of :mod:`rocm_systems_b200._lib`.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -35,7 +33,6 @@ def _lib_ops():
         lib.b200ops_swiglu_fwd.argtypes = [vp, vp, ll, i32, vp]
         lib.b200ops_swiglu_bwd.argtypes = [vp, vp, vp, ll, i32, vp]
         lib.b200ops_cross_entropy.argtypes = [vp, vp, vp, ll, i32, ll, f32, vp]
-        lib.b200ops_distill_loss.argtypes = [vp, vp, vp, vp, i32, vp, i32, vp, ll, i32, i32, ll, ll, f32, f32, f32, vp]
         lib.b200ops_adamw.argtypes = [vp, vp, vp, vp, vp, ll, f32, f32, f32, f32, f32, i32, f32, vp]
         lib.b200ops_embedding_fwd.argtypes = [vp, vp, vp, ll, i32, vp]
         lib.b200ops_embedding_bwd.argtypes = [vp, vp, vp, ll, i32, vp]
@@ -49,14 +46,6 @@ def _lib_ops():
 
 def _s() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-
-
-_here = contextlib.nullcontext()
-
-
-def _on(t: torch.Tensor):
-    """The device of ``t`` made current, if it is not: kernels are launched on that device's current stream."""
-    return _here if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _ck(rc: int, what: str) -> None:
@@ -201,30 +190,9 @@ def distill_loss(logits: torch.Tensor, targets: torch.Tensor, teacher_ids: torch
     one id add up; an entry whose id is outside [0, V) counts nothing, and a row without entries has no second term. A row whose target is
     outside [0, V) (padding) has zero loss and zero gradient. The gradient, times ``grad_scale``, goes to ``grad`` (``logits`` itself: in
     place), by default a new tensor."""
-    assert logits.dim() == 2 and logits.dtype == torch.bfloat16 and logits.stride(1) == 1, "logits: [T, V] in bf16 with dense rows"
-    T, V = logits.shape
-    assert V > 0 and (logits.stride(0) >= V or T <= 1), "logits: rows that do not overlap"
-    assert targets.shape == (T,) and targets.dtype == torch.int64 and targets.is_contiguous(), "targets: contiguous int64 [T]"
-    assert teacher_ids.dim() == 2 and teacher_ids.shape == teacher_logits.shape and teacher_ids.shape[0] == T, "teacher_ids and teacher_logits: [T, K]"
-    K = teacher_ids.shape[1]
-    assert V <= 851968, "a vocabulary of up to 851,968"
-    assert 1 <= K <= 1024, "1 to 1024 teacher entries per row"
-    assert teacher_ids.dtype in (torch.int64, torch.int32) and teacher_logits.dtype in (torch.float32, torch.bfloat16), "int64 or int32 ids, fp32 or bf16 logits"
-    assert 0.0 <= weight <= 1.0 and 0.0 < temperature < math.inf and math.isfinite(grad_scale), "0 <= weight <= 1, temperature above 0"
-    if grad is None:
-        grad = torch.empty(T, V, dtype=torch.bfloat16, device=logits.device)
-    assert grad.shape == (T, V) and grad.dtype == torch.bfloat16 and grad.stride(1) == 1 and (grad.stride(0) >= V or T <= 1), "grad: like logits"
-    if T > 0 and (grad.data_ptr(), grad.stride(0) if T > 1 else V) != (logits.data_ptr(), logits.stride(0) if T > 1 else V):
-        ends = [(t.data_ptr(), t.data_ptr() + 2 * ((T - 1) * t.stride(0) + V)) for t in (logits, grad)]
-        assert ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0], "grad: logits itself, or memory apart from it"
-    assert logits.is_cuda and all(t.device == logits.device for t in (targets, teacher_ids, teacher_logits, grad)), "tensors on one CUDA device expected"
-    ids, values = teacher_ids.contiguous(), teacher_logits.contiguous()
-    loss = torch.empty(T, dtype=torch.float32, device=logits.device)
-    with _on(logits):
-        _ck(_lib_ops().b200ops_distill_loss(logits.data_ptr(), grad.data_ptr(), targets.data_ptr(), ids.data_ptr(), ids.element_size(), values.data_ptr(),
-                                            values.element_size(), loss.data_ptr(), T, V, K, max(logits.stride(0), V), max(grad.stride(0), V), weight, temperature,
-                                            grad_scale, _s()), "distill_loss")
-    return loss, grad
+    from .attention import _ext  # this module is the first to be loaded
+
+    return _ext().distill_loss(logits, targets, teacher_ids, teacher_logits, weight, temperature, grad_scale, grad)
 
 
 def adamw_(master, m, v, grad, param, lr, betas, eps, weight_decay, step, grad_scale=1.0) -> None:

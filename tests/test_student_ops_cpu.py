@@ -7,6 +7,13 @@ import student_oracle as oracle
 bf = torch.bfloat16
 
 
+@pytest.fixture(scope="module", autouse=True)
+def _extension_built():
+    from rocm_systems_b200.utils import build
+
+    build.build_torch_ext()
+
+
 def _qkv(**over):
     a = dict(B=2, S=8, heads=4, kv=2, D=64, dtype=bf)
     a |= over
@@ -34,6 +41,7 @@ def _w(D=64, dtype=bf):
     ("bf16 or fp32", (_qkv(), _w(dtype=torch.float16), _w(dtype=torch.float16), _table(), 4, 2)),
     ("at least S", (_qkv(), _w(), _w(), _table(7), 4, 2)),
     ("contiguous fp32", (_qkv(), _w(), _w(), _table().to(torch.float64), 4, 2)),
+    ("eps", (_qkv(), _w(), _w(), _table(), 4, 2, float("nan"))),
     ("CUDA device", (_qkv(), _w(), _w(), _table(), 4, 2)),
 ])
 def test_qk_norm_rope_refuses(why, args):
@@ -108,10 +116,16 @@ def test_c_entries_refuse_what_they_cannot_run():
     """The exported symbols check their numbers before anything is launched."""
     import ctypes
 
-    from rocm_systems_b200.ops import attention, train_ops
+    from rocm_systems_b200 import _lib
 
     invalid = 1
-    lib = attention._lib_attn()
+    lib = _lib.load()
+    vp, ll, i32, f32 = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
+    lib.b200ops_qk_norm_rope_fwd.argtypes = [vp, vp, vp, i32, vp, vp, vp, ll] + [i32] * 4 + [f32, vp]
+    lib.b200ops_qk_norm_rope_bwd.argtypes = [vp] * 7 + [i32] + [vp] * 5 + [ll] + [i32] * 4 + [f32, vp]
+    lib.b200ops_window_attention_fwd.argtypes = [vp] * 8 + [i32] * 7 + [f32, vp]
+    lib.b200ops_window_attention_bwd.argtypes = [vp] * 13 + [i32] * 7 + [f32, vp]
+    lib.b200ops_distill_loss.argtypes = [vp, vp, vp, vp, i32, vp, i32, vp, ll, i32, i32, ll, ll, f32, f32, f32, vp]
     none = (ctypes.c_longlong * 24)()
     p = 4096  # an address that nothing reads: every call below is refused
     fwd = lambda B=1, H=2, KV=1, S=4, D=64, w=0, si=0, q=p: lib.b200ops_window_attention_fwd(q, p, p, p, None, None, None, none, B, H, KV, S, D, w, si, 1.0, None)
@@ -125,8 +139,7 @@ def test_c_entries_refuse_what_they_cannot_run():
     for seq, heads, kv, D in ((0, 4, 2, 64), (8, 0, 2, 64), (8, 4, 0, 64), (8, 4, 2, 12), (8, 4, 2, 512)):
         assert lib.b200ops_qk_norm_rope_fwd(p, p, p, 1, p, p, p, 8, seq, heads, kv, D, 1e-5, None) == invalid
         assert lib.b200ops_qk_norm_rope_bwd(p, p, p, none, p, p, p, 1, p, p, p, p, p, 8, seq, heads, kv, D, 1e-5, None) == invalid
-    t = train_ops._lib_ops()
-    loss = lambda T=4, V=64, K=3, st=64, gst=64, ib=8, vb=4, tau=1.0: t.b200ops_distill_loss(p, p, p, p, ib, p, vb, p, T, V, K, st, gst, 1.0, tau, 1.0, None)
+    loss = lambda T=4, V=64, K=3, st=64, gst=64, ib=8, vb=4, tau=1.0: lib.b200ops_distill_loss(p, p, p, p, ib, p, vb, p, T, V, K, st, gst, 1.0, tau, 1.0, None)
     for bad in ({"T": -1}, {"V": 0}, {"V": 851969, "st": 851976, "gst": 851976}, {"K": 0}, {"K": 1025}, {"st": 63}, {"gst": 8}, {"ib": 2}, {"vb": 8}, {"tau": 0.0}, {"tau": float("nan")}):
         assert loss(**bad) == invalid, bad
 
