@@ -18,8 +18,9 @@ struct Tensor {
 struct Args {
   Tensor q, k, v, out, dout, dq, dk, dv;
   Tensor rest;         // what rounding took from out (bf16), kept for the backward pass, or nullptr
-  float* lse;          // [batch, heads, padded()]: log2 of the sum of exp over a row's visible scores, infinity for a row behind the sequence's end
-  float* delta;        // the same shape: sum of dout * out over a row (backward)
+  // [batch, heads, padded()], both with the sign that they are added with:
+  float* lse;          // minus log2 of the sum of exp over a row's visible scores, minus infinity for a row behind the sequence's end
+  float* delta;        // minus the sum of dout * out over a row (backward)
   const int* lengths;  // [batch] or nullptr
   int B, H, KV, S, D;
   int window, sinks;   // window >= 1 (S or more: everything)

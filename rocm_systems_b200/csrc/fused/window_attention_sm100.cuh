@@ -10,6 +10,8 @@
 // below 2^kSlack, which costs no precision in bf16 and fp32, and O is hardly ever touched in between.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_sm100.cuh"
 #include "rows.cuh"
 #include "window_attention.h"
@@ -22,6 +24,8 @@ using namespace rows;
 constexpr int kTile = 128;  // queries and keys of a tile
 constexpr uint32_t kBox = kTile * 128;  // bytes of a TMA box: 128 rows of 64 elements
 constexpr float kSlack = 8.f;
+constexpr int kPolyFwd = 4;  // of a row's pairs of powers of two, one in so many is a polynomial
+constexpr int kPolyBwd = 2;
 
 enum ErrCode : int { ERR_FWD_LOAD = 21, ERR_FWD_MMA, ERR_FWD_SOFTMAX, ERR_BWD_LOAD, ERR_BWD_MMA, ERR_BWD_MATH };
 
@@ -66,14 +70,29 @@ template <int HD> struct FwdCfg {
   static constexpr uint32_t kTmemCols = 512;
 };
 
-// Zeroes rows [from, kTile) of a tile in shared memory; all lanes of a warp. Then the tensor cores may read it.
-template <int BOXES> __device__ __forceinline__ void zeroRows(uint8_t* tile, int from, int lane) {
-  for (int n = from * 8 + lane; n < kTile * 8; n += 32)
+// The rows of a tile that lie behind the sequence's end, zeroed in shared memory before the tensor cores sum over them: the issuing warp
+// asks (barrier 0), a warp that does nothing else zeroes and answers (barrier 1).
+struct Clearing {
+  uint64_t* bars;
+  uint32_t phase = 0;
+  __device__ bool request(int lane, volatile int* err, int code) {
+    if (lane == 0) sm100::mbarArrive(&bars[0]);
+    const bool ok = sm100::mbarWait(&bars[1], phase, err, code);
+    phase ^= 1;
+    return __all_sync(0xffffffffu, ok);
+  }
+  template <int BOXES> __device__ bool serve(uint8_t* tile, int from, int lane, volatile int* err, int code) {
+    if (!sm100::mbarWait(&bars[0], phase, err, code)) return false;
+    phase ^= 1;
+    for (int n = from * 8 + lane; n < kTile * 8; n += 32)
 #pragma unroll
-    for (int x = 0; x < BOXES; x++) *reinterpret_cast<uint4*>(tile + x * kBox + n * 16) = make_uint4(0, 0, 0, 0);
-  sm100::fenceProxyAsync();
-  __syncwarp();
-}
+      for (int x = 0; x < BOXES; x++) *reinterpret_cast<uint4*>(tile + x * kBox + n * 16) = make_uint4(0, 0, 0, 0);
+    sm100::fenceProxyAsync();
+    __syncwarp();
+    if (lane == 0) sm100::mbarArrive(&bars[1]);
+    return true;
+  }
+};
 
 // Rows [row0, row0 + 128) of a head to zeros, from warps 0-3 or 4-7.
 __device__ __forceinline__ void zeroOut(const Tensor& t, int b, int h, int row0, int S, int D, int tid) {
@@ -98,10 +117,11 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   uint64_t* sFull = empty + C::kSlots;    // [2] scores in tensor memory
   uint64_t* pReady = sFull + 2;           // [2] weights in their place, O scaled
   uint64_t* oDone = pReady + 2;           // [2] O complete
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(oDone + 2);
+  uint64_t* clear = oDone + 2;            // [2] see Clearing
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(clear + 2);
 
   const Args& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the compiler is to know that it is a warp's)
   volatile int* err = p.err;
   const int heads = a.B * a.H, bh = blockIdx.x % heads, h = bh % a.H, b = bh / a.H, kh = h / a.group();
   const int r0 = (p.tiles - 1 - (int)(blockIdx.x / heads)) * 2 * kTile;  // the longest rows first
@@ -116,6 +136,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   const int nSinks = min(own[0].sinkTiles, own[0].first), count = nSinks + own[1].last - own[0].first + 1;
   const auto tileOf = [&](int n) { return n < nSinks ? n : own[0].first + n - nSinks; };
   const auto active = [&](int t, int n) { return (t == 0 || two) && own[t].has(tileOf(n)); };
+  const auto straddles = [&](int n) { return L - tileOf(n) * kTile < kTile; };
 
   if (threadIdx.x == 0) {
     prefetchTensorMap(&p.q);
@@ -126,6 +147,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       mbarInit(&sFull[t], 1);
       mbarInit(&pReady[t], 4);
       mbarInit(&oDone[t], 1);
+      mbarInit(&clear[t], 1);
     }
     for (int s = 0; s < C::kSlots; s++) {
       mbarInit(&full[s], 1);
@@ -140,7 +162,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
-  const uint32_t tmem = *tmemSlot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmemSlot, 0);
 
   if (warp == 8) {
     setMaxRegsDown<C::kOtherRegs>();
@@ -165,60 +187,73 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   } else if (warp == 9) {
     setMaxRegsDown<C::kOtherRegs>();
     constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescO = instrDescMajor(kTile, HD, 1, 0, 1);
+    // The whole warp walks along and one elected lane issues: what the instructions take from uniform registers is then formed there. (With
+    // `lane == 0` in the place of the election each cost 100 cycles to issue, and runs 64.)
     const auto slot = [&](int n) { return n % C::kSlots; };
-    const auto wait = [&](int n) { return mbarWait(&full[slot(n)], (n / C::kSlots) & 1, err, ERR_FWD_MMA); };
+    const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbarWait(bar, parity, err, ERR_FWD_MMA)); };
+    const auto landed = [&](int n) { return wait(&full[slot(n)], (n / C::kSlots) & 1); };
+    const uint64_t descQ = smemDescSw128(smemAddr(smemQ)), descK = smemDescSw128(smemAddr(ring)), descV = smemDescSw128Mn(smemAddr(ring), kBox);
     const auto scores = [&](int t, int n) {
-      if (lane == 0) {
-        const uint32_t q = smemAddr(smemQ + t * C::kQBytes), k = smemAddr(ring + slot(2 * n) * C::kTileBytes);
+      if (electOne()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; kk++) {
           const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
-          mmaF16(tmem + C::kTmemS + t * kTile, smemDescSw128(q + o), smemDescSw128(k + o), idescS, kk != 0);
+          mmaF16(tmem + C::kTmemS + t * kTile, descQ + ((t * C::kQBytes + o) >> 4), descK + ((slot(2 * n) * C::kTileBytes + o) >> 4), idescS, kk != 0);
         }
         mmaCommit(&sFull[t]);
       }
+      __syncwarp();
     };
+    const auto release = [&](int n) {
+      if (electOne()) mmaCommit(&empty[slot(n)]);
+      __syncwarp();
+    };
+    Clearing clearing{clear};
     bool ok = true, started[2] = {false, false};
     uint32_t phase[2] = {0, 0};
-    for (int t = 0; t < 1 + two && ok; t++) ok = mbarWait(&qFull[t], 0, err, ERR_FWD_MMA);
-    ok = ok && wait(0);
+    for (int t = 0; t < 1 + two && ok; t++) ok = wait(&qFull[t], 0);
+    ok = ok && landed(0);
     if (ok) {
       for (int t = 0; t < 2; t++)
         if (active(t, 0)) scores(t, 0);
-      if (lane == 0) mmaCommit(&empty[slot(0)]);
+      release(0);
     }
     for (int n = 0; n < count && ok; n++) {
-      if (!(ok = wait(2 * n + 1))) break;
-      uint8_t* vTile = ring + slot(2 * n + 1) * C::kTileBytes;
-      const int beyond = L - tileOf(n) * kTile;
-      if (beyond < kTile) zeroRows<C::kBoxes>(vTile, beyond, lane);  // a weight of zero does not silence what lies behind the sequence's end
-      for (int t = 0; t < 2 && ok; t++) {
+      if (!(ok = landed(2 * n + 1))) break;
+      // A weight of zero does not silence what lies behind the sequence's end.
+      if (straddles(n) && !(ok = clearing.request(lane, err, ERR_FWD_MMA))) break;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        if (!ok) break;
         if (active(t, n)) {
-          if (!(ok = mbarWait(&pReady[t], phase[t], err, ERR_FWD_MMA))) break;
+          if (!(ok = wait(&pReady[t], phase[t]))) break;
           phase[t] ^= 1;
           tcFenceAfter();
-          if (lane == 0) {
-            const uint32_t v = smemAddr(vTile);
+          if (electOne()) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; kk++)
-              mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + kk * 8, smemDescSw128Mn(v + kk * 2048, kBox), idescO, started[t] || kk != 0);
+              mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + kk * 8, descV + ((slot(2 * n + 1) * C::kTileBytes + kk * 2048) >> 4), idescO,
+                             started[t] || kk != 0);
             if (tileOf(n) == own[t].last) mmaCommit(&oDone[t]);
           }
+          __syncwarp();
           started[t] = true;
         }
         if (n + 1 < count && active(t, n + 1)) {
-          if (!(ok = wait(2 * n + 2))) break;
+          if (!(ok = landed(2 * n + 2))) break;
           scores(t, n + 1);
         }
       }
       if (!ok) break;
-      if (lane == 0) {
-        mmaCommit(&empty[slot(2 * n + 1)]);
-        if (n + 1 < count) mmaCommit(&empty[slot(2 * n + 2)]);
-      }
-      __syncwarp();
+      release(2 * n + 1);
+      if (n + 1 < count) release(2 * n + 2);
     }
-  } else if (warp >= 10) {
+  } else if (warp == 10) {
+    setMaxRegsDown<C::kOtherRegs>();
+    Clearing clearing{clear};
+    for (int n = 0; n < count; n++)
+      if (straddles(n) && !clearing.serve<C::kBoxes>(ring + (2 * n + 1) % C::kSlots * C::kTileBytes, L - tileOf(n) * kTile, lane, err, ERR_FWD_MMA)) break;
+  } else if (warp == 11) {
     setMaxRegsDown<C::kOtherRegs>();
   } else {
     setMaxRegsUp<C::kMathRegs>();
@@ -240,7 +275,8 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 #pragma unroll
       for (int x = 0; x < 4; x++) tmemLoad32(tS + x * 32, s[x]);
       tmemLoadWait();
-      if (!seesAll(a, r0 + t * kTile, rLast, j0)) {
+      const bool every = seesAll(a, r0 + t * kTile, rLast, j0);
+      if (!every) {
 #pragma unroll
         for (int x = 0; x < 4; x++) {
           const uint32_t bits = maskBits(a, row, j0 + x * 32);
@@ -249,11 +285,15 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
             if (!((bits >> e) & 1)) s[x][e] = 0xff800000u;  // -inf
         }
       }
-      float top = -INFINITY;
+      float best[4];
 #pragma unroll
-      for (int x = 0; x < 4; x++)
+      for (int x = 0; x < 4; x++) {
+        best[x] = __uint_as_float(s[x][0]);
 #pragma unroll
-        for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(s[x][e]));
+        for (int e = 1; e < 31; e += 2) best[x] = fmaxf(fmaxf(best[x], __uint_as_float(s[x][e])), __uint_as_float(s[x][e + 1]));
+        best[x] = fmaxf(best[x], __uint_as_float(s[x][31]));
+      }
+      const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
       const bool move = top > -INFINITY && (m == -INFINITY || (top - m) * p.c > kSlack);
       const float f = move ? exp2Fast((m - top) * p.c) : 1.f;
       if (move) {
@@ -273,17 +313,28 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       }
       any = true;
       const float off = m == -INFINITY ? 0.f : m * p.c;
+      const F2 c2 = makeF2(p.c, p.c), off2 = makeF2(-off, -off);
+      F2 sum[4] = {makeF2(l, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f)};
+      const auto weights = [&](auto polynomials) {
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
-        uint32_t w[16];
+        for (int x = 0; x < 4; x++) {
+          uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float p0 = exp2Fast(fmaf(__uint_as_float(s[x][2 * e]), p.c, -off)), p1 = exp2Fast(fmaf(__uint_as_float(s[x][2 * e + 1]), p.c, -off));
-          l += p0 + p1;
-          w[e] = pack2(p0, p1);
+          for (int e = 0; e < 16; e++) {
+            const F2 v = fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2);
+            const F2 pr = decltype(polynomials)::value && e % kPolyFwd == kPolyFwd - 1 ? exp2Poly(v) : exp2F2(v);
+            sum[e & 3] = addF2(sum[e & 3], pr);
+            w[e] = pack2(pr);
+          }
+          tmemStore16(tS + x * 16, w);
         }
-        tmemStore16(tS + x * 16, w);
-      }
+      };
+      // Masked scores have to become zeros, which the polynomial does not give.
+      if (every) weights(std::true_type{});
+      else weights(std::false_type{});
+      float upper;
+      splitF2(addF2(addF2(sum[0], sum[1]), addF2(sum[2], sum[3])), l, upper);
+      l += upper;
       tmemStoreWait();
       tcFenceBefore();
       __syncwarp();
@@ -293,7 +344,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     if (ok) {
       tcFenceAfter();
       const bool live = row < L;
-      if (a.lse) a.lse[(size_t)bh * a.padded() + row] = live ? m * p.c + log2f(l) : INFINITY;
+      if (a.lse) a.lse[(size_t)bh * a.padded() + row] = live ? -(m * p.c + log2f(l)) : -INFINITY;
       const float inv = 1.f / l;
       uint8_t* stage = smemQ + t * C::kQBytes + q4 * 32 * 256;
       const auto rowsOf = [&](const Tensor& dst) {
@@ -377,13 +428,13 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
   float* half = stats + 4 * kTile;          // queries: [2][128] halves of delta
   uint64_t* bars = reinterpret_cast<uint64_t*>(half + 2 * kTile);
   uint64_t *xFull = bars, *full = bars + 1, *empty = bars + 5, *sFull = bars + 9 /*[2]*/, *dpFull = bars + 11, *pReady = bars + 12, *dsReady = bars + 13,
-           *statFull = bars + 14 /*[2]*/, *statEmpty = bars + 16 /*[2]*/, *done = bars + 18;
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 19);
+           *statFull = bars + 14 /*[2]*/, *statEmpty = bars + 16 /*[2]*/, *done = bars + 18, *clear = bars + 19 /*[2]*/;
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 21);
   // tensor memory: queries S0, S1, dP, dQ; keys S, dP, dV, dK
   constexpr uint32_t kS = 0, kDp = SIDE == kQueries ? 256 : 128, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
 
   const Args& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the compiler is to know that it is a warp's)
   volatile int* err = p.err;
 
   // ---- what this CTA does: rows [x0, x0 + 128) of head xh against tiles [yFirst, yFirst + yTiles) (queries: keys, sinks first) of `group` heads from yh on
@@ -423,6 +474,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
     if constexpr (SIDE == kQueries) return n < sinkTiles ? n : yFirst + n - sinkTiles;
     else return yFirst + n % yTiles;
   };
+  const auto straddles = [&](int n) { return L - tileOf(n) * kTile < kTile; };
   const auto headOf = [&](int n) { return SIDE == kQueries ? yh : yh + n / yTiles; };
   const bool sinkRows = SIDE == kKeys && xTile < p.sinkTiles;  // some rows' sums go through `partials`
   const int partRows = sinkRows ? min(kTile, a.sinks - x0) : 0, partPitch = min(a.sinks, kTile);
@@ -455,6 +507,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       mbarInit(&sFull[s], 1);
       mbarInit(&statFull[s], 1);
       mbarInit(&statEmpty[s], 8);
+      mbarInit(&clear[s], 1);
     }
     mbarInit(dpFull, 1);
     mbarInit(pReady, 8);
@@ -469,7 +522,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
-  const uint32_t tmem = *tmemSlot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmemSlot, 0);
   const auto slot1 = [](int n) { return 2 * (n & 1) + ((n >> 1) & 1); };
   const auto slot2 = [](int n) { return 2 * (n & 1) + 1 - ((n >> 1) & 1); };
 
@@ -507,32 +560,30 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
   } else if (warp == 9) {
     setMaxRegsDown<C::kOtherRegs>();
     constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescAcc = instrDescMajor(kTile, HD, 1, 0, 1);
-    const auto wait = [&](int s, int n) { return mbarWait(&full[s], (n >> 1) & 1, err, ERR_BWD_MMA); };
+    // As in the forward kernel the whole warp walks along and one elected lane issues.
+    Clearing clearing{clear};
+    const auto waitFor = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbarWait(bar, parity, err, ERR_BWD_MMA)); };
     // Rows behind the sequence's end are zeroed where they are summed over: a weight of zero does not silence what may lie there.
-    const auto clear = [&](int s, int n) {
-      const int beyond = L - tileOf(n) * kTile;
-      if (beyond < kTile) zeroRows<C::kBoxes>(ring + s * C::kTileBytes, beyond, lane);
+    const auto landed = [&](int s, int n, bool summed) {
+      return waitFor(&full[s], (n >> 1) & 1) && (!summed || !straddles(n) || clearing.request(lane, err, ERR_BWD_MMA));
     };
+    const uint64_t descX = smemDescSw128(smemAddr(smemX)), descY = smemDescSw128(smemAddr(ring)), descSum = smemDescSw128Mn(smemAddr(ring), kBox);
     const auto product = [&](uint32_t d, int x, int s) {  // d = X Y^T
-      const uint32_t xa = smemAddr(smemX + x * C::kTileBytes), ya = smemAddr(ring + s * C::kTileBytes);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; kk++) {
         const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
-        mmaF16(tmem + d, smemDescSw128(xa + o), smemDescSw128(ya + o), idescS, kk != 0);
+        mmaF16(tmem + d, descX + ((x * C::kTileBytes + o) >> 4), descY + ((s * C::kTileBytes + o) >> 4), idescS, kk != 0);
       }
     };
     const auto gather = [&](uint32_t acc, uint32_t w, int s, bool first) {  // acc += W Y, W: two halves of 64 columns, each packed into 32
-      const uint32_t ya = smemAddr(ring + s * C::kTileBytes);
 #pragma unroll
       for (int kk = 0; kk < kTile / 16; kk++)
-        mmaF16FromTmem(tmem + acc, tmem + w + (kk / 4) * 64 + (kk % 4) * 8, smemDescSw128Mn(ya + kk * 2048, kBox), idescAcc, !first || kk != 0);
+        mmaF16FromTmem(tmem + acc, tmem + w + (kk / 4) * 64 + (kk % 4) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
     };
-    bool ok = mbarWait(xFull, 0, err, ERR_BWD_MMA);
     const auto scores = [&](int n) {
-      if (!wait(slot1(n), n)) return false;
-      clear(slot1(n), n);
-      if (lane == 0) {
-        const int buf = SIDE == kQueries ? n & 1 : 0;
+      if (!landed(slot1(n), n, true)) return false;
+      const int buf = SIDE == kQueries ? n & 1 : 0;
+      if (electOne()) {
         product(kS + buf * kTile, 0, slot1(n));
         mmaCommit(&sFull[buf]);
       }
@@ -540,9 +591,8 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       return true;
     };
     const auto grads = [&](int n) {
-      if (!wait(slot2(n), n)) return false;
-      if (SIDE == kKeys) clear(slot2(n), n);
-      if (lane == 0) {
+      if (!landed(slot2(n), n, SIDE == kKeys)) return false;
+      if (electOne()) {
         product(kDp, 1, slot2(n));
         mmaCommit(dpFull);
         if (SIDE == kQueries) mmaCommit(&empty[slot2(n)]);
@@ -550,22 +600,22 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       __syncwarp();
       return true;
     };
-    ok = ok && scores(0) && grads(0);
+    bool ok = waitFor(xFull, 0) && scores(0) && grads(0);
     if (SIDE == kQueries && count > 1) ok = ok && scores(1);
     for (int n = 0; n < count && ok; n++) {
       if constexpr (SIDE == kKeys) {
-        if (!(ok = mbarWait(pReady, n & 1, err, ERR_BWD_MMA))) break;
+        if (!(ok = waitFor(pReady, n & 1))) break;
         tcFenceAfter();
-        if (lane == 0) {
+        if (electOne()) {
           gather(kAcc1, kS, slot2(n), n == 0);
           mmaCommit(&empty[slot2(n)]);
         }
         __syncwarp();
         if (n + 1 < count && !(ok = scores(n + 1))) break;
       }
-      if (!(ok = mbarWait(dsReady, n & 1, err, ERR_BWD_MMA))) break;
+      if (!(ok = waitFor(dsReady, n & 1))) break;
       tcFenceAfter();
-      if (lane == 0) {
+      if (electOne()) {
         gather(SIDE == kQueries ? kAcc1 : kAcc2, kDp, slot1(n), n == 0);
         mmaCommit(&empty[slot1(n)]);
         if (n + 1 == count) mmaCommit(done);
@@ -574,7 +624,16 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       if (n + 1 < count && !(ok = grads(n + 1))) break;
       if (SIDE == kQueries && n + 2 < count && !(ok = scores(n + 2))) break;
     }
-  } else if (warp >= 10) {
+  } else if (warp == 10) {
+    setMaxRegsDown<C::kOtherRegs>();
+    Clearing clearing{clear};
+    bool ok = true;
+    for (int n = 0; n < count && ok; n++) {
+      if (!straddles(n)) continue;
+      ok = clearing.serve<C::kBoxes>(ring + slot1(n) * C::kTileBytes, L - tileOf(n) * kTile, lane, err, ERR_BWD_MMA);
+      if (SIDE == kKeys) ok = ok && clearing.serve<C::kBoxes>(ring + slot2(n) * C::kTileBytes, L - tileOf(n) * kTile, lane, err, ERR_BWD_MMA);
+    }
+  } else if (warp == 11) {
     setMaxRegsDown<C::kOtherRegs>();
   } else {
     setMaxRegsUp<C::kMathRegs>();
@@ -600,7 +659,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       half[side * kTile + r] = delta;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       delta = half[r] + half[kTile + r];
-      if (side == 0) a.delta[(size_t)bh * a.padded() + row] = delta;
+      if (side == 0) a.delta[(size_t)bh * a.padded() + row] = -delta;
     }
     bool ok = true;
     for (int n = 0; n < count && ok; n++) {
@@ -625,25 +684,44 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
           }
         }
       }
-      float w[64];
-      {
+      F2 w[32];  // the weights
+      const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
+      const ulonglong2* lse2 = reinterpret_cast<const ulonglong2*>(st);
+      const ulonglong2* delta2 = reinterpret_cast<const ulonglong2*>(st + kTile);
+      const auto masked = [&](F2 v, int e) {  // pair e of this thread's 32
+        float lo, hi;
+        splitF2(v, lo, hi);
+        const uint32_t b = bits[e / 16] >> (2 * e % 32);
+        return makeF2(b & 1 ? lo : 0.f, b & 2 ? hi : 0.f);
+      };
+      const auto weights = [&](auto all) {
         uint32_t s[2][32];
         tmemLoad32(base + kS + buf * kTile + cols, s[0]);
         tmemLoad32(base + kS + buf * kTile + cols + 32, s[1]);
         tmemLoadWait();
 #pragma unroll
-        for (int e = 0; e < 64; e++) {
-          const float off = SIDE == kQueries ? lse : st[e];
-          const float v = exp2Fast(fmaf(__uint_as_float(s[e / 32][e % 32]), p.c, -off));
-          w[e] = (bits[e / 32] >> (e % 32)) & 1 ? v : 0.f;
+        for (int e = 0; e < 32; e += 2) {
+          ulonglong2 off = make_ulonglong2(rowLse, rowLse);
+          if (SIDE == kKeys) off = lse2[e / 2];
+          const F2 v0 = fmaF2(makeF2(__uint_as_float(s[e / 16][2 * e % 32]), __uint_as_float(s[e / 16][2 * e % 32 + 1])), c2, off.x);
+          const F2 v1 = fmaF2(makeF2(__uint_as_float(s[e / 16][2 * e % 32 + 2]), __uint_as_float(s[e / 16][2 * e % 32 + 3])), c2, off.y);
+          if constexpr (decltype(all)::value) {
+            w[e] = exp2F2(v0);
+            w[e + 1] = e / 2 % (kPolyBwd / 2) == 0 ? exp2Poly(v1) : exp2F2(v1);
+          } else {
+            w[e] = masked(exp2F2(v0), e);
+            w[e + 1] = masked(exp2F2(v1), e + 1);
+          }
         }
-      }
+      };
+      if (every) weights(std::true_type{});
+      else weights(std::false_type{});
       if constexpr (SIDE == kKeys) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
           uint32_t o[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 32 + 2 * e], w[x * 32 + 2 * e + 1]);
+          for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
           tmemStore16(base + kS + cols + x * 16, o);
         }
         tmemStoreWait();
@@ -653,7 +731,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       }
       if (!(ok = mbarWait(dpFull, n & 1, err, ERR_BWD_MATH))) break;
       tcFenceAfter();
-      {
+      const auto gradients = [&](auto all) {
         uint32_t d[2][32];
         tmemLoad32(base + kDp + cols, d[0]);
         tmemLoad32(base + kDp + cols + 32, d[1]);
@@ -662,19 +740,22 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
         for (int x = 0; x < 2; x++) {
           uint32_t o[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
-            float v[2];
+          for (int e = 0; e < 16; e += 2) {
+            ulonglong2 off = make_ulonglong2(rowDelta, rowDelta);
+            if (SIDE == kKeys) off = delta2[x * 8 + e / 2];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-              const int i = x * 32 + 2 * e + k;
-              v[k] = w[i] * (__uint_as_float(d[x][2 * e + k]) - (SIDE == kQueries ? delta : st[kTile + i]));
-              if (!((bits[x] >> (2 * e + k)) & 1)) v[k] = 0.f;  // what is masked may be anything
+              const int i = x * 16 + e + k;
+              F2 v = mulF2(w[i], addF2(makeF2(__uint_as_float(d[x][2 * (e + k)]), __uint_as_float(d[x][2 * (e + k) + 1])), k ? off.y : off.x));
+              if (!decltype(all)::value) v = masked(v, i);  // what is masked may be anything
+              o[e + k] = pack2(v);
             }
-            o[e] = pack2(v[0], v[1]);
           }
           tmemStore16(base + kDp + cols + x * 16, o);
         }
-      }
+      };
+      if (every) gradients(std::true_type{});
+      else gradients(std::false_type{});
       tmemStoreWait();
       tcFenceBefore();
       __syncwarp();
