@@ -132,10 +132,10 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     return;
   }
   const bool two = r0 + kTile < L;
-  const KeyRange own[2] = {KeyRange(a, r0, min(r0 + kTile, L) - 1), KeyRange(a, two ? r0 + kTile : r0, min(r0 + 2 * kTile, L) - 1)};
-  const int nSinks = min(own[0].sinkTiles, own[0].first), count = nSinks + own[1].last - own[0].first + 1;
-  const auto tileOf = [&](int n) { return n < nSinks ? n : own[0].first + n - nSinks; };
-  const auto active = [&](int t, int n) { return (t == 0 || two) && own[t].has(tileOf(n)); };
+  const KeyRange own0(a, r0, min(r0 + kTile, L) - 1), own1(a, two ? r0 + kTile : r0, min(r0 + 2 * kTile, L) - 1);
+  const int nSinks = min(own0.sinkTiles, own0.first), count = nSinks + own1.last - own0.first + 1;
+  const auto tileOf = [&](int n) { return n < nSinks ? n : own0.first + n - nSinks; };
+  const auto active = [&](int t, int n) { return t == 0 ? own0.has(tileOf(n)) : two && own1.has(tileOf(n)); };
   const auto straddles = [&](int n) { return L - tileOf(n) * kTile < kTile; };
 
   if (threadIdx.x == 0) {
@@ -193,60 +193,53 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbarWait(bar, parity, err, ERR_FWD_MMA)); };
     const auto landed = [&](int n) { return wait(&full[slot(n)], (n / C::kSlots) & 1); };
     const uint64_t descQ = smemDescSw128(smemAddr(smemQ)), descK = smemDescSw128(smemAddr(ring)), descV = smemDescSw128Mn(smemAddr(ring), kBox);
-    const auto scores = [&](int t, int n) {
-      if (electOne()) {
+    const auto scores = [&](int t, int n) {  // by the elected lane
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; kk++) {
-          const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
-          mmaF16(tmem + C::kTmemS + t * kTile, descQ + ((t * C::kQBytes + o) >> 4), descK + ((slot(2 * n) * C::kTileBytes + o) >> 4), idescS, kk != 0);
-        }
-        mmaCommit(&sFull[t]);
+      for (int kk = 0; kk < HD / 16; kk++) {
+        const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
+        mmaF16(tmem + C::kTmemS + t * kTile, descQ + ((t * C::kQBytes + o) >> 4), descK + ((slot(2 * n) * C::kTileBytes + o) >> 4), idescS, kk != 0);
       }
-      __syncwarp();
-    };
-    const auto release = [&](int n) {
-      if (electOne()) mmaCommit(&empty[slot(n)]);
-      __syncwarp();
+      mmaCommit(&sFull[t]);
     };
     Clearing clearing{clear};
-    bool ok = true, started[2] = {false, false};
+    bool ok = wait(&qFull[0], 0) && (!two || wait(&qFull[1], 0)) && landed(0), started[2] = {false, false};
     uint32_t phase[2] = {0, 0};
-    for (int t = 0; t < 1 + two && ok; t++) ok = wait(&qFull[t], 0);
-    ok = ok && landed(0);
-    if (ok) {
-      for (int t = 0; t < 2; t++)
-        if (active(t, 0)) scores(t, 0);
-      release(0);
+    if (ok && electOne()) {
+      scores(0, 0);
+      if (active(1, 0)) scores(1, 0);
+      mmaCommit(&empty[slot(0)]);
     }
+    __syncwarp();
     for (int n = 0; n < count && ok; n++) {
-      if (!(ok = landed(2 * n + 1))) break;
+      const bool more = n + 1 < count;
+      if (!(ok = landed(2 * n + 1) && (!more || landed(2 * n + 2)))) break;
       // A weight of zero does not silence what lies behind the sequence's end.
       if (straddles(n) && !(ok = clearing.request(lane, err, ERR_FWD_MMA))) break;
 #pragma unroll
       for (int t = 0; t < 2; t++) {
-        if (!ok) break;
-        if (active(t, n)) {
+        const bool now = active(t, n), next = more && active(t, n + 1);
+        if (now) {
           if (!(ok = wait(&pReady[t], phase[t]))) break;
           phase[t] ^= 1;
           tcFenceAfter();
-          if (electOne()) {
+        }
+        if (electOne()) {
+          if (now) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; kk++)
               mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + kk * 8, descV + ((slot(2 * n + 1) * C::kTileBytes + kk * 2048) >> 4), idescO,
                              started[t] || kk != 0);
-            if (tileOf(n) == own[t].last) mmaCommit(&oDone[t]);
+            if (tileOf(n) == (t ? own1.last : own0.last)) mmaCommit(&oDone[t]);
           }
-          __syncwarp();
-          started[t] = true;
+          if (next) scores(t, n + 1);
+          if (t == 1) {
+            mmaCommit(&empty[slot(2 * n + 1)]);
+            if (more) mmaCommit(&empty[slot(2 * n + 2)]);
+          }
         }
-        if (n + 1 < count && active(t, n + 1)) {
-          if (!(ok = landed(2 * n + 2))) break;
-          scores(t, n + 1);
-        }
+        __syncwarp();
+        started[t] = started[t] || now;
       }
-      if (!ok) break;
-      release(2 * n + 1);
-      if (n + 1 < count) release(2 * n + 2);
     }
   } else if (warp == 10) {
     setMaxRegsDown<C::kOtherRegs>();
@@ -259,23 +252,26 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     setMaxRegsUp<C::kMathRegs>();
     const int t = warp >> 2, q4 = warp & 3;
     const int row = r0 + t * kTile + q4 * 32 + lane;
-    const int rLast = min(r0 + (t + 1) * kTile, L) - 1;
+    const int rFirst = r0 + t * kTile, rLast = min(rFirst + kTile, L) - 1;
+    const int mySinks = t ? own1.sinkTiles : own0.sinkTiles, myFirst = t ? own1.first : own0.first, myLast = t ? own1.last : own0.last;
     const uint32_t laneBase = (uint32_t)(q4 * 32) << 16;
     const uint32_t tS = tmem + laneBase + C::kTmemS + t * kTile, tO = tmem + laneBase + C::kTmemO + t * HD;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, limit = -INFINITY, l = 0.f;
+    const float slack = kSlack / p.c;
     uint32_t phase = 0;
     bool ok = t == 0 || two, any = false;
     for (int n = 0; n < count && ok; n++) {
-      if (!active(t, n)) continue;
+      const int tile = tileOf(n);
+      if (tile > myLast || (tile < myFirst && tile >= mySinks)) continue;
       if (!(ok = mbarWait(&sFull[t], phase, err, ERR_FWD_SOFTMAX))) break;
       phase ^= 1;
       tcFenceAfter();
-      const int j0 = tileOf(n) * kTile;
+      const int j0 = tile * kTile;
+      const bool every = seesAll(a, rFirst, rLast, j0);
       uint32_t s[4][32];
 #pragma unroll
       for (int x = 0; x < 4; x++) tmemLoad32(tS + x * 32, s[x]);
       tmemLoadWait();
-      const bool every = seesAll(a, r0 + t * kTile, rLast, j0);
       if (!every) {
 #pragma unroll
         for (int x = 0; x < 4; x++) {
@@ -294,10 +290,11 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         best[x] = fmaxf(best[x], __uint_as_float(s[x][31]));
       }
       const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-      const bool move = top > -INFINITY && (m == -INFINITY || (top - m) * p.c > kSlack);
+      const bool move = top > limit;
       const float f = move ? exp2Fast((m - top) * p.c) : 1.f;
       if (move) {
         m = top;
+        limit = top + slack;
         l *= f;
       }
       if (any && __any_sync(0xffffffffu, move)) {
