@@ -111,6 +111,23 @@ __device__ __forceinline__ void unpack8(const uint4& p, float (&f)[8]) {
 }
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) { return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7])); }
 
+// 16 packed words (32 bf16 values) of a row to global memory: in 32-byte pieces where `wide` (the address is on a 32-byte boundary), whole
+// sectors although every lane of a warp has a row of its own, else in 16-byte pieces; `words` of them exist (a multiple of 4, and of 8 where wide).
+__device__ __forceinline__ void storeRow16(__nv_bfloat16* dst, const uint32_t (&w)[16], int words, bool wide) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    if (wide) {
+      if (i < words)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                     "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                     : "memory");
+    } else {
+      if (i < words) *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      if (i + 4 < words) *reinterpret_cast<uint4*>(dst + 2 * i + 8) = make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]);
+    }
+  }
+}
+
 __device__ __forceinline__ float toFloat(float x) { return x; }
 __device__ __forceinline__ float toFloat(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void store(float* p, float x) { *p = x; }

@@ -14,6 +14,7 @@ static bool good(const Args& a) {
   return a.B > 0 && a.H > 0 && a.KV > 0 && a.H % a.KV == 0 && a.S > 0 && a.D >= 8 && a.D <= 128 && a.D % 8 == 0 && a.window > 0 && a.sinks >= 0 && a.scale >= 0.f &&
          (long long)a.B * a.H * a.S <= 0x3fffffffffLL;
 }
+static bool wide(const Tensor& t) { return ((uintptr_t)t.p & 31) == 0 && t.b % 16 == 0 && t.h % 16 == 0 && t.s % 16 == 0; }
 static Tensor packed(const void* p, const Args& a) { return {(const __nv_bfloat16*)p, (long long)a.S * a.H * a.D, a.D, (long long)a.H * a.D}; }
 static bool aligned(const Tensor& t) { return t.p && ((uintptr_t)t.p & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.s % 8 == 0; }
 
@@ -56,12 +57,14 @@ template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
   p.tiles = (a.S + 2 * kTile - 1) / (2 * kTile);
   p.err = gemm::errWord();
   if (!p.err) return cudaErrorMemoryAllocation;
-  const long long ctas = (long long)p.tiles * a.B * a.H;
-  if (ctas > 0x7fffffffLL || !headMap(&p.q, a.q, a.B, a.H, a.S, a.D) || !headMap(&p.k, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.v, a.v, a.B, a.KV, a.S, a.D))
+  p.items = (long long)p.tiles * a.B * a.H;
+  p.wide = wide(a.out) && (!a.rest.p || wide(a.rest)) && a.D % 16 == 0;
+  const int ctas = (int)(p.items < gemm::smCount() ? p.items : gemm::smCount());  // one per SM
+  if (p.items > 0x7fffffffLL || !headMap(&p.q, a.q, a.B, a.H, a.S, a.D) || !headMap(&p.k, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.v, a.v, a.B, a.KV, a.S, a.D))
     return cudaErrorInvalidValue;
   const cudaError_t e = allowSmem(forwardKernel<HD>, FwdCfg<HD>::kSmem, done);
   if (e != cudaSuccess) return e;
-  forwardKernel<HD><<<(unsigned)ctas, FwdCfg<HD>::kThreads, FwdCfg<HD>::kSmem, s>>>(p);
+  forwardKernel<HD><<<ctas, FwdCfg<HD>::kThreads, FwdCfg<HD>::kSmem, s>>>(p);
   return cudaGetLastError();
 }
 

@@ -1,10 +1,10 @@
-// Windowed attention on the 5th-generation tensor cores: the forward pass.
+// Windowed attention on the 5th-generation tensor cores.
 //
-// A CTA owns two tiles of 128 queries of one head and walks the 128-key tiles that either of them sees (the sinks', then the window's). Warp
-// 8 feeds queries once and keys and values through a ring of TMA tiles; one thread of warp 9 issues S = Q K^T into tensor memory and, once
+// Forward: a persistent CTA takes pairs of 128-query tiles of a head and walks the 128-key tiles that either of them sees (the sinks', then
+// the window's). Warp 8 feeds queries, and keys and values through a ring of TMA tiles; warp 9 issues S = Q K^T into tensor memory and, once
 // the softmax is through with it, O += P V with P read from tensor memory as well; warps 0-3 and 4-7 are the two tiles' softmax, one
 // thread per row, so that row maxima and sums need no exchange. P (bf16) takes the place of the scores it was made of. While one tile's
-// softmax runs, the tensor cores work for the other.
+// softmax runs, the tensor cores work for the other; while a pair's answer is written, the next pair's first scores are made.
 //
 // The running maximum is moved, and O in tensor memory scaled down, only when a row's maximum has grown by more than 2^kSlack: weights stay
 // below 2^kSlack, which costs no precision in bf16 and fp32, and O is hardly ever touched in between.
@@ -34,6 +34,8 @@ struct FwdParams {
   Args a;
   float c;              // scores' factor in powers of two, never zero
   int tiles;            // pairs of query tiles
+  long long items;      // pairs of all heads
+  bool wide;            // rows of out and rest start on 32-byte boundaries and are whole 32-byte pieces
   int* err;
 };
 
@@ -61,14 +63,16 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
 template <int HD> struct FwdCfg {
   static constexpr int kThreads = 384;                   // launched with 168 registers each, split as 2 x 128 x 216 and 128 x 64
   static constexpr int kMathRegs = 216, kOtherRegs = 64;
-  static constexpr int kSlots = 4;                       // key and value tiles in turn
+  static constexpr int kSlots = HD == 128 ? 5 : 8;       // key and value tiles in turn
   static constexpr int kBoxes = HD / 64;
   static constexpr uint32_t kTileBytes = kBoxes * kBox;
-  static constexpr uint32_t kQBytes = 4 * 32 * 256;      // a query tile, later the staging buffers of its four warps
-  static constexpr size_t kSmem = 1024 + 2 * kQBytes + kSlots * kTileBytes + 256;
+  static constexpr size_t kSmem = 1024 + (2 + kSlots) * kTileBytes + 256;
   static constexpr uint32_t kTmemS = 0, kTmemO = 256;    // columns: S0, S1 (128 each), O0, O1 (HD each)
   static constexpr uint32_t kTmemCols = 512;
 };
+
+// What a persistent CTA does in its turn `k`: items are sorted by falling cost, so every other turn goes through the CTAs backwards.
+__device__ __forceinline__ long long itemOf(int k) { return (long long)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
 
 // The rows of a tile that lie behind the sequence's end, zeroed in shared memory before the tensor cores sum over them: the issuing warp
 // asks (barrier 0), a warp that does nothing else zeroes and answers (barrier 1).
@@ -109,44 +113,33 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   uint8_t* smemQ = smem;
-  uint8_t* ring = smem + 2 * C::kQBytes;
+  uint8_t* ring = smem + 2 * C::kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kTileBytes);
-  uint64_t* qFull = bars;                 // [2]
+  uint64_t *qFull = bars, *qEmpty = bars + 1;
   uint64_t* full = bars + 2;              // [kSlots]
   uint64_t* empty = full + C::kSlots;     // [kSlots]
   uint64_t* sFull = empty + C::kSlots;    // [2] scores in tensor memory
   uint64_t* pReady = sFull + 2;           // [2] weights in their place, O scaled
   uint64_t* oDone = pReady + 2;           // [2] O complete
-  uint64_t* clear = oDone + 2;            // [2] see Clearing
+  uint64_t* oFree = oDone + 2;            // [2] O read
+  uint64_t* clear = oFree + 2;            // [2] see Clearing
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(clear + 2);
 
   const Args& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the compiler is to know that it is a warp's)
   volatile int* err = p.err;
-  const int heads = a.B * a.H, bh = blockIdx.x % heads, h = bh % a.H, b = bh / a.H, kh = h / a.group();
-  const int r0 = (p.tiles - 1 - (int)(blockIdx.x / heads)) * 2 * kTile;  // the longest rows first
-  const int L = lengthOf(a, b);
-  if (r0 >= L) {
-    if (warp < 8) zeroOut(a.out, b, h, r0 + (warp >> 2) * kTile, a.S, a.D, threadIdx.x & 127);
-    if (warp < 8 && a.rest.p) zeroOut(a.rest, b, h, r0 + (warp >> 2) * kTile, a.S, a.D, threadIdx.x & 127);
-    return;
-  }
-  const bool two = r0 + kTile < L;
-  const KeyRange own0(a, r0, min(r0 + kTile, L) - 1), own1(a, two ? r0 + kTile : r0, min(r0 + 2 * kTile, L) - 1);
-  const int nSinks = min(own0.sinkTiles, own0.first), count = nSinks + own1.last - own0.first + 1;
-  const auto tileOf = [&](int n) { return n < nSinks ? n : own0.first + n - nSinks; };
-  const auto active = [&](int t, int n) { return t == 0 ? own0.has(tileOf(n)) : two && own1.has(tileOf(n)); };
-  const auto straddles = [&](int n) { return L - tileOf(n) * kTile < kTile; };
 
   if (threadIdx.x == 0) {
     prefetchTensorMap(&p.q);
     prefetchTensorMap(&p.k);
     prefetchTensorMap(&p.v);
+    mbarInit(qFull, 1);
+    mbarInit(qEmpty, 1);
     for (int t = 0; t < 2; t++) {
-      mbarInit(&qFull[t], 1);
       mbarInit(&sFull[t], 1);
       mbarInit(&pReady[t], 4);
       mbarInit(&oDone[t], 1);
+      mbarInit(&oFree[t], 4);
       mbarInit(&clear[t], 1);
     }
     for (int s = 0; s < C::kSlots; s++) {
@@ -164,23 +157,56 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   tcFenceAfter();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmemSlot, 0);
 
+  // A pair of query tiles of one head and its key tiles.
+  struct Item {
+    int h, b, kh, r0, L, count, nSinks;
+    bool two;
+    KeyRange own0, own1;
+    __device__ Item(const FwdParams& p, long long item) : own0(p.a, 0, 0), own1(p.a, 0, 0) {
+      const Args& a = p.a;
+      const int heads = a.B * a.H, bh = (int)(item % heads);
+      h = bh % a.H;
+      b = bh / a.H;
+      kh = h / a.group();
+      r0 = (p.tiles - 1 - (int)(item / heads)) * 2 * kTile;  // the longest rows first
+      L = lengthOf(a, b);
+      count = nSinks = 0;
+      two = r0 + kTile < L;
+      if (r0 >= L) return;
+      own0 = KeyRange(a, r0, min(r0 + kTile, L) - 1);
+      own1 = KeyRange(a, two ? r0 + kTile : r0, min(r0 + 2 * kTile, L) - 1);
+      nSinks = min(own0.sinkTiles, own0.first);
+      count = nSinks + own1.last - own0.first + 1;
+    }
+    __device__ int tileOf(int n) const { return n < nSinks ? n : own0.first + n - nSinks; }
+    __device__ bool active(int t, int n) const { return t == 0 ? own0.has(tileOf(n)) : two && own1.has(tileOf(n)); }
+    __device__ bool straddles(int n) const { return L - tileOf(n) * kTile < kTile; }
+  };
+
   if (warp == 8) {
     setMaxRegsDown<C::kOtherRegs>();
     if (lane == 0) {
-      for (int t = 0; t < 1 + two; t++) {
-        mbarArriveExpectTx(&qFull[t], C::kTileBytes);
-        for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(smemQ + t * C::kQBytes + x * kBox, &p.q, x * 64, r0 + t * kTile, h, b, &qFull[t]);
-      }
       bool ok = true;
-      for (int n = 0; n < 2 * count && ok; n++) {
-        const int s = n % C::kSlots;
-        ok = mbarWait(&empty[s], ((n / C::kSlots) & 1) ^ 1, err, ERR_FWD_LOAD);
-        if (!ok) break;
-        mbarArriveExpectTx(&full[s], C::kTileBytes);
-        for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * kBox, n & 1 ? &p.v : &p.k, x * 64, tileOf(n >> 1) * kTile, kh, b, &full[s]);
+      int slot = 0;
+      uint32_t turn = 1, qTurn = 1;
+      for (int k = 0; ok && itemOf(k) < p.items; k++) {
+        const Item it(p, itemOf(k));
+        if (it.count == 0) continue;
+        if (!(ok = mbarWait(qEmpty, qTurn, err, ERR_FWD_LOAD))) break;
+        qTurn ^= 1;
+        mbarArriveExpectTx(qFull, (1 + it.two) * C::kTileBytes);
+        for (int t = 0; t < 1 + it.two; t++)
+          for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(smemQ + t * C::kTileBytes + x * kBox, &p.q, x * 64, it.r0 + t * kTile, it.h, it.b, qFull);
+        for (int n = 0; n < 2 * it.count; n++) {
+          if (!(ok = mbarWait(&empty[slot], turn, err, ERR_FWD_LOAD))) break;
+          mbarArriveExpectTx(&full[slot], C::kTileBytes);
+          for (int x = 0; x < C::kBoxes; x++)
+            tmaLoad4d(ring + slot * C::kTileBytes + x * kBox, n & 1 ? &p.v : &p.k, x * 64, it.tileOf(n >> 1) * kTile, it.kh, it.b, &full[slot]);
+          if (++slot == C::kSlots) slot = 0, turn ^= 1;
+        }
       }
       if (!ok) {  // let loads in flight land
-        for (int t = 0; t < 1 + two; t++) mbarWait(&qFull[t], 0, err, 0, 2000u);
+        mbarWait(qFull, 0, err, 0, 2000u);
         for (int s = 0; s < C::kSlots; s++) mbarWait(&full[s], 0, err, 0, 2000u);
       }
     }
@@ -189,186 +215,220 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescO = instrDescMajor(kTile, HD, 1, 0, 1);
     // The whole warp walks along and one elected lane issues: what the instructions take from uniform registers is then formed there. (With
     // `lane == 0` in the place of the election each cost 100 cycles to issue, and runs 64.)
-    const auto slot = [&](int n) { return n % C::kSlots; };
     const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbarWait(bar, parity, err, ERR_FWD_MMA)); };
-    const auto landed = [&](int n) { return wait(&full[slot(n)], (n / C::kSlots) & 1); };
     const uint64_t descQ = smemDescSw128(smemAddr(smemQ)), descK = smemDescSw128(smemAddr(ring)), descV = smemDescSw128Mn(smemAddr(ring), kBox);
-    const auto scores = [&](int t, int n) {  // by the elected lane
+    Clearing clearing{clear};
+    bool ok = true;
+    uint32_t qPhase = 0, pPhase[2] = {0, 0}, oTurn[2] = {1, 1}, landedPhase = 0;
+    int landedSlot = 0;  // of the next tile to land
+    const auto landed = [&]() {
+      const bool r = wait(&full[landedSlot], landedPhase);
+      if (++landedSlot == C::kSlots) landedSlot = 0, landedPhase ^= 1;
+      return r;
+    };
+    const auto after = [](int s) { return s + 1 == C::kSlots ? 0 : s + 1; };
+    const auto scores = [&](int t, int slot) {  // by the elected lane
 #pragma unroll
       for (int kk = 0; kk < HD / 16; kk++) {
         const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
-        mmaF16(tmem + C::kTmemS + t * kTile, descQ + ((t * C::kQBytes + o) >> 4), descK + ((slot(2 * n) * C::kTileBytes + o) >> 4), idescS, kk != 0);
+        mmaF16(tmem + C::kTmemS + t * kTile, descQ + ((t * C::kTileBytes + o) >> 4), descK + ((slot * C::kTileBytes + o) >> 4), idescS, kk != 0);
       }
       mmaCommit(&sFull[t]);
     };
-    Clearing clearing{clear};
-    bool ok = wait(&qFull[0], 0) && (!two || wait(&qFull[1], 0)) && landed(0), started[2] = {false, false};
-    uint32_t phase[2] = {0, 0};
-    if (ok && electOne()) {
-      scores(0, 0);
-      if (active(1, 0)) scores(1, 0);
-      mmaCommit(&empty[slot(0)]);
-    }
-    __syncwarp();
-    for (int n = 0; n < count && ok; n++) {
-      const bool more = n + 1 < count;
-      if (!(ok = landed(2 * n + 1) && (!more || landed(2 * n + 2)))) break;
-      // A weight of zero does not silence what lies behind the sequence's end.
-      if (straddles(n) && !(ok = clearing.request(lane, err, ERR_FWD_MMA))) break;
+    for (int k = 0; ok && itemOf(k) < p.items; k++) {
+      const Item it(p, itemOf(k));
+      if (it.count == 0) continue;
+      int slotK = landedSlot;
+      if (!(ok = wait(qFull, qPhase) && landed())) break;
+      qPhase ^= 1;
+      if (electOne()) {
+        scores(0, slotK);
+        if (it.active(1, 0)) scores(1, slotK);
+        mmaCommit(&empty[slotK]);
+        if (it.count == 1) mmaCommit(qEmpty);
+      }
+      __syncwarp();
+      bool started[2] = {false, false};
+      for (int n = 0; n < it.count && ok; n++) {
+        const bool more = n + 1 < it.count;
+        const int slotV = after(slotK), slotNext = after(slotV);
+        if (!(ok = landed() && (!more || landed()))) break;
+        // A weight of zero does not silence what lies behind the sequence's end.
+        if (it.straddles(n) && !(ok = clearing.request(lane, err, ERR_FWD_MMA))) break;
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const bool now = active(t, n), next = more && active(t, n + 1);
-        if (now) {
-          if (!(ok = wait(&pReady[t], phase[t]))) break;
-          phase[t] ^= 1;
-          tcFenceAfter();
-        }
-        if (electOne()) {
+        for (int t = 0; t < 2; t++) {
+          const bool now = it.active(t, n), next = more && it.active(t, n + 1), last = it.tileOf(n) == (t ? it.own1.last : it.own0.last);
           if (now) {
+            if (!started[t]) {
+              if (!(ok = wait(&oFree[t], oTurn[t]))) break;
+              oTurn[t] ^= 1;
+            }
+            if (!(ok = wait(&pReady[t], pPhase[t]))) break;
+            pPhase[t] ^= 1;
+            tcFenceAfter();
+          }
+          if (electOne()) {
+            if (now) {
 #pragma unroll
-            for (int kk = 0; kk < kTile / 16; kk++)
-              mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + kk * 8, descV + ((slot(2 * n + 1) * C::kTileBytes + kk * 2048) >> 4), idescO,
-                             started[t] || kk != 0);
-            if (tileOf(n) == (t ? own1.last : own0.last)) mmaCommit(&oDone[t]);
+              for (int kk = 0; kk < kTile / 16; kk++)
+                mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + kk * 8, descV + ((slotV * C::kTileBytes + kk * 2048) >> 4), idescO,
+                               started[t] || kk != 0);
+              if (last) mmaCommit(&oDone[t]);
+            }
+            if (t == 1) mmaCommit(&empty[slotV]);
+            if (next) scores(t, slotNext);
+            if (t == 1 && more) {
+              mmaCommit(&empty[slotNext]);
+              if (n + 2 == it.count) mmaCommit(qEmpty);
+            }
           }
-          if (next) scores(t, n + 1);
-          if (t == 1) {
-            mmaCommit(&empty[slot(2 * n + 1)]);
-            if (more) mmaCommit(&empty[slot(2 * n + 2)]);
-          }
+          __syncwarp();
+          started[t] = started[t] || now;
         }
-        __syncwarp();
-        started[t] = started[t] || now;
+        slotK = slotNext;
       }
     }
   } else if (warp == 10) {
     setMaxRegsDown<C::kOtherRegs>();
     Clearing clearing{clear};
-    for (int n = 0; n < count; n++)
-      if (straddles(n) && !clearing.serve<C::kBoxes>(ring + (2 * n + 1) % C::kSlots * C::kTileBytes, L - tileOf(n) * kTile, lane, err, ERR_FWD_MMA)) break;
+    int tiles = 0;  // that went through the ring before this item
+    bool ok = true;
+    for (int k = 0; ok && itemOf(k) < p.items; k++) {
+      const Item it(p, itemOf(k));
+      for (int n = 0; n < it.count && ok; n++)
+        if (it.straddles(n))
+          ok = clearing.serve<C::kBoxes>(ring + (tiles + 2 * n + 1) % C::kSlots * C::kTileBytes, it.L - it.tileOf(n) * kTile, lane, err, ERR_FWD_MMA);
+      tiles = (tiles + 2 * it.count) % C::kSlots;
+    }
   } else if (warp == 11) {
     setMaxRegsDown<C::kOtherRegs>();
   } else {
     setMaxRegsUp<C::kMathRegs>();
-    const int t = warp >> 2, q4 = warp & 3;
-    const int row = r0 + t * kTile + q4 * 32 + lane;
-    const int rFirst = r0 + t * kTile, rLast = min(rFirst + kTile, L) - 1;
-    const int mySinks = t ? own1.sinkTiles : own0.sinkTiles, myFirst = t ? own1.first : own0.first, myLast = t ? own1.last : own0.last;
+    const int t = warp >> 2, q4 = warp & 3, r = t * kTile + q4 * 32 + lane;
     const uint32_t laneBase = (uint32_t)(q4 * 32) << 16;
     const uint32_t tS = tmem + laneBase + C::kTmemS + t * kTile, tO = tmem + laneBase + C::kTmemO + t * HD;
-    float m = -INFINITY, limit = -INFINITY, l = 0.f;
     const float slack = kSlack / p.c;
-    uint32_t phase = 0;
-    bool ok = t == 0 || two, any = false;
-    for (int n = 0; n < count && ok; n++) {
-      const int tile = tileOf(n);
-      if (tile > myLast || (tile < myFirst && tile >= mySinks)) continue;
-      if (!(ok = mbarWait(&sFull[t], phase, err, ERR_FWD_SOFTMAX))) break;
-      phase ^= 1;
-      tcFenceAfter();
-      const int j0 = tile * kTile;
-      const bool every = seesAll(a, rFirst, rLast, j0);
-      uint32_t s[4][32];
-#pragma unroll
-      for (int x = 0; x < 4; x++) tmemLoad32(tS + x * 32, s[x]);
-      tmemLoadWait();
-      if (!every) {
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-          const uint32_t bits = maskBits(a, row, j0 + x * 32);
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (!((bits >> e) & 1)) s[x][e] = 0xff800000u;  // -inf
-        }
+    uint32_t sPhase = 0, oPhase = 0;
+    bool ok = true;
+    for (int k = 0; ok && itemOf(k) < p.items; k++) {
+      const Item it(p, itemOf(k));
+      const int rFirst = it.r0 + t * kTile, row = it.r0 + r, rLast = min(rFirst + kTile, it.L) - 1;
+      if (rFirst >= it.L) {
+        zeroOut(a.out, it.b, it.h, rFirst, a.S, a.D, threadIdx.x & 127);
+        if (a.rest.p) zeroOut(a.rest, it.b, it.h, rFirst, a.S, a.D, threadIdx.x & 127);
+        continue;
       }
-      float best[4];
+      const KeyRange mine = t ? it.own1 : it.own0;
+      float m = -INFINITY, limit = -INFINITY, l = 0.f;
+      bool any = false;
+      for (int n = 0; n < it.count; n++) {
+        const int tile = it.tileOf(n);
+        if (!mine.has(tile)) continue;
+        if (!(ok = mbarWait(&sFull[t], sPhase, err, ERR_FWD_SOFTMAX))) break;
+        sPhase ^= 1;
+        tcFenceAfter();
+        const int j0 = tile * kTile;
+        const bool every = seesAll(a, rFirst, rLast, j0);
+        uint32_t s[4][32];
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
-        best[x] = __uint_as_float(s[x][0]);
-#pragma unroll
-        for (int e = 1; e < 31; e += 2) best[x] = fmaxf(fmaxf(best[x], __uint_as_float(s[x][e])), __uint_as_float(s[x][e + 1]));
-        best[x] = fmaxf(best[x], __uint_as_float(s[x][31]));
-      }
-      const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-      const bool move = top > limit;
-      const float f = move ? exp2Fast((m - top) * p.c) : 1.f;
-      if (move) {
-        m = top;
-        limit = top + slack;
-        l *= f;
-      }
-      if (any && __any_sync(0xffffffffu, move)) {
-#pragma unroll 1
-        for (int x = 0; x < HD / 16; x++) {
-          uint32_t o[16];
-          tmemLoad16(tO + x * 16, o);
-          tmemLoadWait();
-#pragma unroll
-          for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmemStore16(tO + x * 16, o);
-        }
-      }
-      any = true;
-      const float off = m == -INFINITY ? 0.f : m * p.c;
-      const F2 c2 = makeF2(p.c, p.c), off2 = makeF2(-off, -off);
-      F2 sum[4] = {makeF2(l, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f)};
-      const auto weights = [&](auto polynomials) {
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const F2 v = fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2);
-            const F2 pr = decltype(polynomials)::value && e % kPolyFwd == kPolyFwd - 1 ? exp2Poly(v) : exp2F2(v);
-            sum[e & 3] = addF2(sum[e & 3], pr);
-            w[e] = pack2(pr);
-          }
-          tmemStore16(tS + x * 16, w);
-        }
-      };
-      // Masked scores have to become zeros, which the polynomial does not give.
-      if (every) weights(std::true_type{});
-      else weights(std::false_type{});
-      float upper;
-      splitF2(addF2(addF2(sum[0], sum[1]), addF2(sum[2], sum[3])), l, upper);
-      l += upper;
-      tmemStoreWait();
-      tcFenceBefore();
-      __syncwarp();
-      if (lane == 0) mbarArrive(&pReady[t]);
-    }
-    ok = ok && any && mbarWait(&oDone[t], 0, err, ERR_FWD_SOFTMAX);
-    if (ok) {
-      tcFenceAfter();
-      const bool live = row < L;
-      if (a.lse) a.lse[(size_t)bh * a.padded() + row] = live ? -(m * p.c + log2f(l)) : -INFINITY;
-      const float inv = 1.f / l;
-      uint8_t* stage = smemQ + t * C::kQBytes + q4 * 32 * 256;
-      const auto rowsOf = [&](const Tensor& dst) {
-        return [&](int r) -> __nv_bfloat16* { return row - lane + r < a.S ? dst.at(b, h, row - lane + r) : nullptr; };
-      };
-      const auto load = [&](int x, uint32_t(&acc)[32]) {
-        tmemLoad32(tO + x * 32, acc);
+        for (int x = 0; x < 4; x++) tmemLoad32(tS + x * 32, s[x]);
         tmemLoadWait();
+        if (!every) {
 #pragma unroll
-        for (int e = 0; e < 32; e++) acc[e] = live ? __float_as_uint(__uint_as_float(acc[e]) * inv) : 0u;
-      };
-      gemm::drainStaged(stage, lane, HD, a.D, load, rowsOf(a.out));
-      if (a.rest.p)
-        gemm::drainStaged(
-            stage, lane, HD, a.D,
-            [&](int x, uint32_t(&acc)[32]) {
-              load(x, acc);
+          for (int x = 0; x < 4; x++) {
+            const uint32_t bits = maskBits(a, row, j0 + x * 32);
 #pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const float v = __uint_as_float(acc[e]);
-                acc[e] = __float_as_uint(v - __bfloat162float(__float2bfloat16(v)));
-              }
-            },
-            rowsOf(a.rest));
-    } else if (t == 1 && !two) {
-      zeroOut(a.out, b, h, r0 + kTile, a.S, a.D, threadIdx.x & 127);
-      if (a.rest.p) zeroOut(a.rest, b, h, r0 + kTile, a.S, a.D, threadIdx.x & 127);
+            for (int e = 0; e < 32; e++)
+              if (!((bits >> e) & 1)) s[x][e] = 0xff800000u;  // -inf
+          }
+        }
+        float best[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          best[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) best[x] = fmaxf(fmaxf(best[x], __uint_as_float(s[x][e])), __uint_as_float(s[x][e + 1]));
+          best[x] = fmaxf(best[x], __uint_as_float(s[x][31]));
+        }
+        const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+        const bool move = top > limit;
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? exp2Fast((m - top) * p.c) : 1.f;
+          if (move) {
+            m = top;
+            limit = top + slack;
+            l *= f;
+          }
+          if (any) {
+#pragma unroll 1
+            for (int x = 0; x < HD / 16; x++) {
+              uint32_t o[16];
+              tmemLoad16(tO + x * 16, o);
+              tmemLoadWait();
+#pragma unroll
+              for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmemStore16(tO + x * 16, o);
+            }
+          }
+        }
+        any = true;
+        const float off = m == -INFINITY ? 0.f : m * p.c;
+        const F2 c2 = makeF2(p.c, p.c), off2 = makeF2(-off, -off);
+        F2 sum[4] = {makeF2(l, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f)};
+        const auto weights = [&](auto polynomials) {
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const F2 v = fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2);
+              const F2 pr = decltype(polynomials)::value && e % kPolyFwd == kPolyFwd - 1 ? exp2Poly(v) : exp2F2(v);
+              sum[e & 3] = addF2(sum[e & 3], pr);
+              w[e] = pack2(pr);
+            }
+            tmemStore16(tS + x * 16, w);
+          }
+        };
+        // Masked scores have to become zeros, which the polynomial does not give.
+        if (every) weights(std::true_type{});
+        else weights(std::false_type{});
+        tmemStoreWait();
+        tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArrive(&pReady[t]);
+        float upper;
+        splitF2(addF2(addF2(sum[0], sum[1]), addF2(sum[2], sum[3])), l, upper);
+        l += upper;
+      }
+      if (!ok || !(ok = mbarWait(&oDone[t], oPhase, err, ERR_FWD_SOFTMAX))) break;
+      oPhase ^= 1;
+      tcFenceAfter();
+      const bool live = row < it.L;
+      if (a.lse) a.lse[((size_t)it.b * a.H + it.h) * a.padded() + row] = live ? -(m * p.c + log2f(l)) : -INFINITY;
+      const float inv = live ? 1.f / l : 0.f;
+#pragma unroll
+      for (int x = 0; x < HD / 32; x++) {
+        uint32_t o[32], w[16];
+        tmemLoad32(tO + x * 32, o);
+        tmemLoadWait();
+        if (x == HD / 32 - 1) {
+          tcFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArrive(&oFree[t]);
+        }
+        const int words = a.D / 2 - x * 16;
+#pragma unroll
+        for (int e = 0; e < 32; e++) o[e] = live ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+#pragma unroll
+        for (int e = 0; e < 16; e++) w[e] = pack2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+        if (row < a.S) storeRow16(a.out.at(it.b, it.h, row) + x * 32, w, words, p.wide);
+        if (a.rest.p) {
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            w[e] = pack2(__uint_as_float(o[2 * e]) - __uint_as_float(w[e] << 16), __uint_as_float(o[2 * e + 1]) - __uint_as_float(w[e] & 0xffff0000u));
+          if (row < a.S) storeRow16(a.rest.at(it.b, it.h, row) + x * 32, w, words, p.wide);
+        }
+      }
     }
   }
   tcFenceBefore();
