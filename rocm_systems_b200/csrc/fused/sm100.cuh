@@ -278,6 +278,16 @@ __device__ __forceinline__ uint64_t smemDescSw128Mn(uint32_t smemByteAddr, uint3
   d |= (uint64_t)2 << 61;
   return d;
 }
+// Shared-memory operand descriptor for a K-major tile without swizzle: 8 rows of 16 bytes (a core matrix) are 128 contiguous bytes, the next
+// 8 rows follow `rowGroupBytes` further on, the next 16 bytes along K `kBytes` further on.
+__device__ __forceinline__ uint64_t smemDescPlain(uint32_t smemByteAddr, uint32_t kBytes, uint32_t rowGroupBytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smemByteAddr & 0x3ffff) >> 4);
+  d |= (uint64_t)((kBytes >> 4) & 0x3fff) << 16;
+  d |= (uint64_t)((rowGroupBytes >> 4) & 0x3fff) << 32;
+  d |= (uint64_t)1 << 46;
+  return d;
+}
 // Instruction descriptor with the operands' majors: 0 K-major, 1 MN-major.
 __host__ __device__ constexpr uint32_t instrDescMajor(uint32_t M, uint32_t N, uint32_t abFormat, uint32_t aMn, uint32_t bMn) {
   return (1u << 4) | (abFormat << 7) | (abFormat << 10) | (aMn << 15) | (bMn << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);

@@ -153,7 +153,7 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
   a.dk = tensor(dk, 6);
   a.dv = tensor(dv, 7);
   a.lse = const_cast<float*>(lse);
-  a.delta = scratch;
+  a.stat = reinterpret_cast<__nv_bfloat16*>(scratch);
   a.lengths = lengths;
   a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
   a.window = window == 0 ? S : window;
@@ -163,7 +163,7 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
   if (!good(a) || !lse || !scratch || !rest || (((uintptr_t)rest | (uintptr_t)lse | (uintptr_t)scratch) & 15)) return (int)cudaErrorInvalidValue;
   for (const Tensor* t : {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv})
     if (!aligned(*t)) return (int)cudaErrorInvalidValue;
-  float* partials = scratch + (size_t)B * H * a.padded();
+  float* partials = scratch + (size_t)B * H * a.padded() * 4;
   return (int)(D <= 64 ? backward<64>(a, partials, s) : backward<128>(a, partials, s));
 }
 
@@ -175,7 +175,7 @@ long long b200ops_window_attention_bwd_scratch(int B, int H, int KV, int S, int 
   if (!good(a)) return -1;
   BwdParams p{};
   splitSinks(a, p);
-  return (long long)B * H * a.padded() + partialWords(a, p);
+  return (long long)B * H * a.padded() * 4 + partialWords(a, p);
 }
 
 }  // extern "C"

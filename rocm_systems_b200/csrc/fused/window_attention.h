@@ -18,9 +18,8 @@ struct Tensor {
 struct Args {
   Tensor q, k, v, out, dout, dq, dk, dv;
   Tensor rest;         // what rounding took from out (bf16), kept for the backward pass, or nullptr
-  // [batch, heads, padded()], both with the sign that they are added with:
-  float* lse;          // minus log2 of the sum of exp over a row's visible scores, minus infinity for a row behind the sequence's end
-  float* delta;        // minus the sum of dout * out over a row (backward)
+  float* lse;          // [batch, heads, padded()]: minus log2 of the sum of exp over a row's visible scores, minus infinity behind the sequence's end
+  __nv_bfloat16* stat; // [batch, heads, padded(), 8]: of a row -lse / c and -delta, the sum of dout * out, as three values each (backward)
   const int* lengths;  // [batch] or nullptr
   int B, H, KV, S, D;
   int window, sinks;   // window >= 1 (S or more: everything)

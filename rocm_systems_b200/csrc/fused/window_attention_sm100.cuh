@@ -24,7 +24,7 @@ using namespace rows;
 constexpr int kTile = 128;  // queries and keys of a tile
 constexpr uint32_t kBox = kTile * 128;  // bytes of a TMA box: 128 rows of 64 elements
 constexpr float kSlack = 8.f;
-constexpr int kPolyFwd = 4;  // of a row's pairs of powers of two, one in so many is a polynomial
+constexpr int kPolyFwd = 99;  // of a row's pairs of powers of two, one in so many is a polynomial
 constexpr int kPolyBwd = 2;
 
 enum ErrCode : int { ERR_FWD_LOAD = 21, ERR_FWD_MMA, ERR_FWD_SOFTMAX, ERR_BWD_LOAD, ERR_BWD_MMA, ERR_BWD_MATH };
@@ -446,6 +446,11 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 //   keys:    X = K, V;   Y = Q, dO;  dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head.
 // In the keys' kernel dV of a tile and the next tile's S run while its dS is made, dK and the next dP while the next P is made.
 //
+// In the keys' kernel lse and delta belong to the columns. Read from shared memory by every thread they took half of its bandwidth, which the
+// products need (3800 cycles a tile of 128 x 128; the products themselves run 2200). So they enter by one more step of the products instead:
+// each row of Y gets six more elements, -lse / c and -delta as the sums of three bf16 values each (`stat`, left by the queries' kernel), each
+// row of X1 ones at the first three and of X2 at the others. Then P = 2^(S c) and dS = P dP.
+//
 // Y1 of tile n + 2 takes the slot of Y2 of tile n, which is through first, and the other way round.
 //
 // Keys that every later query sees (sinks) would keep their CTAs far longer than the others: the queries behind the window are split over
@@ -469,7 +474,8 @@ template <int HD> struct BwdCfg {
   static constexpr int kBoxes = HD / 64;
   static constexpr uint32_t kTileBytes = kBoxes * kBox;
   static constexpr uint32_t kXBytes = 8 * 32 * 256;  // X1 and X2, later the staging buffers of eight warps
-  static constexpr size_t kSmem = 1024 + kXBytes + 4 * kTileBytes + 2 * 2 * kTile * 4 + 2 * kTile * 4 + 256;
+  static constexpr uint32_t kStatBytes = kTile * 16;  // eight more elements of a tile's rows
+  static constexpr size_t kSmem = 1024 + kXBytes + 4 * kTileBytes + 5 * kStatBytes + 256;
   static constexpr uint32_t kTmemCols = 512;
 };
 
@@ -481,9 +487,9 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   uint8_t* smemX = smem;                    // X1, X2
   uint8_t* ring = smem + C::kXBytes;        // 4 slots
-  float* stats = reinterpret_cast<float*>(ring + 4 * C::kTileBytes);  // keys: [2][lse, delta][128]
-  float* half = stats + 4 * kTile;          // queries: [2][128] halves of delta
-  uint64_t* bars = reinterpret_cast<uint64_t*>(half + 2 * kTile);
+  uint8_t* stats = ring + 4 * C::kTileBytes;              // keys: X1's and X2's further elements, Y's of two tiles, zeros
+  float* half = reinterpret_cast<float*>(stats);          // queries: [2][128] halves of delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + 5 * C::kStatBytes);
   uint64_t *xFull = bars, *full = bars + 1, *empty = bars + 5, *sFull = bars + 9 /*[2]*/, *dpFull = bars + 11, *pReady = bars + 12, *dsReady = bars + 13,
            *statFull = bars + 14 /*[2]*/, *statEmpty = bars + 16 /*[2]*/, *done = bars + 18, *clear = bars + 19 /*[2]*/;
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 21);
@@ -563,7 +569,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
     for (int s = 0; s < 2; s++) {
       mbarInit(&sFull[s], 1);
       mbarInit(&statFull[s], 1);
-      mbarInit(&statEmpty[s], 8);
+      mbarInit(&statEmpty[s], 1);
       mbarInit(&clear[s], 1);
     }
     mbarInit(dpFull, 1);
@@ -575,6 +581,14 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
   if (warp == 9) {
     tmemAlloc(tmemSlot, C::kTmemCols);
     tmemRelinquish();
+  }
+  if (SIDE == kKeys && warp < 4) {
+    const uint32_t two = 0x3f803f80u, low = 0x3f80u, high = 0x3f800000u;  // bf16 ones
+    uint4* rows = reinterpret_cast<uint4*>(stats) + threadIdx.x;
+    rows[0] = make_uint4(two, low, 0, 0);
+    rows[kTile] = make_uint4(0, high, two, 0);
+    rows[4 * kTile] = make_uint4(0, 0, 0, 0);
+    fenceProxyAsync();
   }
   tcFenceBefore();
   __syncthreads();
@@ -603,10 +617,8 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
         }
         if constexpr (SIDE == kKeys) {
           if (!ok || !(ok = mbarWait(&statEmpty[n & 1], turn, err, ERR_BWD_LOAD))) break;
-          const size_t at = ((size_t)b * a.H + h) * a.padded() + y0;
-          mbarArriveExpectTx(&statFull[n & 1], 2 * kTile * 4);
-          bulkLoad(stats + (n & 1) * 2 * kTile, a.lse + at, kTile * 4, &statFull[n & 1]);
-          bulkLoad(stats + (n & 1) * 2 * kTile + kTile, a.delta + at, kTile * 4, &statFull[n & 1]);
+          mbarArriveExpectTx(&statFull[n & 1], C::kStatBytes);
+          bulkLoad(stats + (2 + (n & 1)) * C::kStatBytes, a.stat + (((size_t)b * a.H + h) * a.padded() + y0) * 8, C::kStatBytes, &statFull[n & 1]);
         }
       }
       if (!ok) {  // let loads in flight land
@@ -637,11 +649,17 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       for (int kk = 0; kk < kTile / 16; kk++)
         mmaF16FromTmem(tmem + acc, tmem + w + (kk / 4) * 64 + (kk % 4) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
     };
+    const auto further = [&](uint32_t d, int x, int n) {  // keys: the step of lse or delta
+      const uint32_t at = smemAddr(stats);
+      const int y = 2 + (n & 1);
+      mmaF16(tmem + d, smemDescPlain(at + x * C::kStatBytes, (4 - x) * C::kStatBytes, 128), smemDescPlain(at + y * C::kStatBytes, (4 - y) * C::kStatBytes, 128), idescS, 1);
+    };
     const auto scores = [&](int n) {
-      if (!landed(slot1(n), n, true)) return false;
+      if (!landed(slot1(n), n, true) || (SIDE == kKeys && !waitFor(&statFull[n & 1], (n >> 1) & 1))) return false;
       const int buf = SIDE == kQueries ? n & 1 : 0;
       if (electOne()) {
         product(kS + buf * kTile, 0, slot1(n));
+        if (SIDE == kKeys) further(kS, 0, n);
         mmaCommit(&sFull[buf]);
       }
       __syncwarp();
@@ -651,8 +669,9 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       if (!landed(slot2(n), n, SIDE == kKeys)) return false;
       if (electOne()) {
         product(kDp, 1, slot2(n));
+        if (SIDE == kKeys) further(kDp, 1, n);
         mmaCommit(dpFull);
-        if (SIDE == kQueries) mmaCommit(&empty[slot2(n)]);
+        mmaCommit(SIDE == kQueries ? &empty[slot2(n)] : &statEmpty[n & 1]);
       }
       __syncwarp();
       return true;
@@ -716,13 +735,25 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       half[side * kTile + r] = delta;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       delta = half[r] + half[kTile + r];
-      if (side == 0) a.delta[(size_t)bh * a.padded() + row] = -delta;
+      if (side == 0) {
+        uint32_t w[3];
+        __nv_bfloat16 part[6];
+        const float of[2] = {live ? lse / p.c : 0.f, live ? -delta : 0.f};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          part[3 * i] = __float2bfloat16(of[i]);
+          const float rest = of[i] - __bfloat162float(part[3 * i]);
+          part[3 * i + 1] = __float2bfloat16(rest);
+          part[3 * i + 2] = __float2bfloat16(rest - __bfloat162float(part[3 * i + 1]));
+        }
+#pragma unroll
+        for (int i = 0; i < 3; i++) w[i] = (uint32_t)__bfloat16_as_ushort(part[2 * i]) | (uint32_t)__bfloat16_as_ushort(part[2 * i + 1]) << 16;
+        reinterpret_cast<uint4*>(a.stat)[(size_t)bh * a.padded() + row] = make_uint4(w[0], w[1], w[2], 0);
+      }
     }
     bool ok = true;
     for (int n = 0; n < count && ok; n++) {
       const int y0 = tileOf(n) * kTile;
-      const float* st = stats + (n & 1) * 2 * kTile + cols;
-      if (SIDE == kKeys && !(ok = mbarWait(&statFull[n & 1], (n >> 1) & 1, err, ERR_BWD_MATH))) break;
       const int buf = SIDE == kQueries ? n & 1 : 0;
       if (!(ok = mbarWait(&sFull[buf], SIDE == kQueries ? (n >> 1) & 1 : n & 1, err, ERR_BWD_MATH))) break;
       tcFenceAfter();
@@ -743,8 +774,6 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       }
       F2 w[32];  // the weights
       const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
-      const ulonglong2* lse2 = reinterpret_cast<const ulonglong2*>(st);
-      const ulonglong2* delta2 = reinterpret_cast<const ulonglong2*>(st + kTile);
       const auto masked = [&](F2 v, int e) {  // pair e of this thread's 32
         float lo, hi;
         splitF2(v, lo, hi);
@@ -757,18 +786,11 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
         tmemLoad32(base + kS + buf * kTile + cols + 32, s[1]);
         tmemLoadWait();
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          ulonglong2 off = make_ulonglong2(rowLse, rowLse);
-          if (SIDE == kKeys) off = lse2[e / 2];
-          const F2 v0 = fmaF2(makeF2(__uint_as_float(s[e / 16][2 * e % 32]), __uint_as_float(s[e / 16][2 * e % 32 + 1])), c2, off.x);
-          const F2 v1 = fmaF2(makeF2(__uint_as_float(s[e / 16][2 * e % 32 + 2]), __uint_as_float(s[e / 16][2 * e % 32 + 3])), c2, off.y);
-          if constexpr (decltype(all)::value) {
-            w[e] = exp2F2(v0);
-            w[e + 1] = e / 2 % (kPolyBwd / 2) == 0 ? exp2Poly(v1) : exp2F2(v1);
-          } else {
-            w[e] = masked(exp2F2(v0), e);
-            w[e + 1] = masked(exp2F2(v1), e + 1);
-          }
+        for (int e = 0; e < 32; e++) {
+          const F2 score = makeF2(__uint_as_float(s[e / 16][2 * e % 32]), __uint_as_float(s[e / 16][2 * e % 32 + 1]));
+          const F2 v = SIDE == kQueries ? fmaF2(score, c2, rowLse) : mulF2(score, c2);
+          if constexpr (decltype(all)::value) w[e] = e % kPolyBwd == kPolyBwd - 1 ? exp2Poly(v) : exp2F2(v);
+          else w[e] = masked(exp2F2(v), e);
         }
       };
       if (every) weights(std::true_type{});
@@ -797,16 +819,11 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
         for (int x = 0; x < 2; x++) {
           uint32_t o[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            ulonglong2 off = make_ulonglong2(rowDelta, rowDelta);
-            if (SIDE == kKeys) off = delta2[x * 8 + e / 2];
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const int i = x * 16 + e + k;
-              F2 v = mulF2(w[i], addF2(makeF2(__uint_as_float(d[x][2 * (e + k)]), __uint_as_float(d[x][2 * (e + k) + 1])), k ? off.y : off.x));
-              if (!decltype(all)::value) v = masked(v, i);  // what is masked may be anything
-              o[e + k] = pack2(v);
-            }
+          for (int e = 0; e < 16; e++) {
+            const F2 dp = makeF2(__uint_as_float(d[x][2 * e]), __uint_as_float(d[x][2 * e + 1]));
+            F2 v = mulF2(w[x * 16 + e], SIDE == kQueries ? addF2(dp, rowDelta) : dp);
+            if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
+            o[e] = pack2(v);
           }
           tmemStore16(base + kDp + cols + x * 16, o);
         }
@@ -816,10 +833,7 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
       tmemStoreWait();
       tcFenceBefore();
       __syncwarp();
-      if (lane == 0) {
-        mbarArrive(dsReady);
-        if (SIDE == kKeys) mbarArrive(&statEmpty[n & 1]);
-      }
+      if (lane == 0) mbarArrive(dsReady);
     }
     ok = ok && mbarWait(done, 0, err, ERR_BWD_MATH);
     if (ok) {
