@@ -74,29 +74,14 @@ template <int HD> struct FwdCfg {
 // What a persistent CTA does in its turn `k`: items are sorted by falling cost, so every other turn goes through the CTAs backwards.
 __device__ __forceinline__ long long itemOf(int k) { return (long long)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
 
-// The rows of a tile that lie behind the sequence's end, zeroed in shared memory before the tensor cores sum over them: the issuing warp
-// asks (barrier 0), a warp that does nothing else zeroes and answers (barrier 1).
-struct Clearing {
-  uint64_t* bars;
-  uint32_t phase = 0;
-  __device__ bool request(int lane, volatile int* err, int code) {
-    if (lane == 0) sm100::mbarArrive(&bars[0]);
-    const bool ok = sm100::mbarWait(&bars[1], phase, err, code);
-    phase ^= 1;
-    return __all_sync(0xffffffffu, ok);
-  }
-  template <int BOXES> __device__ bool serve(uint8_t* tile, int from, int lane, volatile int* err, int code) {
-    if (!sm100::mbarWait(&bars[0], phase, err, code)) return false;
-    phase ^= 1;
-    for (int n = from * 8 + lane; n < kTile * 8; n += 32)
+// Zeroes rows [from, ROWS) of a tile of BOXES boxes of ROWS rows x 128 bytes, by a whole warp: a weight of zero does not silence what may lie
+// behind a sequence's end, so it must not be there where the tensor cores sum over a tile's rows.
+template <int BOXES, int ROWS> __device__ __forceinline__ void zeroRows(uint8_t* tile, int from, int lane) {
+  for (int n = from * 8 + lane; n < ROWS * 8; n += 32)
 #pragma unroll
-      for (int x = 0; x < BOXES; x++) *reinterpret_cast<uint4*>(tile + x * kBox + n * 16) = make_uint4(0, 0, 0, 0);
-    sm100::fenceProxyAsync();
-    __syncwarp();
-    if (lane == 0) sm100::mbarArrive(&bars[1]);
-    return true;
-  }
-};
+    for (int x = 0; x < BOXES; x++) *reinterpret_cast<uint4*>(tile + x * ROWS * 128 + n * 16) = make_uint4(0, 0, 0, 0);
+  sm100::fenceProxyAsync();
+}
 
 // Rows [row0, row0 + 128) of a head to zeros, from warps 0-3 or 4-7.
 __device__ __forceinline__ void zeroOut(const Tensor& t, int b, int h, int row0, int S, int D, int tid) {
@@ -119,11 +104,10 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   uint64_t* full = bars + 2;              // [kSlots]
   uint64_t* empty = full + C::kSlots;     // [kSlots]
   uint64_t* sFull = empty + C::kSlots;    // [2] scores in tensor memory
-  uint64_t* pReady = sFull + 2;           // [2] weights in their place, O scaled
+  uint64_t* pReady = sFull + 2;           // [2] weights in their place, O scaled; this step's values and the next one's keys have landed
   uint64_t* oDone = pReady + 2;           // [2] O complete
   uint64_t* oFree = oDone + 2;            // [2] O read
-  uint64_t* clear = oFree + 2;            // [2] see Clearing
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(clear + 2);
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(oFree + 2);
 
   const Args& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the compiler is to know that it is a warp's)
@@ -133,14 +117,13 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     prefetchTensorMap(&p.q);
     prefetchTensorMap(&p.k);
     prefetchTensorMap(&p.v);
-    mbarInit(qFull, 1);
+    mbarInit(qFull, 2);
     mbarInit(qEmpty, 1);
     for (int t = 0; t < 2; t++) {
       mbarInit(&sFull[t], 1);
-      mbarInit(&pReady[t], 4);
+      mbarInit(&pReady[t], 5);
       mbarInit(&oDone[t], 1);
       mbarInit(&oFree[t], 4);
-      mbarInit(&clear[t], 1);
     }
     for (int s = 0; s < C::kSlots; s++) {
       mbarInit(&full[s], 1);
@@ -215,17 +198,11 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescO = instrDescMajor(kTile, HD, 1, 0, 1);
     // The whole warp walks along and one elected lane issues: what the instructions take from uniform registers is then formed there. (With
     // `lane == 0` in the place of the election each cost 100 cycles to issue, and runs 64.)
-    const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbarWait(bar, parity, err, ERR_FWD_MMA)); };
     const uint64_t descQ = smemDescSw128(smemAddr(smemQ)), descK = smemDescSw128(smemAddr(ring)), descV = smemDescSw128Mn(smemAddr(ring), kBox);
-    Clearing clearing{clear};
-    bool ok = true;
-    uint32_t qPhase = 0, pPhase[2] = {0, 0}, oTurn[2] = {1, 1}, landedPhase = 0;
-    int landedSlot = 0;  // of the next tile to land
-    const auto landed = [&]() {
-      const bool r = wait(&full[landedSlot], landedPhase);
-      if (++landedSlot == C::kSlots) landedSlot = 0, landedPhase ^= 1;
-      return r;
-    };
+    bool ok = true, all = true;  // of this lane's waits; of the warp's, looked at once per tile and off the products' way: waits behind one that was given up are short
+    const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = mbarWait(bar, parity, err, ERR_FWD_MMA) && ok; };
+    uint32_t qPhase = 0, pPhase[2] = {0, 0}, oTurn[2] = {1, 1};
+    int slotK = 0;
     const auto after = [](int s) { return s + 1 == C::kSlots ? 0 : s + 1; };
     const auto scores = [&](int t, int slot) {  // by the elected lane
 #pragma unroll
@@ -235,11 +212,10 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       }
       mmaCommit(&sFull[t]);
     };
-    for (int k = 0; ok && itemOf(k) < p.items; k++) {
+    for (int k = 0; all && itemOf(k) < p.items; k++) {
       const Item it(p, itemOf(k));
       if (it.count == 0) continue;
-      int slotK = landedSlot;
-      if (!(ok = wait(qFull, qPhase) && landed())) break;
+      wait(qFull, qPhase);  // and the first keys, see warp 10
       qPhase ^= 1;
       if (electOne()) {
         scores(0, slotK);
@@ -249,21 +225,18 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       }
       __syncwarp();
       bool started[2] = {false, false};
-      for (int n = 0; n < it.count && ok; n++) {
+      for (int n = 0; n < it.count && all; n++) {
         const bool more = n + 1 < it.count;
         const int slotV = after(slotK), slotNext = after(slotV);
-        if (!(ok = landed() && (!more || landed()))) break;
-        // A weight of zero does not silence what lies behind the sequence's end.
-        if (it.straddles(n) && !(ok = clearing.request(lane, err, ERR_FWD_MMA))) break;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
           const bool now = it.active(t, n), next = more && it.active(t, n + 1), last = it.tileOf(n) == (t ? it.own1.last : it.own0.last);
           if (now) {
             if (!started[t]) {
-              if (!(ok = wait(&oFree[t], oTurn[t]))) break;
+              wait(&oFree[t], oTurn[t]);
               oTurn[t] ^= 1;
             }
-            if (!(ok = wait(&pReady[t], pPhase[t]))) break;
+            wait(&pReady[t], pPhase[t]);
             pPhase[t] ^= 1;
             tcFenceAfter();
           }
@@ -285,20 +258,45 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
           __syncwarp();
           started[t] = started[t] || now;
         }
-        slotK = slotNext;
+        if (more) slotK = slotNext;
+        all = __all_sync(0xffffffffu, ok);
       }
+      slotK = after(after(slotK));
     }
   } else if (warp == 10) {
+    // Looks after the landed tiles, so that the issuing warp has one barrier to wait for per step (each wait is 100 to 200 cycles of its time,
+    // which the tensor cores stand still): takes part in the barriers that it waits for when the tiles of the step are there.
     setMaxRegsDown<C::kOtherRegs>();
-    Clearing clearing{clear};
-    int tiles = 0;  // that went through the ring before this item
+    int slot = 0;
+    uint32_t phase = 0, pPhase[2] = {0, 0};
     bool ok = true;
+    const auto landed = [&]() {
+      const int s = slot;
+      ok = ok && mbarWait(&full[s], phase, err, ERR_FWD_MMA);
+      if (++slot == C::kSlots) slot = 0, phase ^= 1;
+      return s;
+    };
     for (int k = 0; ok && itemOf(k) < p.items; k++) {
       const Item it(p, itemOf(k));
-      for (int n = 0; n < it.count && ok; n++)
-        if (it.straddles(n))
-          ok = clearing.serve<C::kBoxes>(ring + (tiles + 2 * n + 1) % C::kSlots * C::kTileBytes, it.L - it.tileOf(n) * kTile, lane, err, ERR_FWD_MMA);
-      tiles = (tiles + 2 * it.count) % C::kSlots;
+      if (it.count == 0) continue;
+      landed();
+      __syncwarp();
+      if (lane == 0) mbarArrive(qFull);
+      for (int n = 0; n < it.count && ok; n++) {
+        const int v = landed();
+        if (n + 1 < it.count) landed();
+        if (it.straddles(n)) zeroRows<C::kBoxes, kTile>(ring + v * C::kTileBytes, it.L - it.tileOf(n) * kTile, lane);
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+          if (lane == 0 && it.active(t, n)) mbarArrive(&pReady[t]);
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+          if (it.active(t, n)) {  // not ahead of them
+            ok = ok && mbarWait(&pReady[t], pPhase[t], err, ERR_FWD_MMA);
+            pPhase[t] ^= 1;
+          }
+      }
     }
   } else if (warp == 11) {
     setMaxRegsDown<C::kOtherRegs>();
@@ -438,24 +436,28 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 
 // ---- backward ---------------------------------------------------------------------------------------------------
 // Two kernels of one shape, which both form the weights again instead of sharing them through memory, so that no gradient is summed by
-// atomics: a CTA owns 128 rows of two operands (X1, X2), streams 128-row tiles of two others (Y1, Y2) and has in tensor memory
+// atomics: a persistent CTA takes 128 rows of two operands (X1, X2) after one another, copies them into tensor memory, streams tiles of two
+// others (Y1, Y2) through shared memory and has in tensor memory
 //   S = X1 Y1^T   and   dP = X2 Y2^T   (or their transposes),
 // from which 256 threads, two per row, make P = 2^(S c - lse) and dS = P (dP - delta) in bf16, in the place of what they were made of, as
 // the tensor-memory operands of the products that follow:
-//   queries: X = Q, dO;  Y = K, V;   dQ += dS Y1. Scores are double buffered. delta is formed here.
-//   keys:    X = K, V;   Y = Q, dO;  dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head.
-// In the keys' kernel dV of a tile and the next tile's S run while its dS is made, dK and the next dP while the next P is made.
+//   queries: X = Q, dO;  Y = K, V in tiles of 128;    dQ += dS Y1. delta is formed here.
+//   keys:    X = K, V;   Y = Q, dO in tiles of 64;    dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head.
+// All products thus read one operand from shared memory. With both there, 128 x 128 x 16 takes 85 cycles instead of 64: shared memory hands out 128
+// bytes a cycle, which is just what such a product takes, and the tiles have to be written as well. (The keys' two accumulators leave room
+// for 64 columns of S and dP.)
 //
-// In the keys' kernel lse and delta belong to the columns. Read from shared memory by every thread they took half of its bandwidth, which the
-// products need (3800 cycles a tile of 128 x 128; the products themselves run 2200). So they enter by one more step of the products instead:
-// each row of Y gets six more elements, -lse / c and -delta as the sums of three bf16 values each (`stat`, left by the queries' kernel), each
-// row of X1 ones at the first three and of X2 at the others. Then P = 2^(S c) and dS = P dP.
+// In the keys' kernel lse and delta belong to the columns. Read from shared memory by every thread they took another share of its bandwidth. So
+// they enter by one more step of the products instead: each row of Y gets six more elements, -lse / c and -delta as the sums of three
+// bf16 values each (`stat`, left by the queries' kernel), each row of X1 ones at the first three and of X2 at the others. Then
+// P = 2^(S c) and dS = P dP.
 //
-// Y1 of tile n + 2 takes the slot of Y2 of tile n, which is through first, and the other way round.
+// While an item's gradients are written, the next one's first products run.
 //
 // Keys that every later query sees (sinks) would keep their CTAs far longer than the others: the queries behind the window are split over
-// further CTAs, whose fp32 sums joinSinks adds up in a fixed order.
+// further items, whose fp32 sums joinSinks adds up in a fixed order.
 enum Side { kQueries, kKeys };
+constexpr int kKeysTile = 64;  // queries of a streamed tile in the keys' kernel
 
 struct BwdParams {
   CUtensorMap x1, x2, y1, y2;
@@ -463,98 +465,108 @@ struct BwdParams {
   float c;
   int tiles;      // 128-row tiles of a sequence
   int sinkTiles;  // key tiles whose far queries are split off; 0: none
-  int farChunk, farCount;  // query tiles per split, splits per sink tile
+  int farChunk, farCount;  // 64-query tiles per split, splits per sink tile
+  long long items;
+  bool wide;               // rows of the gradients start on 32-byte boundaries and are whole 32-byte pieces
   float* partials;         // [B * KV][sinkTiles][1 + farCount][dK, dV][min(sinks, 128)][D]
   int* err;
 };
 
-template <int HD> struct BwdCfg {
+template <int HD, Side SIDE> struct BwdCfg {
   static constexpr int kThreads = 384;                // split as in the forward kernel
   static constexpr int kMathRegs = 216, kOtherRegs = 64;
   static constexpr int kBoxes = HD / 64;
-  static constexpr uint32_t kTileBytes = kBoxes * kBox;
-  static constexpr uint32_t kXBytes = 8 * 32 * 256;  // X1 and X2, later the staging buffers of eight warps
-  static constexpr uint32_t kStatBytes = kTile * 16;  // eight more elements of a tile's rows
-  static constexpr size_t kSmem = 1024 + kXBytes + 4 * kTileBytes + 5 * kStatBytes + 256;
+  static constexpr int kRows = SIDE == kQueries ? kTile : kKeysTile;  // of a streamed tile
+  static constexpr int kSlots = SIDE == kQueries ? 4 : 8;
+  static constexpr uint32_t kXBytes = kBoxes * kBox;
+  static constexpr uint32_t kBoxBytes = kRows * 128, kTileBytes = kBoxes * kBoxBytes;
+  static constexpr uint32_t kOnes = kTile * 16, kStat = kRows * 16;   // eight more elements of X's and Y's rows
+  static constexpr uint32_t kExtra = SIDE == kQueries ? 2 * kTile * 4 : 3 * kOnes + 2 * kStat;
+  static constexpr size_t kSmem = 1024 + 2 * kXBytes + kSlots * kTileBytes + kExtra + 256;
   static constexpr uint32_t kTmemCols = 512;
+  // columns: X1, X2; S, dP (kRows each); dQ, or dV and dK
+  static constexpr uint32_t kX1 = 0, kX2 = 64, kS = 128, kDp = kS + kRows, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
 };
 
 template <int HD, Side SIDE>
-__global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const __grid_constant__ BwdParams p) {
-  using C = BwdCfg<HD>;
+__global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(const __grid_constant__ BwdParams p) {
+  using C = BwdCfg<HD, SIDE>;
   using namespace sm100;
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* smemX = smem;                    // X1, X2
-  uint8_t* ring = smem + C::kXBytes;        // 4 slots
-  uint8_t* stats = ring + 4 * C::kTileBytes;              // keys: X1's and X2's further elements, Y's of two tiles, zeros
-  float* half = reinterpret_cast<float*>(stats);          // queries: [2][128] halves of delta
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + 5 * C::kStatBytes);
-  uint64_t *xFull = bars, *full = bars + 1, *empty = bars + 5, *sFull = bars + 9 /*[2]*/, *dpFull = bars + 11, *pReady = bars + 12, *dsReady = bars + 13,
-           *statFull = bars + 14 /*[2]*/, *statEmpty = bars + 16 /*[2]*/, *done = bars + 18, *clear = bars + 19 /*[2]*/;
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 21);
-  // tensor memory: queries S0, S1, dP, dQ; keys S, dP, dV, dK
-  constexpr uint32_t kS = 0, kDp = SIDE == kQueries ? 256 : 128, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
+  uint8_t* smemX = smem;                              // X1, X2
+  uint8_t* ring = smem + 2 * C::kXBytes;
+  uint8_t* extra = ring + C::kSlots * C::kTileBytes;  // keys: X1's and X2's further elements, Y's of two tiles, zeros
+  float* half = reinterpret_cast<float*>(extra);      // queries: [2][128] halves of delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(extra + C::kExtra);
+  uint64_t *xFull = bars, *xReady = bars + 1, *sFull = bars + 2, *sTaken = bars + 3 /* queries: scores read; keys: weights in their place */, *dpFull = bars + 4,
+           *dsReady = bars + 5, *statFull = bars + 6 /*[2]*/, *statEmpty = bars + 8 /*[2]*/, *done = bars + 10, *full = bars + 11,
+           *empty = full + C::kSlots;
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(empty + C::kSlots);
 
   const Args& a = p.a;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the compiler is to know that it is a warp's)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* err = p.err;
 
-  // ---- what this CTA does: rows [x0, x0 + 128) of head xh against tiles [yFirst, yFirst + yTiles) (queries: keys, sinks first) of `group` heads from yh on
-  const int xHeads = SIDE == kQueries ? a.H : a.KV, all = a.B * xHeads;
-  const int bh = blockIdx.x % all, xh = bh % xHeads, b = bh / xHeads;
-  const int L = lengthOf(a, b);
-  int item = blockIdx.x / all, xTile, far = -1;
-  if constexpr (SIDE == kQueries) {
-    xTile = p.tiles - 1 - item;  // the longest rows first
-  } else {
-    xTile = item < p.tiles ? item : (item - p.tiles) / p.farCount;
-    if (item >= p.tiles) far = (item - p.tiles) % p.farCount;
-  }
-  const int x0 = xTile * kTile;
-  int yFirst, yTiles, sinkTiles = 0;
-  if constexpr (SIDE == kQueries) {
-    const KeyRange r(a, x0, min(x0 + kTile, L) - 1);
-    yFirst = r.first;
-    sinkTiles = min(r.sinkTiles, r.first);
-    yTiles = x0 < L ? sinkTiles + r.last - r.first + 1 : 0;
-  } else {
-    const int lastTile = (L - 1) / kTile;  // of the sequence
-    const int reach = a.window > a.S - x0 ? a.S : x0 + kTile + a.window - 1;  // first query that sees none of the tile's keys through the window
-    const int nearLast = x0 < a.sinks && p.sinkTiles == 0 ? lastTile : min(lastTile, (reach - 1) / kTile);
-    if (far < 0) {
-      yFirst = xTile;
-      yTiles = nearLast - xTile + 1;
-    } else {
-      yFirst = (reach - 1) / kTile + 1 + far * p.farChunk;
-      yTiles = min(p.farChunk, lastTile - yFirst + 1);
-    }
-    if (x0 >= L || yTiles < 0) yTiles = 0;
-  }
-  const int group = SIDE == kQueries ? 1 : a.group(), yh = SIDE == kQueries ? xh / a.group() : xh * a.group();
-  const int count = yTiles * group;
-  const auto tileOf = [&](int n) {
-    if constexpr (SIDE == kQueries) return n < sinkTiles ? n : yFirst + n - sinkTiles;
-    else return yFirst + n % yTiles;
-  };
-  const auto straddles = [&](int n) { return L - tileOf(n) * kTile < kTile; };
-  const auto headOf = [&](int n) { return SIDE == kQueries ? yh : yh + n / yTiles; };
-  const bool sinkRows = SIDE == kKeys && xTile < p.sinkTiles;  // some rows' sums go through `partials`
-  const int partRows = sinkRows ? min(kTile, a.sinks - x0) : 0, partPitch = min(a.sinks, kTile);
-  float* part = sinkRows ? p.partials + ((size_t)(bh * p.sinkTiles + xTile) * (1 + p.farCount) + 1 + far) * 2 * partPitch * a.D : nullptr;
-
-  if (count == 0) {
-    if (warp < 8) {
-      const int tid = threadIdx.x & 127, which = warp >> 2;
+  // Rows [x0, x0 + 128) of head xh against `yTiles` streamed tiles (queries: the sinks' first) of `group` heads from yh on.
+  struct Item {
+    int b, xh, bh, L, xTile, x0, far, yFirst, yTiles, sinkTiles, yh, count, partRows;
+    __device__ Item(const BwdParams& p, long long item) {
+      const Args& a = p.a;
+      const int xHeads = SIDE == kQueries ? a.H : a.KV, all = a.B * xHeads, turn = (int)(item / all);
+      bh = (int)(item % all);
+      xh = bh % xHeads;
+      b = bh / xHeads;
+      L = lengthOf(a, b);
+      far = -1;
+      sinkTiles = partRows = 0;
       if constexpr (SIDE == kQueries) {
-        if (which == 0) zeroOut(a.dq, b, xh, x0, a.S, a.D, tid);
+        xTile = p.tiles - 1 - turn;  // the longest rows first
+        x0 = xTile * kTile;
+        const KeyRange r(a, x0, min(x0 + kTile, L) - 1);
+        yFirst = r.first;
+        sinkTiles = min(r.sinkTiles, r.first);
+        yTiles = sinkTiles + r.last - r.first + 1;
+        yh = xh / a.group();
+        count = x0 < L ? yTiles : 0;
       } else {
-        if (far < 0) zeroOut(which ? a.dk : a.dv, b, xh, x0, a.S, a.D, tid);
-        for (int n = tid; n < partRows * a.D; n += 128) part[(which ? 0 : partPitch * a.D) + n] = 0.f;
+        xTile = turn < p.tiles ? turn : (turn - p.tiles) / p.farCount;
+        if (turn >= p.tiles) far = (turn - p.tiles) % p.farCount;
+        x0 = xTile * kTile;
+        const int lastTile = (L - 1) / kKeysTile;                                   // of the sequence
+        const int reach = a.window > a.S - x0 ? a.S : x0 + kTile + a.window - 1;  // first query that sees none of the tile's keys through the window
+        const int nearLast = x0 < a.sinks && p.sinkTiles == 0 ? lastTile : min(lastTile, (reach - 1) / kKeysTile);
+        if (far < 0) {
+          yFirst = x0 / kKeysTile;
+          yTiles = nearLast - yFirst + 1;
+        } else {
+          yFirst = (reach - 1) / kKeysTile + 1 + far * p.farChunk;
+          yTiles = min(p.farChunk, lastTile - yFirst + 1);
+        }
+        if (x0 >= L || yTiles < 0) yTiles = 0;
+        yh = xh * a.group();
+        count = yTiles * a.group();
+        if (xTile < p.sinkTiles) partRows = min(kTile, a.sinks - x0);
       }
     }
-    return;
-  }
+    // The streamed tiles in their order.
+    __device__ int firstTile() const { return SIDE == kQueries && sinkTiles ? 0 : yFirst; }
+    __device__ int nextTile(int tile) const {
+      const int end = SIDE == kQueries ? sinkTiles : yFirst + yTiles;  // queries: from the sinks to the window; keys: to the next head's first
+      return tile + 1 == end ? yFirst : tile + 1;
+    }
+    __device__ bool straddles(int tile) const { return L - tile * C::kRows < C::kRows; }
+    // Where the sums of this item's sinks go: dK's rows, then dV's.
+    __device__ float* part(const BwdParams& p, bool dv) const {
+      const int pitch = min(p.a.sinks, kTile);
+      return p.partials + (((size_t)(bh * p.sinkTiles + xTile) * (1 + p.farCount) + 1 + far) * 2 + dv) * pitch * p.a.D;
+    }
+  };
+  // The streamed tiles are counted through all items. Queries: Y1 of a tile takes the slot of Y2 of the tile but one before it, which is
+  // through first, and the other way round.
+  const auto slot1 = [](uint32_t g) { return SIDE == kQueries ? 2 * (g & 1) + (g >> 1 & 1) : 2 * (g & 3); };
+  const auto slot2 = [](uint32_t g) { return SIDE == kQueries ? 2 * (g & 1) + 1 - (g >> 1 & 1) : 2 * (g & 3) + 1; };
+  const auto ringPhase = [](uint32_t g) { return SIDE == kQueries ? g >> 1 & 1 : g >> 2 & 1; };
 
   if (threadIdx.x == 0) {
     prefetchTensorMap(&p.x1);
@@ -562,20 +574,20 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
     prefetchTensorMap(&p.y1);
     prefetchTensorMap(&p.y2);
     mbarInit(xFull, 1);
-    for (int s = 0; s < 4; s++) {
+    mbarInit(xReady, 9);
+    mbarInit(sFull, 1);
+    mbarInit(sTaken, 9);
+    mbarInit(dpFull, 1);
+    mbarInit(dsReady, 9);
+    mbarInit(done, 1);
+    for (int s = 0; s < 2; s++) {
+      mbarInit(&statFull[s], 1);
+      mbarInit(&statEmpty[s], 1);
+    }
+    for (int s = 0; s < C::kSlots; s++) {
       mbarInit(&full[s], 1);
       mbarInit(&empty[s], 1);
     }
-    for (int s = 0; s < 2; s++) {
-      mbarInit(&sFull[s], 1);
-      mbarInit(&statFull[s], 1);
-      mbarInit(&statEmpty[s], 1);
-      mbarInit(&clear[s], 1);
-    }
-    mbarInit(dpFull, 1);
-    mbarInit(pReady, 8);
-    mbarInit(dsReady, 8);
-    mbarInit(done, 1);
     fenceBarrierInit();
   }
   if (warp == 9) {
@@ -584,292 +596,379 @@ __global__ void __launch_bounds__(BwdCfg<HD>::kThreads, 1) backwardKernel(const 
   }
   if (SIDE == kKeys && warp < 4) {
     const uint32_t two = 0x3f803f80u, low = 0x3f80u, high = 0x3f800000u;  // bf16 ones
-    uint4* rows = reinterpret_cast<uint4*>(stats) + threadIdx.x;
-    rows[0] = make_uint4(two, low, 0, 0);
-    rows[kTile] = make_uint4(0, high, two, 0);
-    rows[4 * kTile] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(extra)[threadIdx.x] = make_uint4(two, low, 0, 0);
+    reinterpret_cast<uint4*>(extra + C::kOnes)[threadIdx.x] = make_uint4(0, high, two, 0);
+    reinterpret_cast<uint4*>(extra + 2 * C::kOnes + 2 * C::kStat)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     fenceProxyAsync();
   }
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmemSlot, 0);
-  const auto slot1 = [](int n) { return 2 * (n & 1) + ((n >> 1) & 1); };
-  const auto slot2 = [](int n) { return 2 * (n & 1) + 1 - ((n >> 1) & 1); };
 
   if (warp == 8) {
     setMaxRegsDown<C::kOtherRegs>();
     if (lane == 0) {
-      mbarArriveExpectTx(xFull, 2 * C::kTileBytes);
-      for (int x = 0; x < C::kBoxes; x++) {
-        tmaLoad4d(smemX + x * kBox, &p.x1, x * 64, x0, xh, b, xFull);
-        tmaLoad4d(smemX + C::kTileBytes + x * kBox, &p.x2, x * 64, x0, xh, b, xFull);
-      }
+      uint32_t g = 0, turn = 1;  // tiles and items so far
       bool ok = true;
-      for (int n = 0; n < count && ok; n++) {
-        const int y0 = tileOf(n) * kTile, h = headOf(n);
-        const uint32_t turn = ((n >> 1) & 1) ^ 1;
-        for (int w = 0; w < 2 && ok; w++) {
-          const int s = w ? slot2(n) : slot1(n);
-          if (!(ok = mbarWait(&empty[s], turn, err, ERR_BWD_LOAD))) break;
-          mbarArriveExpectTx(&full[s], C::kTileBytes);
-          for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * kBox, w ? &p.y2 : &p.y1, x * 64, y0, h, b, &full[s]);
+      for (int k = 0; ok && itemOf(k) < p.items; k++) {
+        const Item it(p, itemOf(k));
+        if (it.count == 0) continue;
+        if (!(ok = mbarWait(xReady, turn, err, ERR_BWD_LOAD))) break;  // the rows before are in tensor memory
+        turn ^= 1;
+        mbarArriveExpectTx(xFull, 2 * C::kXBytes);
+        for (int x = 0; x < C::kBoxes; x++) {
+          tmaLoad4d(smemX + x * kBox, &p.x1, x * 64, it.x0, it.xh, it.b, xFull);
+          tmaLoad4d(smemX + C::kXBytes + x * kBox, &p.x2, x * 64, it.x0, it.xh, it.b, xFull);
         }
-        if constexpr (SIDE == kKeys) {
-          if (!ok || !(ok = mbarWait(&statEmpty[n & 1], turn, err, ERR_BWD_LOAD))) break;
-          mbarArriveExpectTx(&statFull[n & 1], C::kStatBytes);
-          bulkLoad(stats + (2 + (n & 1)) * C::kStatBytes, a.stat + (((size_t)b * a.H + h) * a.padded() + y0) * 8, C::kStatBytes, &statFull[n & 1]);
+        int tile = it.firstTile(), h = it.yh;
+        for (int n = 0; n < it.count && ok; n++, g++) {
+          const int y0 = tile * C::kRows;
+          for (int w = 0; w < 2 && ok; w++) {
+            const int s = w ? slot2(g) : slot1(g);
+            if (!(ok = mbarWait(&empty[s], ringPhase(g) ^ 1, err, ERR_BWD_LOAD))) break;
+            mbarArriveExpectTx(&full[s], C::kTileBytes);
+            for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * C::kBoxBytes, w ? &p.y2 : &p.y1, x * 64, y0, h, it.b, &full[s]);
+          }
+          if constexpr (SIDE == kKeys) {
+            if (!ok || !(ok = mbarWait(&statEmpty[g & 1], (g >> 1 & 1) ^ 1, err, ERR_BWD_LOAD))) break;
+            mbarArriveExpectTx(&statFull[g & 1], C::kStat);
+            bulkLoad(extra + 2 * C::kOnes + (g & 1) * C::kStat, a.stat + (((size_t)it.b * a.H + h) * a.padded() + y0) * 8, C::kStat, &statFull[g & 1]);
+          }
+          tile = it.nextTile(tile);
+          if (SIDE == kKeys && tile == it.yFirst) h++;
         }
       }
       if (!ok) {  // let loads in flight land
         mbarWait(xFull, 0, err, 0, 2000u);
-        for (int s = 0; s < 4; s++) mbarWait(&full[s], 0, err, 0, 2000u);
+        for (int s = 0; s < C::kSlots; s++) mbarWait(&full[s], 0, err, 0, 2000u);
       }
     }
   } else if (warp == 9) {
     setMaxRegsDown<C::kOtherRegs>();
-    constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescAcc = instrDescMajor(kTile, HD, 1, 0, 1);
+    constexpr uint32_t idescS = instrDesc(kTile, C::kRows, 1 /*bf16*/), idescAcc = instrDescMajor(kTile, HD, 1, 0, 1);
     // As in the forward kernel the whole warp walks along and one elected lane issues.
-    Clearing clearing{clear};
-    const auto waitFor = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbarWait(bar, parity, err, ERR_BWD_MMA)); };
-    // Rows behind the sequence's end are zeroed where they are summed over: a weight of zero does not silence what may lie there.
-    const auto landed = [&](int s, int n, bool summed) {
-      return waitFor(&full[s], (n >> 1) & 1) && (!summed || !straddles(n) || clearing.request(lane, err, ERR_BWD_MMA));
-    };
-    const uint64_t descX = smemDescSw128(smemAddr(smemX)), descY = smemDescSw128(smemAddr(ring)), descSum = smemDescSw128Mn(smemAddr(ring), kBox);
-    const auto product = [&](uint32_t d, int x, int s) {  // d = X Y^T
+    const uint64_t descY = smemDescSw128(smemAddr(ring)), descSum = smemDescSw128Mn(smemAddr(ring), C::kBoxBytes);
+    const auto product = [&](uint32_t d, uint32_t x, int s) {  // d = X Y^T
 #pragma unroll
-      for (int kk = 0; kk < HD / 16; kk++) {
-        const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
-        mmaF16(tmem + d, descX + ((x * C::kTileBytes + o) >> 4), descY + ((s * C::kTileBytes + o) >> 4), idescS, kk != 0);
-      }
+      for (int kk = 0; kk < HD / 16; kk++)
+        mmaF16FromTmem(tmem + d, tmem + x + kk * 8, descY + ((s * C::kTileBytes + (kk / 4) * C::kBoxBytes + (kk % 4) * 32) >> 4), idescS, kk != 0);
     };
-    const auto gather = [&](uint32_t acc, uint32_t w, int s, bool first) {  // acc += W Y, W: two halves of 64 columns, each packed into 32
+    const auto gather = [&](uint32_t acc, uint32_t w, int s, bool first) {  // acc += W Y, W: two halves of the tile's columns, each packed into half of its own
+      constexpr int kSteps = C::kRows / 32;
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; kk++)
-        mmaF16FromTmem(tmem + acc, tmem + w + (kk / 4) * 64 + (kk % 4) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
+      for (int kk = 0; kk < C::kRows / 16; kk++)
+        mmaF16FromTmem(tmem + acc, tmem + w + (kk / kSteps) * (C::kRows / 2) + (kk % kSteps) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
     };
-    const auto further = [&](uint32_t d, int x, int n) {  // keys: the step of lse or delta
-      const uint32_t at = smemAddr(stats);
-      const int y = 2 + (n & 1);
-      mmaF16(tmem + d, smemDescPlain(at + x * C::kStatBytes, (4 - x) * C::kStatBytes, 128), smemDescPlain(at + y * C::kStatBytes, (4 - y) * C::kStatBytes, 128), idescS, 1);
+    const auto further = [&](uint32_t d, int x, uint32_t g) {  // keys: the step of lse or delta
+      const uint32_t zeros = smemAddr(extra) + 2 * C::kOnes + 2 * C::kStat, xa = smemAddr(extra) + x * C::kOnes, ya = smemAddr(extra) + 2 * C::kOnes + (g & 1) * C::kStat;
+      mmaF16(tmem + d, smemDescPlain(xa, zeros - xa, 128), smemDescPlain(ya, zeros - ya, 128), idescS, 1);
     };
-    const auto scores = [&](int n) {
-      if (!landed(slot1(n), n, true) || (SIDE == kKeys && !waitFor(&statFull[n & 1], (n >> 1) & 1))) return false;
-      const int buf = SIDE == kQueries ? n & 1 : 0;
-      if (electOne()) {
-        product(kS + buf * kTile, 0, slot1(n));
-        if (SIDE == kKeys) further(kS, 0, n);
-        mmaCommit(&sFull[buf]);
-      }
-      __syncwarp();
-      return true;
-    };
-    const auto grads = [&](int n) {
-      if (!landed(slot2(n), n, SIDE == kKeys)) return false;
-      if (electOne()) {
-        product(kDp, 1, slot2(n));
-        if (SIDE == kKeys) further(kDp, 1, n);
+    uint32_t g = 0, xPhase = 0;
+    bool ok = true, all = true;  // of this lane's waits; of the warp's, looked at once per tile and off the products' way: waits behind one that was given up are short
+    const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = mbarWait(bar, parity, err, ERR_BWD_MMA) && ok; };
+    for (int k = 0; all && itemOf(k) < p.items; k++) {
+      const Item it(p, itemOf(k));
+      if (it.count == 0) continue;
+      const auto scores = [&](uint32_t g) {  // by the elected lane, as grads
+        product(C::kS, C::kX1, slot1(g));
+        if (SIDE == kKeys) further(C::kS, 0, g);
+        mmaCommit(sFull);
+      };
+      const auto grads = [&](uint32_t g) {
+        product(C::kDp, C::kX2, slot2(g));
+        if (SIDE == kKeys) further(C::kDp, 1, g);
         mmaCommit(dpFull);
-        mmaCommit(SIDE == kQueries ? &empty[slot2(n)] : &statEmpty[n & 1]);
-      }
-      __syncwarp();
-      return true;
-    };
-    bool ok = waitFor(xFull, 0) && scores(0) && grads(0);
-    if (SIDE == kQueries && count > 1) ok = ok && scores(1);
-    for (int n = 0; n < count && ok; n++) {
-      if constexpr (SIDE == kKeys) {
-        if (!(ok = waitFor(pReady, n & 1))) break;
-        tcFenceAfter();
-        if (electOne()) {
-          gather(kAcc1, kS, slot2(n), n == 0);
-          mmaCommit(&empty[slot2(n)]);
-        }
-        __syncwarp();
-        if (n + 1 < count && !(ok = scores(n + 1))) break;
-      }
-      if (!(ok = waitFor(dsReady, n & 1))) break;
+        mmaCommit(SIDE == kQueries ? &empty[slot2(g)] : &statEmpty[g & 1]);
+      };
+      wait(xReady, xPhase);  // the first tiles have landed too, see warp 10
+      xPhase ^= 1;
       tcFenceAfter();
       if (electOne()) {
-        gather(SIDE == kQueries ? kAcc1 : kAcc2, kDp, slot1(n), n == 0);
-        mmaCommit(&empty[slot1(n)]);
-        if (n + 1 == count) mmaCommit(done);
+        scores(g);
+        grads(g);
       }
       __syncwarp();
-      if (n + 1 < count && !(ok = grads(n + 1))) break;
-      if (SIDE == kQueries && n + 2 < count && !(ok = scores(n + 2))) break;
+      for (int n = 0; n < it.count && all; n++, g++) {
+        const bool more = n + 1 < it.count;
+        if (SIDE == kKeys || more) {
+          wait(sTaken, g & 1);
+          tcFenceAfter();
+          if (electOne()) {
+            if constexpr (SIDE == kKeys) {
+              gather(C::kAcc1, C::kS, slot2(g), n == 0);
+              mmaCommit(&empty[slot2(g)]);
+            }
+            if (more) scores(g + 1);
+          }
+          __syncwarp();
+        }
+        wait(dsReady, g & 1);
+        tcFenceAfter();
+        if (electOne()) {
+          gather(SIDE == kQueries ? C::kAcc1 : C::kAcc2, C::kDp, slot1(g), n == 0);
+          mmaCommit(&empty[slot1(g)]);
+          if (more) grads(g + 1);
+          else mmaCommit(done);
+        }
+        __syncwarp();
+        all = __all_sync(0xffffffffu, ok);
+      }
     }
   } else if (warp == 10) {
+    // As in the forward kernel: looks after the landed tiles and takes part in the barriers that the issuing warp waits for.
     setMaxRegsDown<C::kOtherRegs>();
-    Clearing clearing{clear};
+    uint32_t g = 0;
     bool ok = true;
-    for (int n = 0; n < count && ok; n++) {
-      if (!straddles(n)) continue;
-      ok = clearing.serve<C::kBoxes>(ring + slot1(n) * C::kTileBytes, L - tileOf(n) * kTile, lane, err, ERR_BWD_MMA);
-      if (SIDE == kKeys) ok = ok && clearing.serve<C::kBoxes>(ring + slot2(n) * C::kTileBytes, L - tileOf(n) * kTile, lane, err, ERR_BWD_MMA);
+    const auto landed = [&](const Item& it, int tile, uint32_t g, int which) {
+      const int s = which ? slot2(g) : slot1(g);
+      ok = ok && mbarWait(&full[s], ringPhase(g), err, ERR_BWD_MMA);
+      if (SIDE == kKeys && which == 0) ok = ok && mbarWait(&statFull[g & 1], g >> 1 & 1, err, ERR_BWD_MMA);
+      if ((SIDE == kKeys || which == 0) && it.straddles(tile)) zeroRows<C::kBoxes, C::kRows>(ring + s * C::kTileBytes, it.L - tile * C::kRows, lane);
+      __syncwarp();
+    };
+    for (int k = 0; ok && itemOf(k) < p.items; k++) {
+      const Item it(p, itemOf(k));
+      if (it.count == 0) continue;
+      int tile = it.firstTile();
+      landed(it, tile, g, 0);
+      landed(it, tile, g, 1);
+      if (lane == 0) mbarArrive(xReady);
+      for (int n = 0; n < it.count && ok; n++, g++) {
+        tile = it.nextTile(tile);
+        if (n + 1 < it.count) landed(it, tile, g + 1, 0);
+        if (lane == 0) mbarArrive(sTaken);
+        if (n + 1 < it.count) landed(it, tile, g + 1, 1);
+        if (lane == 0) mbarArrive(dsReady);
+        ok = ok && mbarWait(sTaken, g & 1, err, ERR_BWD_MMA) && mbarWait(dsReady, g & 1, err, ERR_BWD_MMA);  // not ahead of them
+      }
     }
   } else if (warp == 11) {
     setMaxRegsDown<C::kOtherRegs>();
   } else {
     setMaxRegsUp<C::kMathRegs>();
-    const int q4 = warp & 3, side = warp >> 2, r = q4 * 32 + lane, row = x0 + r;
-    const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16), cols = side * 64;
-    const bool live = row < L;
-    float lse = 0.f, delta = 0.f;
-    if constexpr (SIDE == kQueries) {
-      if (live) {
-        lse = a.lse[(size_t)bh * a.padded() + row];
-        const uint4* o = reinterpret_cast<const uint4*>(a.out.at(b, xh, row));
-        const uint4* e = reinterpret_cast<const uint4*>(a.rest.at(b, xh, row));
-        const uint4* g = reinterpret_cast<const uint4*>(a.dout.at(b, xh, row));
-        for (int n = side * (HD / 16); n < min(a.D / 8, (side + 1) * (HD / 16)); n++) {
-          float x[8], y[8], z[8];
-          unpack8(o[n], x);
-          unpack8(e[n], y);
-          unpack8(g[n], z);
-#pragma unroll
-          for (int i = 0; i < 8; i++) delta += (x[i] + y[i]) * z[i];
-        }
-      }
-      half[side * kTile + r] = delta;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      delta = half[r] + half[kTile + r];
-      if (side == 0) {
-        uint32_t w[3];
-        __nv_bfloat16 part[6];
-        const float of[2] = {live ? lse / p.c : 0.f, live ? -delta : 0.f};
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          part[3 * i] = __float2bfloat16(of[i]);
-          const float rest = of[i] - __bfloat162float(part[3 * i]);
-          part[3 * i + 1] = __float2bfloat16(rest);
-          part[3 * i + 2] = __float2bfloat16(rest - __bfloat162float(part[3 * i + 1]));
-        }
-#pragma unroll
-        for (int i = 0; i < 3; i++) w[i] = (uint32_t)__bfloat16_as_ushort(part[2 * i]) | (uint32_t)__bfloat16_as_ushort(part[2 * i + 1]) << 16;
-        reinterpret_cast<uint4*>(a.stat)[(size_t)bh * a.padded() + row] = make_uint4(w[0], w[1], w[2], 0);
-      }
-    }
+    constexpr int kCols = C::kRows / 2, kPairs = kCols / 2;  // of a tile's columns, this thread's
+    constexpr int kWords = HD / 4;                         // of X's rows, this thread's
+    const int q4 = warp & 3, side = warp >> 2, r = q4 * 32 + lane;
+    const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16), cols = side * kCols;
+    uint32_t g = 0, xPhase = 0, donePhase = 0;
     bool ok = true;
-    for (int n = 0; n < count && ok; n++) {
-      const int y0 = tileOf(n) * kTile;
-      const int buf = SIDE == kQueries ? n & 1 : 0;
-      if (!(ok = mbarWait(&sFull[buf], SIDE == kQueries ? (n >> 1) & 1 : n & 1, err, ERR_BWD_MATH))) break;
-      tcFenceAfter();
-      uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
-      const bool every = SIDE == kQueries ? x0 + kTile <= L && seesAll(a, x0, x0 + kTile - 1, y0) : y0 + kTile <= L && seesAll(a, y0, y0 + kTile - 1, x0);
-      if (!every) {
+    uint32_t mine[kWords];  // queries: half a row of dO
+    // The next item that has anything to do; what the others have to write is zeros.
+    const auto advance = [&](int k) {
+      for (; itemOf(k) < p.items; k++) {
+        const Item it(p, itemOf(k));
+        if (it.count) break;
+        const int tid = threadIdx.x & 127;
+        if constexpr (SIDE == kQueries) {
+          if (side == 0) zeroOut(a.dq, it.b, it.xh, it.x0, a.S, a.D, tid);
+        } else {
+          if (it.far < 0) zeroOut(side ? a.dk : a.dv, it.b, it.xh, it.x0, a.S, a.D, tid);
+          if (it.partRows)
+            for (int n = tid; n < it.partRows * a.D; n += 128) it.part(p, side == 0)[n] = 0.f;
+        }
+      }
+      return k;
+    };
+    const auto copyX = [&]() {  // this thread's halves of X1's and X2's row to tensor memory
+      if (!mbarWait(xFull, xPhase, err, ERR_BWD_MATH)) return false;
+      xPhase ^= 1;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int y = y0 + cols + x * 32;
-          if constexpr (SIDE == kQueries) {
-            bits[x] = live ? maskBits(a, row, y) : 0u;
-          } else {  // queries [row, end) see key `row`
-            const auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
-            const int end = row < a.sinks || a.window > L - row ? L : row + a.window;
-            bits[x] = below(end - y) & ~below(row - y);
+      for (int x = 0; x < 2; x++) {
+        const uint8_t* row = smemX + x * C::kXBytes + (HD == 128 ? side * kBox : 0) + r * 128;
+        const int chunk0 = HD == 128 ? 0 : side * 4;
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(row + (((chunk0 + i / 4) ^ (r & 7)) << 4));
+          mine[i] = v.x, mine[i + 1] = v.y, mine[i + 2] = v.z, mine[i + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; i += 16) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) w[e] = mine[i + e];
+          tmemStore16(base + (x ? C::kX2 : C::kX1) + side * kWords + i, w);
+        }
+      }
+      tmemStoreWait();
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(xReady);
+      return true;
+    };
+    int k = advance(0);
+    if (itemOf(k) < p.items) ok = copyX();
+    while (ok && itemOf(k) < p.items) {
+      const Item it(p, itemOf(k));
+      const int row = it.x0 + r;
+      const bool live = row < it.L;
+      float lse = 0.f, delta = 0.f;
+      if constexpr (SIDE == kQueries) {
+        const size_t at = (size_t)it.bh * a.padded() + row;
+        if (live) {
+          lse = a.lse[at];
+          const uint4* o = reinterpret_cast<const uint4*>(a.out.at(it.b, it.xh, row));
+          const uint4* e = reinterpret_cast<const uint4*>(a.rest.at(it.b, it.xh, row));
+#pragma unroll
+          for (int n = 0; n < HD / 16; n++) {
+            const int c = side * (HD / 16) + n;
+            if (c * 8 < a.D) {
+              float x[8], y[8], z[8];
+              unpack8(o[c], x);
+              unpack8(e[c], y);
+              unpack8(make_uint4(mine[4 * n], mine[4 * n + 1], mine[4 * n + 2], mine[4 * n + 3]), z);
+#pragma unroll
+              for (int i = 0; i < 8; i++) delta += (x[i] + y[i]) * z[i];
+            }
           }
         }
-      }
-      F2 w[32];  // the weights
-      const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
-      const auto masked = [&](F2 v, int e) {  // pair e of this thread's 32
-        float lo, hi;
-        splitF2(v, lo, hi);
-        const uint32_t b = bits[e / 16] >> (2 * e % 32);
-        return makeF2(b & 1 ? lo : 0.f, b & 2 ? hi : 0.f);
-      };
-      const auto weights = [&](auto all) {
-        uint32_t s[2][32];
-        tmemLoad32(base + kS + buf * kTile + cols, s[0]);
-        tmemLoad32(base + kS + buf * kTile + cols + 32, s[1]);
-        tmemLoadWait();
+        half[side * kTile + r] = delta;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        delta = half[r] + half[kTile + r];
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // read by all before the next item's is written
+        if (side == 0) {
+          uint32_t w[3];
+          __nv_bfloat16 part[6];
+          const float of[2] = {live ? lse / p.c : 0.f, live ? -delta : 0.f};
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          const F2 score = makeF2(__uint_as_float(s[e / 16][2 * e % 32]), __uint_as_float(s[e / 16][2 * e % 32 + 1]));
-          const F2 v = SIDE == kQueries ? fmaF2(score, c2, rowLse) : mulF2(score, c2);
-          if constexpr (decltype(all)::value) w[e] = e % kPolyBwd == kPolyBwd - 1 ? exp2Poly(v) : exp2F2(v);
-          else w[e] = masked(exp2F2(v), e);
+          for (int i = 0; i < 2; i++) {
+            part[3 * i] = __float2bfloat16(of[i]);
+            const float rest = of[i] - __bfloat162float(part[3 * i]);
+            part[3 * i + 1] = __float2bfloat16(rest);
+            part[3 * i + 2] = __float2bfloat16(rest - __bfloat162float(part[3 * i + 1]));
+          }
+#pragma unroll
+          for (int i = 0; i < 3; i++) w[i] = (uint32_t)__bfloat16_as_ushort(part[2 * i]) | (uint32_t)__bfloat16_as_ushort(part[2 * i + 1]) << 16;
+          reinterpret_cast<uint4*>(a.stat)[at] = make_uint4(w[0], w[1], w[2], 0);
         }
-      };
-      if (every) weights(std::true_type{});
-      else weights(std::false_type{});
-      if constexpr (SIDE == kKeys) {
+      }
+      const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
+      int tile = it.firstTile();
+      for (int n = 0; n < it.count; n++, g++) {
+        const int y0 = tile * C::kRows;
+        tile = it.nextTile(tile);
+        const bool every = SIDE == kQueries ? it.x0 + kTile <= it.L && seesAll(a, it.x0, it.x0 + kTile - 1, y0)
+                                            : y0 + C::kRows <= it.L && seesAll(a, y0, y0 + C::kRows - 1, it.x0);
+        uint32_t bits[kCols / 32];
+        if (!every) {
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          uint32_t o[16];
+          for (int x = 0; x < kCols / 32; x++) {
+            const int y = y0 + cols + x * 32;
+            if constexpr (SIDE == kQueries) {
+              bits[x] = live ? maskBits(a, row, y) : 0u;
+            } else {  // queries [row, end) see key `row`
+              const auto below = [](int b) { return b <= 0 ? 0u : b >= 32 ? 0xffffffffu : (1u << b) - 1u; };
+              const int end = row < a.sinks || a.window > it.L - row ? it.L : row + a.window;
+              bits[x] = below(end - y) & ~below(row - y);
+            }
+          }
+        }
+        const auto masked = [&](F2 v, int e) {  // pair e of this thread's
+          float lo, hi;
+          splitF2(v, lo, hi);
+          const uint32_t b = bits[e / 16] >> (2 * e % 32);
+          return makeF2(b & 1 ? lo : 0.f, b & 2 ? hi : 0.f);
+        };
+        if (!(ok = mbarWait(sFull, g & 1, err, ERR_BWD_MATH))) break;
+        tcFenceAfter();
+        F2 w[kPairs];  // the weights
+        {
+          uint32_t s[kCols / 32][32];
 #pragma unroll
-          for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
-          tmemStore16(base + kS + cols + x * 16, o);
+          for (int x = 0; x < kCols / 32; x++) tmemLoad32(base + C::kS + cols + x * 32, s[x]);
+          tmemLoadWait();
+          if constexpr (SIDE == kQueries) {
+            tcFenceBefore();
+            __syncwarp();
+            if (lane == 0) mbarArrive(sTaken);
+          }
+          const auto weights = [&](auto all) {
+#pragma unroll
+            for (int e = 0; e < kPairs; e++) {
+              const F2 score = makeF2(__uint_as_float(s[e / 16][2 * e % 32]), __uint_as_float(s[e / 16][2 * e % 32 + 1]));
+              const F2 v = SIDE == kQueries ? fmaF2(score, c2, rowLse) : mulF2(score, c2);
+              if constexpr (decltype(all)::value) w[e] = e % kPolyBwd == kPolyBwd - 1 ? exp2Poly(v) : exp2F2(v);
+              else w[e] = masked(exp2F2(v), e);
+            }
+          };
+          if (every) weights(std::true_type{});
+          else weights(std::false_type{});
+        }
+        if constexpr (SIDE == kKeys) {
+#pragma unroll
+          for (int x = 0; x < kCols / 32; x++) {
+            uint32_t o[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
+            tmemStore16(base + C::kS + cols + x * 16, o);
+          }
+          tmemStoreWait();
+          tcFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArrive(sTaken);
+        }
+        if (!(ok = mbarWait(dpFull, g & 1, err, ERR_BWD_MATH))) break;
+        tcFenceAfter();
+        {
+          uint32_t d[kCols / 32][32];
+#pragma unroll
+          for (int x = 0; x < kCols / 32; x++) tmemLoad32(base + C::kDp + cols + x * 32, d[x]);
+          tmemLoadWait();
+          const auto gradients = [&](auto all) {
+#pragma unroll
+            for (int x = 0; x < kCols / 32; x++) {
+              uint32_t o[16];
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const F2 dp = makeF2(__uint_as_float(d[x][2 * e]), __uint_as_float(d[x][2 * e + 1]));
+                F2 v = mulF2(w[x * 16 + e], SIDE == kQueries ? addF2(dp, rowDelta) : dp);
+                if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
+                o[e] = pack2(v);
+              }
+              tmemStore16(base + C::kDp + cols + x * 16, o);
+            }
+          };
+          if (every) gradients(std::true_type{});
+          else gradients(std::false_type{});
         }
         tmemStoreWait();
         tcFenceBefore();
         __syncwarp();
-        if (lane == 0) mbarArrive(pReady);
+        if (lane == 0) mbarArrive(dsReady);
       }
-      if (!(ok = mbarWait(dpFull, n & 1, err, ERR_BWD_MATH))) break;
+      if (!ok || !(ok = mbarWait(done, donePhase, err, ERR_BWD_MATH))) break;
+      donePhase ^= 1;
       tcFenceAfter();
-      const auto gradients = [&](auto all) {
-        uint32_t d[2][32];
-        tmemLoad32(base + kDp + cols, d[0]);
-        tmemLoad32(base + kDp + cols + 32, d[1]);
-        tmemLoadWait();
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          uint32_t o[16];
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const F2 dp = makeF2(__uint_as_float(d[x][2 * e]), __uint_as_float(d[x][2 * e + 1]));
-            F2 v = mulF2(w[x * 16 + e], SIDE == kQueries ? addF2(dp, rowDelta) : dp);
-            if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
-            o[e] = pack2(v);
-          }
-          tmemStore16(base + kDp + cols + x * 16, o);
-        }
-      };
-      if (every) gradients(std::true_type{});
-      else gradients(std::false_type{});
-      tmemStoreWait();
-      tcFenceBefore();
-      __syncwarp();
-      if (lane == 0) mbarArrive(dsReady);
-    }
-    ok = ok && mbarWait(done, 0, err, ERR_BWD_MATH);
-    if (ok) {
-      tcFenceAfter();
-      uint8_t* stage = smemX + warp * 32 * 256;
+      k = advance(k + 1);
+      if (itemOf(k) < p.items && !(ok = copyX())) break;
+
+      // ---- the gradients: queries: each of a row's two threads has half of dQ's columns; keys: one has dV, the other dK
       const float f = SIDE == kKeys && side == 0 ? 1.f : a.scale;
-      // queries: each of a row's two threads has half of dQ's columns; keys: one has dV, the other dK
-      const uint32_t acc = base + (SIDE == kQueries ? kAcc1 + side * (HD / 2) : side ? kAcc2 : kAcc1);
-      const int width = SIDE == kQueries ? HD / 2 : HD, col0 = SIDE == kQueries ? side * (HD / 2) : 0;
+      const uint32_t acc = base + (SIDE == kQueries ? C::kAcc1 + side * (HD / 2) : side ? C::kAcc2 : C::kAcc1);
+      constexpr int kWidth = SIDE == kQueries ? HD / 2 : HD;
+      const int col0 = SIDE == kQueries ? side * (HD / 2) : 0;
       const Tensor& dst = SIDE == kQueries ? a.dq : side ? a.dk : a.dv;
-      if (far < 0)
-        gemm::drainStaged(
-            stage, lane, width, a.D - col0,
-            [&](int x, uint32_t(&v)[32]) {
-              tmemLoad32(acc + x * 32, v);
-              tmemLoadWait();
+      const bool summed = r < it.partRows, written = it.far < 0 && !summed && row < a.S;
+#pragma unroll 1
+      for (int x = 0; x < kWidth / 32; x++) {
+        uint32_t v[32];
+        tmemLoad32(acc + x * 32, v);
+        tmemLoadWait();
+        const int col = col0 + x * 32;
+        if (summed) {
+          float* to = it.part(p, side == 0) + (size_t)r * a.D + col;
 #pragma unroll
-              for (int e = 0; e < 32; e++) v[e] = live ? __float_as_uint(__uint_as_float(v[e]) * f) : 0u;
-            },
-            [&](int k) -> __nv_bfloat16* {
-              const int out = row - lane + k;
-              return out < a.S && q4 * 32 + k >= partRows ? dst.at(b, xh, out) + col0 : nullptr;
-            });
-      if (q4 * 32 < partRows)
-        for (int x = 0; x < HD / 32; x++) {
-          uint32_t v[32];
-          tmemLoad32(acc + x * 32, v);
-          tmemLoadWait();
-          float* to = part + (size_t)(side ? 0 : partPitch + 0) * a.D + (size_t)r * a.D + x * 32;
-          if (r < partRows)
+          for (int e = 0; e < 32; e += 4)
+            if (col + e < a.D)
+              *reinterpret_cast<float4*>(to + e) = live ? make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]))
+                                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (written) {
+          uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (x * 32 + e < a.D)
-                *reinterpret_cast<float4*>(to + e) = live ? make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]))
-                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int e = 0; e < 16; e++) w[e] = live ? pack2(__uint_as_float(v[2 * e]) * f, __uint_as_float(v[2 * e + 1]) * f) : 0u;
+          storeRow16(dst.at(it.b, it.xh, row) + col, w, (a.D - col) / 2, p.wide);
         }
+      }
     }
   }
   tcFenceBefore();
