@@ -26,14 +26,14 @@ static void bindContext() {
   if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
 }
 
-// Boxes of `rows` positions x 64 elements of one head, 128-byte swizzle; what lies outside the tensor reads as zeros.
-static bool headMap(CUtensorMap* map, const Tensor& t, int B, int heads, int S, int D, int rows = kTile) {
+// Boxes of 128 positions x 64 elements of one head, 128-byte swizzle; what lies outside the tensor reads as zeros.
+static bool headMap(CUtensorMap* map, const Tensor& t, int B, int heads, int S, int D) {
   const CuDrv& d = CuDrv::get();
   if (!d.cuTensorMapEncodeTiled) return false;
   const auto stride = [&](long long st, int n) { return (cuuint64_t)(n > 1 ? st : D) * 2; };  // of a dimension of one it does not matter
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
   const cuuint64_t strides[3] = {stride(t.s, S), stride(t.h, heads), stride(t.b, B)};
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, kTile, 1, 1}, ones[4] = {1, 1, 1, 1};
   return d.cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16*>(t.p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -72,11 +72,11 @@ template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
 static void splitSinks(const Args& a, BwdParams& p) {
   p.tiles = (a.S + kTile - 1) / kTile;
   if (a.sinks == 0 || a.window >= a.S) return;
-  const int all = (a.S + kKeysTile - 1) / kKeysTile, near = (kTile + a.window - 2) / kKeysTile + 1;  // streamed tiles that see a key tile through the window
-  const int far = all - near;                                                                       // of the first tile; the others have fewer
+  const int near = (kTile + a.window - 2) / kTile + 1;  // query tiles that see a key tile through the window
+  const int far = p.tiles - near;                       // of the first tile; the others have fewer
   if (far <= 0) return;
   p.sinkTiles = (a.sinks + kTile - 1) / kTile;
-  p.farChunk = near < 8 ? 8 : near;
+  p.farChunk = near < 4 ? 4 : near;
   p.farCount = (far + p.farChunk - 1) / p.farChunk;
 }
 static long long partialWords(const Args& a, const BwdParams& p) {
@@ -100,10 +100,9 @@ template <int HD> static cudaError_t backward(const Args& a, float* partials, cu
   p.items = (long long)p.tiles * a.B * a.H;
   k.items = (long long)(p.tiles + p.sinkTiles * p.farCount) * a.B * a.KV;
   if (p.items > 0x7fffffffLL || k.items > 0x7fffffffLL || a.B * (long long)a.KV > 65535 || !headMap(&p.x1, a.q, a.B, a.H, a.S, a.D) ||
-      !headMap(&p.x2, a.dout, a.B, a.H, a.S, a.D) || !headMap(&p.y1, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.y2, a.v, a.B, a.KV, a.S, a.D) ||
-      !headMap(&k.y1, a.q, a.B, a.H, a.S, a.D, kKeysTile) || !headMap(&k.y2, a.dout, a.B, a.H, a.S, a.D, kKeysTile))
+      !headMap(&p.x2, a.dout, a.B, a.H, a.S, a.D) || !headMap(&p.y1, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.y2, a.v, a.B, a.KV, a.S, a.D))
     return cudaErrorInvalidValue;
-  k.x1 = p.y1, k.x2 = p.y2;
+  k.x1 = p.y1, k.x2 = p.y2, k.y1 = p.x1, k.y2 = p.x2;
   cudaError_t e = allowSmem(backwardKernel<HD, kQueries>, Q::kSmem, doneQ);
   if (e == cudaSuccess) e = allowSmem(backwardKernel<HD, kKeys>, K::kSmem, doneK);
   if (e != cudaSuccess) return e;

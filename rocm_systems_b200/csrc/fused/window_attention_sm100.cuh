@@ -24,8 +24,6 @@ using namespace rows;
 constexpr int kTile = 128;  // queries and keys of a tile
 constexpr uint32_t kBox = kTile * 128;  // bytes of a TMA box: 128 rows of 64 elements
 constexpr float kSlack = 8.f;
-constexpr int kPolyFwd = 99;  // of a row's pairs of powers of two, one in so many is a polynomial
-constexpr int kPolyBwd = 2;
 
 enum ErrCode : int { ERR_FWD_LOAD = 21, ERR_FWD_MMA, ERR_FWD_SOFTMAX, ERR_BWD_LOAD, ERR_BWD_MMA, ERR_BWD_MATH };
 
@@ -373,23 +371,17 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         const float off = m == -INFINITY ? 0.f : m * p.c;
         const F2 c2 = makeF2(p.c, p.c), off2 = makeF2(-off, -off);
         F2 sum[4] = {makeF2(l, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f)};
-        const auto weights = [&](auto polynomials) {
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            uint32_t w[16];
+        for (int x = 0; x < 4; x++) {
+          uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-              const F2 v = fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2);
-              const F2 pr = decltype(polynomials)::value && e % kPolyFwd == kPolyFwd - 1 ? exp2Poly(v) : exp2F2(v);
-              sum[e & 3] = addF2(sum[e & 3], pr);
-              w[e] = pack2(pr);
-            }
-            tmemStore16(tS + x * 16, w);
+          for (int e = 0; e < 16; e++) {
+            const F2 pr = exp2F2(fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2));
+            sum[e & 3] = addF2(sum[e & 3], pr);
+            w[e] = pack2(pr);
           }
-        };
-        // Masked scores have to become zeros, which the polynomial does not give.
-        if (every) weights(std::true_type{});
-        else weights(std::false_type{});
+          tmemStore16(tS + x * 16, w);
+        }
         tmemStoreWait();
         tcFenceBefore();
         __syncwarp();
@@ -436,18 +428,19 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 
 // ---- backward ---------------------------------------------------------------------------------------------------
 // Two kernels of one shape, which both form the weights again instead of sharing them through memory, so that no gradient is summed by
-// atomics: a persistent CTA takes 128 rows of two operands (X1, X2) after one another, copies them into tensor memory, streams tiles of two
-// others (Y1, Y2) through shared memory and has in tensor memory
+// atomics: a persistent CTA takes 128 rows of two operands (X1, X2) after one another, streams 128-row tiles of two others (Y1, Y2) and has in
+// tensor memory
 //   S = X1 Y1^T   and   dP = X2 Y2^T   (or their transposes),
 // from which 256 threads, two per row, make P = 2^(S c - lse) and dS = P (dP - delta) in bf16, in the place of what they were made of, as
 // the tensor-memory operands of the products that follow:
-//   queries: X = Q, dO;  Y = K, V in tiles of 128;    dQ += dS Y1. delta is formed here.
-//   keys:    X = K, V;   Y = Q, dO in tiles of 64;    dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head.
-// All products thus read one operand from shared memory. With both there, 128 x 128 x 16 takes 85 cycles instead of 64: shared memory hands out 128
-// bytes a cycle, which is just what such a product takes, and the tiles have to be written as well. (The keys' two accumulators leave room
-// for 64 columns of S and dP.)
+//   queries: X = Q, dO;  Y = K, V;   dQ += dS Y1. X is copied into tensor memory, so that every product reads one operand only from shared memory,
+//            which hands out 128 bytes a cycle: just what a product of 128 x 128 x 16 with both operands there takes (64 cycles, and 85 while
+//            the tiles are written as well). delta is formed here.
+//   keys:    X = K, V;   Y = Q, dO;  dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head. With two accumulators tensor memory has no
+//            room for X. (With tiles of 64 queries it has, but each step's waits, 400 cycles, then come twice as often: 3900 cycles per
+//            128 queries.) dV of a tile and the next tile's S run while its dS is made, dK and the next dP while the next P is made.
 //
-// In the keys' kernel lse and delta belong to the columns. Read from shared memory by every thread they took another share of its bandwidth. So
+// In the keys' kernel lse and delta belong to the columns. Read from shared memory by every thread they took half of its bandwidth. So
 // they enter by one more step of the products instead: each row of Y gets six more elements, -lse / c and -delta as the sums of three
 // bf16 values each (`stat`, left by the queries' kernel), each row of X1 ones at the first three and of X2 at the others. Then
 // P = 2^(S c) and dS = P dP.
@@ -457,7 +450,6 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 // Keys that every later query sees (sinks) would keep their CTAs far longer than the others: the queries behind the window are split over
 // further items, whose fp32 sums joinSinks adds up in a fixed order.
 enum Side { kQueries, kKeys };
-constexpr int kKeysTile = 64;  // queries of a streamed tile in the keys' kernel
 
 struct BwdParams {
   CUtensorMap x1, x2, y1, y2;
@@ -465,7 +457,7 @@ struct BwdParams {
   float c;
   int tiles;      // 128-row tiles of a sequence
   int sinkTiles;  // key tiles whose far queries are split off; 0: none
-  int farChunk, farCount;  // 64-query tiles per split, splits per sink tile
+  int farChunk, farCount;  // query tiles per split, splits per sink tile
   long long items;
   bool wide;               // rows of the gradients start on 32-byte boundaries and are whole 32-byte pieces
   float* partials;         // [B * KV][sinkTiles][1 + farCount][dK, dV][min(sinks, 128)][D]
@@ -476,16 +468,14 @@ template <int HD, Side SIDE> struct BwdCfg {
   static constexpr int kThreads = 384;                // split as in the forward kernel
   static constexpr int kMathRegs = 216, kOtherRegs = 64;
   static constexpr int kBoxes = HD / 64;
-  static constexpr int kRows = SIDE == kQueries ? kTile : kKeysTile;  // of a streamed tile
-  static constexpr int kSlots = SIDE == kQueries ? 4 : 8;
-  static constexpr uint32_t kXBytes = kBoxes * kBox;
-  static constexpr uint32_t kBoxBytes = kRows * 128, kTileBytes = kBoxes * kBoxBytes;
-  static constexpr uint32_t kOnes = kTile * 16, kStat = kRows * 16;   // eight more elements of X's and Y's rows
-  static constexpr uint32_t kExtra = SIDE == kQueries ? 2 * kTile * 4 : 3 * kOnes + 2 * kStat;
-  static constexpr size_t kSmem = 1024 + 2 * kXBytes + kSlots * kTileBytes + kExtra + 256;
+  static constexpr int kSlots = 4;
+  static constexpr uint32_t kTileBytes = kBoxes * kBox;
+  static constexpr uint32_t kStat = kTile * 16;       // eight more elements of a tile's rows
+  static constexpr uint32_t kExtra = SIDE == kQueries ? 2 * kTile * 4 : 5 * kStat;
+  static constexpr size_t kSmem = 1024 + (2 + kSlots) * kTileBytes + kExtra + 256;
   static constexpr uint32_t kTmemCols = 512;
-  // columns: X1, X2; S, dP (kRows each); dQ, or dV and dK
-  static constexpr uint32_t kX1 = 0, kX2 = 64, kS = 128, kDp = kS + kRows, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
+  // columns: queries: X1, X2 (64 each), S, dP, dQ; keys: S, dP, dV, dK
+  static constexpr uint32_t kX1 = 0, kX2 = 64, kS = SIDE == kQueries ? 128 : 0, kDp = kS + 128, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
 };
 
 template <int HD, Side SIDE>
@@ -495,14 +485,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   uint8_t* smemX = smem;                              // X1, X2
-  uint8_t* ring = smem + 2 * C::kXBytes;
+  uint8_t* ring = smem + 2 * C::kTileBytes;
   uint8_t* extra = ring + C::kSlots * C::kTileBytes;  // keys: X1's and X2's further elements, Y's of two tiles, zeros
   float* half = reinterpret_cast<float*>(extra);      // queries: [2][128] halves of delta
   uint64_t* bars = reinterpret_cast<uint64_t*>(extra + C::kExtra);
-  uint64_t *xFull = bars, *xReady = bars + 1, *sFull = bars + 2, *sTaken = bars + 3 /* queries: scores read; keys: weights in their place */, *dpFull = bars + 4,
+  uint64_t *xFull = bars, *xEmpty = bars + 19, *xReady = bars + 1, *sFull = bars + 2, *sTaken = bars + 3 /* queries: scores read; keys: weights in their place */, *dpFull = bars + 4,
            *dsReady = bars + 5, *statFull = bars + 6 /*[2]*/, *statEmpty = bars + 8 /*[2]*/, *done = bars + 10, *full = bars + 11,
            *empty = full + C::kSlots;
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(empty + C::kSlots);
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 20);
 
   const Args& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -533,14 +523,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         xTile = turn < p.tiles ? turn : (turn - p.tiles) / p.farCount;
         if (turn >= p.tiles) far = (turn - p.tiles) % p.farCount;
         x0 = xTile * kTile;
-        const int lastTile = (L - 1) / kKeysTile;                                   // of the sequence
+        const int lastTile = (L - 1) / kTile;                                   // of the sequence
         const int reach = a.window > a.S - x0 ? a.S : x0 + kTile + a.window - 1;  // first query that sees none of the tile's keys through the window
-        const int nearLast = x0 < a.sinks && p.sinkTiles == 0 ? lastTile : min(lastTile, (reach - 1) / kKeysTile);
+        const int nearLast = x0 < a.sinks && p.sinkTiles == 0 ? lastTile : min(lastTile, (reach - 1) / kTile);
         if (far < 0) {
-          yFirst = x0 / kKeysTile;
+          yFirst = x0 / kTile;
           yTiles = nearLast - yFirst + 1;
         } else {
-          yFirst = (reach - 1) / kKeysTile + 1 + far * p.farChunk;
+          yFirst = (reach - 1) / kTile + 1 + far * p.farChunk;
           yTiles = min(p.farChunk, lastTile - yFirst + 1);
         }
         if (x0 >= L || yTiles < 0) yTiles = 0;
@@ -555,18 +545,18 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       const int end = SIDE == kQueries ? sinkTiles : yFirst + yTiles;  // queries: from the sinks to the window; keys: to the next head's first
       return tile + 1 == end ? yFirst : tile + 1;
     }
-    __device__ bool straddles(int tile) const { return L - tile * C::kRows < C::kRows; }
+    __device__ bool straddles(int tile) const { return L - tile * kTile < kTile; }
     // Where the sums of this item's sinks go: dK's rows, then dV's.
     __device__ float* part(const BwdParams& p, bool dv) const {
       const int pitch = min(p.a.sinks, kTile);
       return p.partials + (((size_t)(bh * p.sinkTiles + xTile) * (1 + p.farCount) + 1 + far) * 2 + dv) * pitch * p.a.D;
     }
   };
-  // The streamed tiles are counted through all items. Queries: Y1 of a tile takes the slot of Y2 of the tile but one before it, which is
-  // through first, and the other way round.
-  const auto slot1 = [](uint32_t g) { return SIDE == kQueries ? 2 * (g & 1) + (g >> 1 & 1) : 2 * (g & 3); };
-  const auto slot2 = [](uint32_t g) { return SIDE == kQueries ? 2 * (g & 1) + 1 - (g >> 1 & 1) : 2 * (g & 3) + 1; };
-  const auto ringPhase = [](uint32_t g) { return SIDE == kQueries ? g >> 1 & 1 : g >> 2 & 1; };
+  // The streamed tiles are counted through all items. Y1 of a tile takes the slot of Y2 of the tile but one before it, which is through first, and
+  // the other way round.
+  const auto slot1 = [](uint32_t g) { return 2 * (g & 1) + (g >> 1 & 1); };
+  const auto slot2 = [](uint32_t g) { return 2 * (g & 1) + 1 - (g >> 1 & 1); };
+  const auto ringPhase = [](uint32_t g) { return g >> 1 & 1; };
 
   if (threadIdx.x == 0) {
     prefetchTensorMap(&p.x1);
@@ -574,7 +564,8 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
     prefetchTensorMap(&p.y1);
     prefetchTensorMap(&p.y2);
     mbarInit(xFull, 1);
-    mbarInit(xReady, 9);
+    mbarInit(xEmpty, SIDE == kQueries ? 8 : 1);
+    mbarInit(xReady, SIDE == kQueries ? 9 : 1);
     mbarInit(sFull, 1);
     mbarInit(sTaken, 9);
     mbarInit(dpFull, 1);
@@ -596,9 +587,10 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
   }
   if (SIDE == kKeys && warp < 4) {
     const uint32_t two = 0x3f803f80u, low = 0x3f80u, high = 0x3f800000u;  // bf16 ones
-    reinterpret_cast<uint4*>(extra)[threadIdx.x] = make_uint4(two, low, 0, 0);
-    reinterpret_cast<uint4*>(extra + C::kOnes)[threadIdx.x] = make_uint4(0, high, two, 0);
-    reinterpret_cast<uint4*>(extra + 2 * C::kOnes + 2 * C::kStat)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    uint4* rows = reinterpret_cast<uint4*>(extra) + threadIdx.x;  // X1's, X2's, of two streamed tiles, zeros
+    rows[0] = make_uint4(two, low, 0, 0);
+    rows[kTile] = make_uint4(0, high, two, 0);
+    rows[4 * kTile] = make_uint4(0, 0, 0, 0);
     fenceProxyAsync();
   }
   tcFenceBefore();
@@ -614,26 +606,26 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       for (int k = 0; ok && itemOf(k) < p.items; k++) {
         const Item it(p, itemOf(k));
         if (it.count == 0) continue;
-        if (!(ok = mbarWait(xReady, turn, err, ERR_BWD_LOAD))) break;  // the rows before are in tensor memory
+        if (!(ok = mbarWait(xEmpty, turn, err, ERR_BWD_LOAD))) break;
         turn ^= 1;
-        mbarArriveExpectTx(xFull, 2 * C::kXBytes);
+        mbarArriveExpectTx(xFull, 2 * C::kTileBytes);
         for (int x = 0; x < C::kBoxes; x++) {
           tmaLoad4d(smemX + x * kBox, &p.x1, x * 64, it.x0, it.xh, it.b, xFull);
-          tmaLoad4d(smemX + C::kXBytes + x * kBox, &p.x2, x * 64, it.x0, it.xh, it.b, xFull);
+          tmaLoad4d(smemX + C::kTileBytes + x * kBox, &p.x2, x * 64, it.x0, it.xh, it.b, xFull);
         }
         int tile = it.firstTile(), h = it.yh;
         for (int n = 0; n < it.count && ok; n++, g++) {
-          const int y0 = tile * C::kRows;
+          const int y0 = tile * kTile;
           for (int w = 0; w < 2 && ok; w++) {
             const int s = w ? slot2(g) : slot1(g);
             if (!(ok = mbarWait(&empty[s], ringPhase(g) ^ 1, err, ERR_BWD_LOAD))) break;
             mbarArriveExpectTx(&full[s], C::kTileBytes);
-            for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * C::kBoxBytes, w ? &p.y2 : &p.y1, x * 64, y0, h, it.b, &full[s]);
+            for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * kBox, w ? &p.y2 : &p.y1, x * 64, y0, h, it.b, &full[s]);
           }
           if constexpr (SIDE == kKeys) {
             if (!ok || !(ok = mbarWait(&statEmpty[g & 1], (g >> 1 & 1) ^ 1, err, ERR_BWD_LOAD))) break;
             mbarArriveExpectTx(&statFull[g & 1], C::kStat);
-            bulkLoad(extra + 2 * C::kOnes + (g & 1) * C::kStat, a.stat + (((size_t)it.b * a.H + h) * a.padded() + y0) * 8, C::kStat, &statFull[g & 1]);
+            bulkLoad(extra + (2 + (g & 1)) * C::kStat, a.stat + (((size_t)it.b * a.H + h) * a.padded() + y0) * 8, C::kStat, &statFull[g & 1]);
           }
           tile = it.nextTile(tile);
           if (SIDE == kKeys && tile == it.yFirst) h++;
@@ -646,23 +638,28 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
     }
   } else if (warp == 9) {
     setMaxRegsDown<C::kOtherRegs>();
-    constexpr uint32_t idescS = instrDesc(kTile, C::kRows, 1 /*bf16*/), idescAcc = instrDescMajor(kTile, HD, 1, 0, 1);
+    constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescAcc = instrDescMajor(kTile, HD, 1, 0, 1);
     // As in the forward kernel the whole warp walks along and one elected lane issues.
-    const uint64_t descY = smemDescSw128(smemAddr(ring)), descSum = smemDescSw128Mn(smemAddr(ring), C::kBoxBytes);
-    const auto product = [&](uint32_t d, uint32_t x, int s) {  // d = X Y^T
+    const uint64_t descX = smemDescSw128(smemAddr(smemX)), descY = smemDescSw128(smemAddr(ring)), descSum = smemDescSw128Mn(smemAddr(ring), kBox);
+    const auto product = [&](uint32_t d, int x, int s) {  // d = X Y^T
 #pragma unroll
-      for (int kk = 0; kk < HD / 16; kk++)
-        mmaF16FromTmem(tmem + d, tmem + x + kk * 8, descY + ((s * C::kTileBytes + (kk / 4) * C::kBoxBytes + (kk % 4) * 32) >> 4), idescS, kk != 0);
+      for (int kk = 0; kk < HD / 16; kk++) {
+        const uint32_t o = (kk / 4) * kBox + (kk % 4) * 32;
+        const uint64_t y = descY + ((s * C::kTileBytes + o) >> 4);
+        if (SIDE == kQueries) mmaF16FromTmem(tmem + d, tmem + (x ? C::kX2 : C::kX1) + kk * 8, y, idescS, kk != 0);
+        else mmaF16(tmem + d, descX + ((x * C::kTileBytes + o) >> 4), y, idescS, kk != 0);
+      }
     };
     const auto gather = [&](uint32_t acc, uint32_t w, int s, bool first) {  // acc += W Y, W: two halves of the tile's columns, each packed into half of its own
-      constexpr int kSteps = C::kRows / 32;
+      constexpr int kSteps = kTile / 32;
 #pragma unroll
-      for (int kk = 0; kk < C::kRows / 16; kk++)
-        mmaF16FromTmem(tmem + acc, tmem + w + (kk / kSteps) * (C::kRows / 2) + (kk % kSteps) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
+      for (int kk = 0; kk < kTile / 16; kk++)
+        mmaF16FromTmem(tmem + acc, tmem + w + (kk / kSteps) * (kTile / 2) + (kk % kSteps) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
     };
     const auto further = [&](uint32_t d, int x, uint32_t g) {  // keys: the step of lse or delta
-      const uint32_t zeros = smemAddr(extra) + 2 * C::kOnes + 2 * C::kStat, xa = smemAddr(extra) + x * C::kOnes, ya = smemAddr(extra) + 2 * C::kOnes + (g & 1) * C::kStat;
-      mmaF16(tmem + d, smemDescPlain(xa, zeros - xa, 128), smemDescPlain(ya, zeros - ya, 128), idescS, 1);
+      const uint32_t at = smemAddr(extra);
+      const int y = 2 + (g & 1);
+      mmaF16(tmem + d, smemDescPlain(at + x * C::kStat, (4 - x) * C::kStat, 128), smemDescPlain(at + y * C::kStat, (4 - y) * C::kStat, 128), idescS, 1);
     };
     uint32_t g = 0, xPhase = 0;
     bool ok = true, all = true;  // of this lane's waits; of the warp's, looked at once per tile and off the products' way: waits behind one that was given up are short
@@ -671,12 +668,12 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       const Item it(p, itemOf(k));
       if (it.count == 0) continue;
       const auto scores = [&](uint32_t g) {  // by the elected lane, as grads
-        product(C::kS, C::kX1, slot1(g));
+        product(C::kS, 0, slot1(g));
         if (SIDE == kKeys) further(C::kS, 0, g);
         mmaCommit(sFull);
       };
       const auto grads = [&](uint32_t g) {
-        product(C::kDp, C::kX2, slot2(g));
+        product(C::kDp, 1, slot2(g));
         if (SIDE == kKeys) further(C::kDp, 1, g);
         mmaCommit(dpFull);
         mmaCommit(SIDE == kQueries ? &empty[slot2(g)] : &statEmpty[g & 1]);
@@ -709,7 +706,10 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           gather(SIDE == kQueries ? C::kAcc1 : C::kAcc2, C::kDp, slot1(g), n == 0);
           mmaCommit(&empty[slot1(g)]);
           if (more) grads(g + 1);
-          else mmaCommit(done);
+          else {
+            mmaCommit(done);
+            if (SIDE == kKeys) mmaCommit(xEmpty);
+          }
         }
         __syncwarp();
         all = __all_sync(0xffffffffu, ok);
@@ -718,19 +718,23 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
   } else if (warp == 10) {
     // As in the forward kernel: looks after the landed tiles and takes part in the barriers that the issuing warp waits for.
     setMaxRegsDown<C::kOtherRegs>();
-    uint32_t g = 0;
+    uint32_t g = 0, xPhase = 0;
     bool ok = true;
     const auto landed = [&](const Item& it, int tile, uint32_t g, int which) {
       const int s = which ? slot2(g) : slot1(g);
       ok = ok && mbarWait(&full[s], ringPhase(g), err, ERR_BWD_MMA);
       if (SIDE == kKeys && which == 0) ok = ok && mbarWait(&statFull[g & 1], g >> 1 & 1, err, ERR_BWD_MMA);
-      if ((SIDE == kKeys || which == 0) && it.straddles(tile)) zeroRows<C::kBoxes, C::kRows>(ring + s * C::kTileBytes, it.L - tile * C::kRows, lane);
+      if ((SIDE == kKeys || which == 0) && it.straddles(tile)) zeroRows<C::kBoxes, kTile>(ring + s * C::kTileBytes, it.L - tile * kTile, lane);
       __syncwarp();
     };
     for (int k = 0; ok && itemOf(k) < p.items; k++) {
       const Item it(p, itemOf(k));
       if (it.count == 0) continue;
       int tile = it.firstTile();
+      if (SIDE == kKeys) {
+        ok = ok && mbarWait(xFull, xPhase, err, ERR_BWD_MMA);
+        xPhase ^= 1;
+      }
       landed(it, tile, g, 0);
       landed(it, tile, g, 1);
       if (lane == 0) mbarArrive(xReady);
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
     setMaxRegsDown<C::kOtherRegs>();
   } else {
     setMaxRegsUp<C::kMathRegs>();
-    constexpr int kCols = C::kRows / 2, kPairs = kCols / 2;  // of a tile's columns, this thread's
+    constexpr int kCols = kTile / 2, kPairs = kCols / 2;   // of a tile's columns, this thread's
     constexpr int kWords = HD / 4;                         // of X's rows, this thread's
     const int q4 = warp & 3, side = warp >> 2, r = q4 * 32 + lane;
     const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16), cols = side * kCols;
@@ -775,7 +779,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       xPhase ^= 1;
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-        const uint8_t* row = smemX + x * C::kXBytes + (HD == 128 ? side * kBox : 0) + r * 128;
+        const uint8_t* row = smemX + x * C::kTileBytes + (HD == 128 ? side * kBox : 0) + r * 128;
         const int chunk0 = HD == 128 ? 0 : side * 4;
 #pragma unroll
         for (int i = 0; i < kWords; i += 4) {
@@ -793,11 +797,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       tmemStoreWait();
       tcFenceBefore();
       __syncwarp();
-      if (lane == 0) mbarArrive(xReady);
+      if (lane == 0) {
+        mbarArrive(xReady);
+        mbarArrive(xEmpty);
+      }
       return true;
     };
     int k = advance(0);
-    if (itemOf(k) < p.items) ok = copyX();
+    if (SIDE == kQueries && itemOf(k) < p.items) ok = copyX();
     while (ok && itemOf(k) < p.items) {
       const Item it(p, itemOf(k));
       const int row = it.x0 + r;
@@ -845,10 +852,10 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
       int tile = it.firstTile();
       for (int n = 0; n < it.count; n++, g++) {
-        const int y0 = tile * C::kRows;
+        const int y0 = tile * kTile;
         tile = it.nextTile(tile);
         const bool every = SIDE == kQueries ? it.x0 + kTile <= it.L && seesAll(a, it.x0, it.x0 + kTile - 1, y0)
-                                            : y0 + C::kRows <= it.L && seesAll(a, y0, y0 + C::kRows - 1, it.x0);
+                                            : y0 + kTile <= it.L && seesAll(a, y0, y0 + kTile - 1, it.x0);
         uint32_t bits[kCols / 32];
         if (!every) {
 #pragma unroll
@@ -887,8 +894,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
             for (int e = 0; e < kPairs; e++) {
               const F2 score = makeF2(__uint_as_float(s[e / 16][2 * e % 32]), __uint_as_float(s[e / 16][2 * e % 32 + 1]));
               const F2 v = SIDE == kQueries ? fmaF2(score, c2, rowLse) : mulF2(score, c2);
-              if constexpr (decltype(all)::value) w[e] = e % kPolyBwd == kPolyBwd - 1 ? exp2Poly(v) : exp2F2(v);
-              else w[e] = masked(exp2F2(v), e);
+              w[e] = decltype(all)::value ? exp2F2(v) : masked(exp2F2(v), e);
             }
           };
           if (every) weights(std::true_type{});
@@ -940,7 +946,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       donePhase ^= 1;
       tcFenceAfter();
       k = advance(k + 1);
-      if (itemOf(k) < p.items && !(ok = copyX())) break;
+      if (SIDE == kQueries && itemOf(k) < p.items && !(ok = copyX())) break;
 
       // ---- the gradients: queries: each of a row's two threads has half of dQ's columns; keys: one has dV, the other dK
       const float f = SIDE == kKeys && side == 0 ? 1.f : a.scale;
