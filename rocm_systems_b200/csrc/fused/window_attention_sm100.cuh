@@ -431,14 +431,13 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 // atomics: a persistent CTA takes 128 rows of two operands (X1, X2) after one another, streams 128-row tiles of two others (Y1, Y2) and has in
 // tensor memory
 //   S = X1 Y1^T   and   dP = X2 Y2^T   (or their transposes),
-// from which 256 threads, two per row, make P = 2^(S c - lse) and dS = P (dP - delta) in bf16, in the place of what they were made of, as
-// the tensor-memory operands of the products that follow:
+// from which 256 threads, two per row, make P = 2^(S c - lse) and dS = P (dP - delta) in bf16, both in dP's place, as the tensor-memory
+// operands of the products that follow, while the next tile's S, whose place is free once it has been read, is already there:
 //   queries: X = Q, dO;  Y = K, V;   dQ += dS Y1. X is copied into tensor memory, so that every product reads one operand only from shared memory,
 //            which hands out 128 bytes a cycle: just what a product of 128 x 128 x 16 with both operands there takes (64 cycles, and 85 while
 //            the tiles are written as well). delta is formed here.
 //   keys:    X = K, V;   Y = Q, dO;  dV += P^T Y2, dK += dS^T Y1, over all query heads of the key head. With two accumulators tensor memory has no
-//            room for X. (With tiles of 64 queries it has, but each step's waits, 400 cycles, then come twice as often: 3900 cycles per
-//            128 queries.) dV of a tile and the next tile's S run while its dS is made, dK and the next dP while the next P is made.
+//            room for X.
 //
 // In the keys' kernel lse and delta belong to the columns. Read from shared memory by every thread they took half of its bandwidth. So
 // they enter by one more step of the products instead: each row of Y gets six more elements, -lse / c and -delta as the sums of three
@@ -489,7 +488,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
   uint8_t* extra = ring + C::kSlots * C::kTileBytes;  // keys: X1's and X2's further elements, Y's of two tiles, zeros
   float* half = reinterpret_cast<float*>(extra);      // queries: [2][128] halves of delta
   uint64_t* bars = reinterpret_cast<uint64_t*>(extra + C::kExtra);
-  uint64_t *xFull = bars, *xEmpty = bars + 19, *xReady = bars + 1, *sFull = bars + 2, *sTaken = bars + 3 /* queries: scores read; keys: weights in their place */, *dpFull = bars + 4,
+  uint64_t *xFull = bars, *xEmpty = bars + 19, *xReady = bars + 1, *sFull = bars + 2, *sTaken = bars + 3, *dpFull = bars + 4,
            *dsReady = bars + 5, *statFull = bars + 6 /*[2]*/, *statEmpty = bars + 8 /*[2]*/, *done = bars + 10, *full = bars + 11,
            *empty = full + C::kSlots;
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 20);
@@ -616,16 +615,16 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         int tile = it.firstTile(), h = it.yh;
         for (int n = 0; n < it.count && ok; n++, g++) {
           const int y0 = tile * kTile;
+          if constexpr (SIDE == kKeys) {  // first, as its place is free long before the tiles'
+            if (!(ok = mbarWait(&statEmpty[g & 1], (g >> 1 & 1) ^ 1, err, ERR_BWD_LOAD))) break;
+            mbarArriveExpectTx(&statFull[g & 1], C::kStat);
+            bulkLoad(extra + (2 + (g & 1)) * C::kStat, a.stat + (((size_t)it.b * a.H + h) * a.padded() + y0) * 8, C::kStat, &statFull[g & 1]);
+          }
           for (int w = 0; w < 2 && ok; w++) {
             const int s = w ? slot2(g) : slot1(g);
             if (!(ok = mbarWait(&empty[s], ringPhase(g) ^ 1, err, ERR_BWD_LOAD))) break;
             mbarArriveExpectTx(&full[s], C::kTileBytes);
             for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * kBox, w ? &p.y2 : &p.y1, x * 64, y0, h, it.b, &full[s]);
-          }
-          if constexpr (SIDE == kKeys) {
-            if (!ok || !(ok = mbarWait(&statEmpty[g & 1], (g >> 1 & 1) ^ 1, err, ERR_BWD_LOAD))) break;
-            mbarArriveExpectTx(&statFull[g & 1], C::kStat);
-            bulkLoad(extra + (2 + (g & 1)) * C::kStat, a.stat + (((size_t)it.b * a.H + h) * a.padded() + y0) * 8, C::kStat, &statFull[g & 1]);
           }
           tile = it.nextTile(tile);
           if (SIDE == kKeys && tile == it.yFirst) h++;
@@ -688,22 +687,20 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       __syncwarp();
       for (int n = 0; n < it.count && all; n++, g++) {
         const bool more = n + 1 < it.count;
-        if (SIDE == kKeys || more) {
+        if (more) {
           wait(sTaken, g & 1);
           tcFenceAfter();
-          if (electOne()) {
-            if constexpr (SIDE == kKeys) {
-              gather(C::kAcc1, C::kS, slot2(g), n == 0);
-              mmaCommit(&empty[slot2(g)]);
-            }
-            if (more) scores(g + 1);
-          }
+          if (electOne()) scores(g + 1);
           __syncwarp();
         }
         wait(dsReady, g & 1);
         tcFenceAfter();
         if (electOne()) {
-          gather(SIDE == kQueries ? C::kAcc1 : C::kAcc2, C::kDp, slot1(g), n == 0);
+          if constexpr (SIDE == kKeys) {
+            gather(C::kAcc1, C::kDp, slot2(g), n == 0);
+            mmaCommit(&empty[slot2(g)]);
+          }
+          gather(SIDE == kQueries ? C::kAcc1 : C::kAcc2, SIDE == kQueries ? C::kDp : C::kDp + 32, slot1(g), n == 0);
           mmaCommit(&empty[slot1(g)]);
           if (more) grads(g + 1);
           else {
@@ -884,11 +881,9 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
 #pragma unroll
           for (int x = 0; x < kCols / 32; x++) tmemLoad32(base + C::kS + cols + x * 32, s[x]);
           tmemLoadWait();
-          if constexpr (SIDE == kQueries) {
-            tcFenceBefore();
-            __syncwarp();
-            if (lane == 0) mbarArrive(sTaken);
-          }
+          tcFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArrive(sTaken);
           const auto weights = [&](auto all) {
 #pragma unroll
             for (int e = 0; e < kPairs; e++) {
@@ -900,19 +895,6 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           if (every) weights(std::true_type{});
           else weights(std::false_type{});
         }
-        if constexpr (SIDE == kKeys) {
-#pragma unroll
-          for (int x = 0; x < kCols / 32; x++) {
-            uint32_t o[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
-            tmemStore16(base + C::kS + cols + x * 16, o);
-          }
-          tmemStoreWait();
-          tcFenceBefore();
-          __syncwarp();
-          if (lane == 0) mbarArrive(sTaken);
-        }
         if (!(ok = mbarWait(dpFull, g & 1, err, ERR_BWD_MATH))) break;
         tcFenceAfter();
         {
@@ -920,6 +902,15 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
 #pragma unroll
           for (int x = 0; x < kCols / 32; x++) tmemLoad32(base + C::kDp + cols + x * 32, d[x]);
           tmemLoadWait();
+          if constexpr (SIDE == kKeys) {
+#pragma unroll
+            for (int x = 0; x < kCols / 32; x++) {
+              uint32_t o[16];
+#pragma unroll
+              for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
+              tmemStore16(base + C::kDp + cols + x * 16, o);
+            }
+          }
           const auto gradients = [&](auto all) {
 #pragma unroll
             for (int x = 0; x < kCols / 32; x++) {
@@ -931,7 +922,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
                 if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
                 o[e] = pack2(v);
               }
-              tmemStore16(base + C::kDp + cols + x * 16, o);
+              tmemStore16(base + C::kDp + cols + (SIDE == kKeys ? 32 : 0) + x * 16, o);
             }
           };
           if (every) gradients(std::true_type{});
