@@ -57,10 +57,11 @@ template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
   p.tiles = (a.S + 2 * kTile - 1) / (2 * kTile);
   p.err = gemm::errWord();
   if (!p.err) return cudaErrorMemoryAllocation;
-  p.items = (long long)p.tiles * a.B * a.H;
+  const long long items = (long long)p.tiles * a.B * a.H;
+  p.items = (uint32_t)items;
   p.wide = wide(a.out) && (!a.rest.p || wide(a.rest)) && a.D % 16 == 0;
-  const int ctas = (int)(p.items < gemm::smCount() ? p.items : gemm::smCount());  // one per SM
-  if (p.items > 0x7fffffffLL || !headMap(&p.q, a.q, a.B, a.H, a.S, a.D) || !headMap(&p.k, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.v, a.v, a.B, a.KV, a.S, a.D))
+  const int ctas = (int)(items < gemm::smCount() ? items : gemm::smCount());  // one per SM
+  if (items > 0x3fffffffLL || !headMap(&p.q, a.q, a.B, a.H, a.S, a.D) || !headMap(&p.k, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.v, a.v, a.B, a.KV, a.S, a.D))
     return cudaErrorInvalidValue;
   const cudaError_t e = allowSmem(forwardKernel<HD>, FwdCfg<HD>::kSmem, done);
   if (e != cudaSuccess) return e;
@@ -97,18 +98,20 @@ template <int HD> static cudaError_t backward(const Args& a, float* partials, cu
   p.partials = partials;
   p.wide = a.D % 16 == 0 && wide(a.dq) && wide(a.dk) && wide(a.dv);
   BwdParams k = p;
-  p.items = (long long)p.tiles * a.B * a.H;
-  k.items = (long long)(p.tiles + p.sinkTiles * p.farCount) * a.B * a.KV;
-  if (p.items > 0x7fffffffLL || k.items > 0x7fffffffLL || a.B * (long long)a.KV > 65535 || !headMap(&p.x1, a.q, a.B, a.H, a.S, a.D) ||
-      !headMap(&p.x2, a.dout, a.B, a.H, a.S, a.D) || !headMap(&p.y1, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.y2, a.v, a.B, a.KV, a.S, a.D))
+  const long long itemsQ = (long long)p.tiles * a.B * a.H, itemsK = (long long)(p.tiles + p.sinkTiles * p.farCount) * a.B * a.KV;
+  p.items = (uint32_t)itemsQ;
+  k.items = (uint32_t)itemsK;
+  if (itemsQ > 0x3fffffffLL || itemsK > 0x3fffffffLL || a.B * (long long)a.KV > 65535 || !headMap(&p.x1, a.q, a.B, a.H, a.S, a.D) ||
+      !headMap(&p.x2, a.dout, a.B, a.H, a.S, a.D) || !headMap(&p.y1, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.y2, a.v, a.B, a.KV, a.S, a.D) ||
+      !headMap(&p.out, a.out, a.B, a.H, a.S, a.D) || !headMap(&p.rest, a.rest, a.B, a.H, a.S, a.D))
     return cudaErrorInvalidValue;
   k.x1 = p.y1, k.x2 = p.y2, k.y1 = p.x1, k.y2 = p.x2;
   cudaError_t e = allowSmem(backwardKernel<HD, kQueries>, Q::kSmem, doneQ);
   if (e == cudaSuccess) e = allowSmem(backwardKernel<HD, kKeys>, K::kSmem, doneK);
   if (e != cudaSuccess) return e;
   const auto ctas = [](long long items) { return (unsigned)(items < gemm::smCount() ? items : gemm::smCount()); };  // one per SM
-  backwardKernel<HD, kQueries><<<ctas(p.items), Q::kThreads, Q::kSmem, s>>>(p);
-  backwardKernel<HD, kKeys><<<ctas(k.items), K::kThreads, K::kSmem, s>>>(k);
+  backwardKernel<HD, kQueries><<<ctas(itemsQ), Q::kThreads, Q::kSmem, s>>>(p);
+  backwardKernel<HD, kKeys><<<ctas(itemsK), K::kThreads, K::kSmem, s>>>(k);
   if (p.sinkTiles) joinSinks<<<dim3(a.sinks, a.B * a.KV), 128, 0, s>>>(k);
   return cudaGetLastError();
 }

@@ -32,7 +32,7 @@ struct FwdParams {
   Args a;
   float c;              // scores' factor in powers of two, never zero
   int tiles;            // pairs of query tiles
-  long long items;      // pairs of all heads
+  uint32_t items;       // pairs of all heads
   bool wide;            // rows of out and rest start on 32-byte boundaries and are whole 32-byte pieces
   int* err;
 };
@@ -70,7 +70,7 @@ template <int HD> struct FwdCfg {
 };
 
 // What a persistent CTA does in its turn `k`: items are sorted by falling cost, so every other turn goes through the CTAs backwards.
-__device__ __forceinline__ long long itemOf(int k) { return (long long)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
+__device__ __forceinline__ uint32_t itemOf(uint32_t k) { return k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
 
 // Zeroes rows [from, ROWS) of a tile of BOXES boxes of ROWS rows x 128 bytes, by a whole warp: a weight of zero does not silence what may lie
 // behind a sequence's end, so it must not be there where the tensor cores sum over a tile's rows.
@@ -143,11 +143,11 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     int h, b, kh, r0, L, count, nSinks;
     bool two;
     KeyRange own0, own1;
-    __device__ Item(const FwdParams& p, long long item) : own0(p.a, 0, 0), own1(p.a, 0, 0) {
+    __device__ Item(const FwdParams& p, uint32_t item) : own0(p.a, 0, 0), own1(p.a, 0, 0) {
       const Args& a = p.a;
-      const int heads = a.B * a.H, bh = (int)(item % heads);
-      h = bh % a.H;
-      b = bh / a.H;
+      const uint32_t heads = a.B * a.H, bh = item % heads;
+      h = bh % (uint32_t)a.H;
+      b = bh / (uint32_t)a.H;
       kh = h / a.group();
       r0 = (p.tiles - 1 - (int)(item / heads)) * 2 * kTile;  // the longest rows first
       L = lengthOf(a, b);
@@ -452,12 +452,13 @@ enum Side { kQueries, kKeys };
 
 struct BwdParams {
   CUtensorMap x1, x2, y1, y2;
+  CUtensorMap out, rest;   // queries
   Args a;
   float c;
   int tiles;      // 128-row tiles of a sequence
   int sinkTiles;  // key tiles whose far queries are split off; 0: none
   int farChunk, farCount;  // query tiles per split, splits per sink tile
-  long long items;
+  uint32_t items;
   bool wide;               // rows of the gradients start on 32-byte boundaries and are whole 32-byte pieces
   float* partials;         // [B * KV][sinkTiles][1 + farCount][dK, dV][min(sinks, 128)][D]
   int* err;
@@ -500,12 +501,13 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
   // Rows [x0, x0 + 128) of head xh against `yTiles` streamed tiles (queries: the sinks' first) of `group` heads from yh on.
   struct Item {
     int b, xh, bh, L, xTile, x0, far, yFirst, yTiles, sinkTiles, yh, count, partRows;
-    __device__ Item(const BwdParams& p, long long item) {
+    __device__ Item(const BwdParams& p, uint32_t item) {
       const Args& a = p.a;
-      const int xHeads = SIDE == kQueries ? a.H : a.KV, all = a.B * xHeads, turn = (int)(item / all);
-      bh = (int)(item % all);
-      xh = bh % xHeads;
-      b = bh / xHeads;
+      const uint32_t xHeads = SIDE == kQueries ? a.H : a.KV, all = a.B * xHeads;
+      const int turn = item / all;
+      bh = item % all;
+      xh = (uint32_t)bh % xHeads;
+      b = (uint32_t)bh / xHeads;
       L = lengthOf(a, b);
       far = -1;
       sinkTiles = partRows = 0;
@@ -562,6 +564,10 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
     prefetchTensorMap(&p.x2);
     prefetchTensorMap(&p.y1);
     prefetchTensorMap(&p.y2);
+    if (SIDE == kQueries) {
+      prefetchTensorMap(&p.out);
+      prefetchTensorMap(&p.rest);
+    }
     mbarInit(xFull, 1);
     mbarInit(xEmpty, SIDE == kQueries ? 8 : 1);
     mbarInit(xReady, SIDE == kQueries ? 9 : 1);
@@ -613,6 +619,17 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           tmaLoad4d(smemX + C::kTileBytes + x * kBox, &p.x2, x * 64, it.x0, it.xh, it.b, xFull);
         }
         int tile = it.firstTile(), h = it.yh;
+        // Queries: the answer and what rounding took from it take the place of X when that is in tensor memory, delta is made of them; behind as many
+        // streamed tiles as the ring takes meanwhile.
+        const auto answer = [&]() {
+          if (!(ok = mbarWait(xEmpty, turn, err, ERR_BWD_LOAD))) return;
+          turn ^= 1;
+          mbarArriveExpectTx(xFull, 2 * C::kTileBytes);
+          for (int x = 0; x < C::kBoxes; x++) {
+            tmaLoad4d(smemX + x * kBox, &p.out, x * 64, it.x0, it.xh, it.b, xFull);
+            tmaLoad4d(smemX + C::kTileBytes + x * kBox, &p.rest, x * 64, it.x0, it.xh, it.b, xFull);
+          }
+        };
         for (int n = 0; n < it.count && ok; n++, g++) {
           const int y0 = tile * kTile;
           if constexpr (SIDE == kKeys) {  // first, as its place is free long before the tiles'
@@ -628,6 +645,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           }
           tile = it.nextTile(tile);
           if (SIDE == kKeys && tile == it.yFirst) h++;
+          if (SIDE == kQueries && ok && n == min(1, it.count - 1)) answer();
         }
       }
       if (!ok) {  // let loads in flight land
@@ -771,16 +789,19 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       }
       return k;
     };
+    // Words [4 i, 4 i + 4) of this thread's half of its row of X1 or X2 in shared memory.
+    const auto rowWords = [&](int x, int i) {
+      const uint8_t* row = smemX + x * C::kTileBytes + (HD == 128 ? side * kBox : 0) + r * 128;
+      return *reinterpret_cast<const uint4*>(row + ((((HD == 128 ? 0 : side * 4) + i) ^ (r & 7)) << 4));
+    };
     const auto copyX = [&]() {  // this thread's halves of X1's and X2's row to tensor memory
       if (!mbarWait(xFull, xPhase, err, ERR_BWD_MATH)) return false;
       xPhase ^= 1;
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-        const uint8_t* row = smemX + x * C::kTileBytes + (HD == 128 ? side * kBox : 0) + r * 128;
-        const int chunk0 = HD == 128 ? 0 : side * 4;
 #pragma unroll
         for (int i = 0; i < kWords; i += 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(row + (((chunk0 + i / 4) ^ (r & 7)) << 4));
+          const uint4 v = rowWords(x, i / 4);
           mine[i] = v.x, mine[i + 1] = v.y, mine[i + 2] = v.z, mine[i + 3] = v.w;
         }
 #pragma unroll
@@ -809,23 +830,20 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       float lse = 0.f, delta = 0.f;
       if constexpr (SIDE == kQueries) {
         const size_t at = (size_t)it.bh * a.padded() + row;
-        if (live) {
-          lse = a.lse[at];
-          const uint4* o = reinterpret_cast<const uint4*>(a.out.at(it.b, it.xh, row));
-          const uint4* e = reinterpret_cast<const uint4*>(a.rest.at(it.b, it.xh, row));
+        if (live) lse = a.lse[at];
+        if (!(ok = mbarWait(xFull, xPhase, err, ERR_BWD_MATH))) break;
+        xPhase ^= 1;
 #pragma unroll
-          for (int n = 0; n < HD / 16; n++) {
-            const int c = side * (HD / 16) + n;
-            if (c * 8 < a.D) {
-              float x[8], y[8], z[8];
-              unpack8(o[c], x);
-              unpack8(e[c], y);
-              unpack8(make_uint4(mine[4 * n], mine[4 * n + 1], mine[4 * n + 2], mine[4 * n + 3]), z);
+        for (int n = 0; n < kWords / 4; n++) {
+          float x[8], y[8], z[8];
+          unpack8(rowWords(0, n), x);
+          unpack8(rowWords(1, n), y);
+          unpack8(make_uint4(mine[4 * n], mine[4 * n + 1], mine[4 * n + 2], mine[4 * n + 3]), z);
 #pragma unroll
-              for (int i = 0; i < 8; i++) delta += (x[i] + y[i]) * z[i];
-            }
-          }
+          for (int i = 0; i < 8; i++) delta += (x[i] + y[i]) * z[i];
         }
+        __syncwarp();
+        if (lane == 0) mbarArrive(xEmpty);
         half[side * kTile + r] = delta;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         delta = half[r] + half[kTile + r];
