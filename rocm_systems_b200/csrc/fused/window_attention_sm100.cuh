@@ -1,10 +1,10 @@
 // Windowed attention on the 5th-generation tensor cores.
 //
 // Forward: a persistent CTA takes pairs of 128-query tiles of a head and walks the 128-key tiles that either of them sees (the sinks', then
-// the window's). Warp 8 feeds queries, and keys and values through a ring of TMA tiles; warp 9 issues S = Q K^T into tensor memory and, once
-// the softmax is through with it, O += P V with P read from tensor memory as well; warps 0-3 and 4-7 are the two tiles' softmax, one
-// thread per row, so that row maxima and sums need no exchange. P (bf16) takes the place of the scores it was made of. While one tile's
-// softmax runs, the tensor cores work for the other; while a pair's answer is written, the next pair's first scores are made.
+// the window's). One warp feeds queries, and keys and values through a ring of TMA tiles; one issues S = Q K^T into tensor memory and, once
+// the softmax is through with it, O += P V with P read from tensor memory as well; eight warps for each of the two tiles are its softmax, two
+// threads per row. P (bf16) takes the place of the scores it was made of. While one tile's softmax runs, the tensor cores work for the other;
+// while a pair's answer is written, the next pair's first scores are made.
 //
 // The running maximum is moved, and O in tensor memory scaled down, only when a row's maximum has grown by more than 2^kSlack: weights stay
 // below 2^kSlack, which costs no precision in bf16 and fp32, and O is hardly ever touched in between.
@@ -59,12 +59,14 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
 }
 
 template <int HD> struct FwdCfg {
-  static constexpr int kThreads = 384;                   // launched with 168 registers each, split as 2 x 128 x 216 and 128 x 64
-  static constexpr int kMathRegs = 216, kOtherRegs = 64;
-  static constexpr int kSlots = HD == 128 ? 5 : 8;       // key and value tiles in turn
+  static constexpr int kMath = 16;                       // warps 0-7 and 8-15 are the two tiles' softmax
+  static constexpr int kThreads = 32 * (kMath + 4);      // launched with 96 registers each, split as 4 x 128 x 104 and 128 x 64
+  static constexpr int kMathRegs = 104, kOtherRegs = 64;
+  static constexpr int kSlots = HD == 128 ? 4 : 8;       // key and value tiles in turn
   static constexpr int kBoxes = HD / 64;
   static constexpr uint32_t kTileBytes = kBoxes * kBox;
-  static constexpr size_t kSmem = 1024 + (2 + kSlots) * kTileBytes + 256;
+  static constexpr uint32_t kMeet = 2 * 2 * kTile * 4;   // what a row's two threads tell each other
+  static constexpr size_t kSmem = 1024 + (2 + kSlots) * kTileBytes + kMeet + 256;
   static constexpr uint32_t kTmemS = 0, kTmemO = 256;    // columns: S0, S1 (128 each), O0, O1 (HD each)
   static constexpr uint32_t kTmemCols = 512;
 };
@@ -81,8 +83,9 @@ template <int BOXES, int ROWS> __device__ __forceinline__ void zeroRows(uint8_t*
   sm100::fenceProxyAsync();
 }
 
-// Rows [row0, row0 + 128) of a head to zeros, from warps 0-3 or 4-7.
+// Rows [row0, row0 + 128) of a head to zeros, by 128 threads.
 __device__ __forceinline__ void zeroOut(const Tensor& t, int b, int h, int row0, int S, int D, int tid) {
+  if (!t.p) return;
   for (int n = tid; n < kTile * (D / 8); n += 128) {
     const int r = row0 + n / (D / 8);
     if (r < S) reinterpret_cast<uint4*>(t.at(b, h, r))[n % (D / 8)] = make_uint4(0, 0, 0, 0);
@@ -97,7 +100,8 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   uint8_t* smemQ = smem;
   uint8_t* ring = smem + 2 * C::kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kTileBytes);
+  float* meet = reinterpret_cast<float*>(ring + C::kSlots * C::kTileBytes);  // [tile][half][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(meet + 4 * kTile);
   uint64_t *qFull = bars, *qEmpty = bars + 1;
   uint64_t* full = bars + 2;              // [kSlots]
   uint64_t* empty = full + C::kSlots;     // [kSlots]
@@ -119,9 +123,9 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     mbarInit(qEmpty, 1);
     for (int t = 0; t < 2; t++) {
       mbarInit(&sFull[t], 1);
-      mbarInit(&pReady[t], 5);
+      mbarInit(&pReady[t], 9);
       mbarInit(&oDone[t], 1);
-      mbarInit(&oFree[t], 4);
+      mbarInit(&oFree[t], 8);
     }
     for (int s = 0; s < C::kSlots; s++) {
       mbarInit(&full[s], 1);
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     }
     fenceBarrierInit();
   }
-  if (warp == 9) {
+  if (warp == C::kMath + 1) {
     tmemAlloc(tmemSlot, C::kTmemCols);
     tmemRelinquish();
   }
@@ -164,7 +168,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     __device__ bool straddles(int n) const { return L - tileOf(n) * kTile < kTile; }
   };
 
-  if (warp == 8) {
+  if (warp == C::kMath) {
     setMaxRegsDown<C::kOtherRegs>();
     if (lane == 0) {
       bool ok = true;
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         for (int s = 0; s < C::kSlots; s++) mbarWait(&full[s], 0, err, 0, 2000u);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == C::kMath + 1) {
     setMaxRegsDown<C::kOtherRegs>();
     constexpr uint32_t idescS = instrDesc(kTile, kTile, 1 /*bf16*/), idescO = instrDescMajor(kTile, HD, 1, 0, 1);
     // The whole warp walks along and one elected lane issues: what the instructions take from uniform registers is then formed there. (With
@@ -213,7 +217,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
     for (int k = 0; all && itemOf(k) < p.items; k++) {
       const Item it(p, itemOf(k));
       if (it.count == 0) continue;
-      wait(qFull, qPhase);  // and the first keys, see warp 10
+      wait(qFull, qPhase);  // and the first keys, see the next warp
       qPhase ^= 1;
       if (electOne()) {
         scores(0, slotK);
@@ -242,7 +246,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
             if (now) {
 #pragma unroll
               for (int kk = 0; kk < kTile / 16; kk++)
-                mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + kk * 8, descV + ((slotV * C::kTileBytes + kk * 2048) >> 4), idescO,
+                mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + (kk / 4) * 64 + (kk % 4) * 8, descV + ((slotV * C::kTileBytes + kk * 2048) >> 4), idescO,
                                started[t] || kk != 0);
               if (last) mmaCommit(&oDone[t]);
             }
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       }
       slotK = after(after(slotK));
     }
-  } else if (warp == 10) {
+  } else if (warp == C::kMath + 2) {
     // Looks after the landed tiles, so that the issuing warp has one barrier to wait for per step (each wait is 100 to 200 cycles of its time,
     // which the tensor cores stand still): takes part in the barriers that it waits for when the tiles of the step are there.
     setMaxRegsDown<C::kOtherRegs>();
@@ -296,43 +300,46 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
           }
       }
     }
-  } else if (warp == 11) {
+  } else if (warp == C::kMath + 3) {
     setMaxRegsDown<C::kOtherRegs>();
   } else {
     setMaxRegsUp<C::kMathRegs>();
-    const int t = warp >> 2, q4 = warp & 3, r = t * kTile + q4 * 32 + lane;
+    constexpr int kCols = kTile / 2;  // of a row's scores, this thread's
+    const int t = warp >> 3, side = warp >> 2 & 1, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t laneBase = (uint32_t)(q4 * 32) << 16;
-    const uint32_t tS = tmem + laneBase + C::kTmemS + t * kTile, tO = tmem + laneBase + C::kTmemO + t * HD;
+    const uint32_t tS = tmem + laneBase + C::kTmemS + t * kTile + side * kCols, tO = tmem + laneBase + C::kTmemO + t * HD + side * (HD / 2);
     const float slack = kSlack / p.c;
+    float *mine = meet + (2 * t + side) * kTile + r, *other = meet + (2 * t + 1 - side) * kTile + r;
+    // Both halves of a row's warps; what is told is read before the next S, or the next item, is there.
+    const auto meeting = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + q4) : "memory"); };
     uint32_t sPhase = 0, oPhase = 0;
     bool ok = true;
     for (int k = 0; ok && itemOf(k) < p.items; k++) {
       const Item it(p, itemOf(k));
-      const int rFirst = it.r0 + t * kTile, row = it.r0 + r, rLast = min(rFirst + kTile, it.L) - 1;
+      const int rFirst = it.r0 + t * kTile, row = rFirst + r, rLast = min(rFirst + kTile, it.L) - 1;
       if (rFirst >= it.L) {
-        zeroOut(a.out, it.b, it.h, rFirst, a.S, a.D, threadIdx.x & 127);
-        if (a.rest.p) zeroOut(a.rest, it.b, it.h, rFirst, a.S, a.D, threadIdx.x & 127);
+        zeroOut(side ? a.rest : a.out, it.b, it.h, rFirst, a.S, a.D, threadIdx.x & 127);
         continue;
       }
-      const KeyRange mine = t ? it.own1 : it.own0;
+      const KeyRange own = t ? it.own1 : it.own0;
       float m = -INFINITY, limit = -INFINITY, l = 0.f;
       bool any = false;
       for (int n = 0; n < it.count; n++) {
         const int tile = it.tileOf(n);
-        if (!mine.has(tile)) continue;
+        if (!own.has(tile)) continue;
+        const int j0 = tile * kTile;
+        const bool every = seesAll(a, rFirst, rLast, j0);
         if (!(ok = mbarWait(&sFull[t], sPhase, err, ERR_FWD_SOFTMAX))) break;
         sPhase ^= 1;
         tcFenceAfter();
-        const int j0 = tile * kTile;
-        const bool every = seesAll(a, rFirst, rLast, j0);
-        uint32_t s[4][32];
+        uint32_t s[2][32];
 #pragma unroll
-        for (int x = 0; x < 4; x++) tmemLoad32(tS + x * 32, s[x]);
+        for (int x = 0; x < 2; x++) tmemLoad32(tS + x * 32, s[x]);
         tmemLoadWait();
         if (!every) {
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            const uint32_t bits = maskBits(a, row, j0 + x * 32);
+          for (int x = 0; x < 2; x++) {
+            const uint32_t bits = maskBits(a, row, j0 + side * kCols + x * 32);
 #pragma unroll
             for (int e = 0; e < 32; e++)
               if (!((bits >> e) & 1)) s[x][e] = 0xff800000u;  // -inf
@@ -341,12 +348,16 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         float best[4];
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-          best[x] = __uint_as_float(s[x][0]);
+          best[x] = __uint_as_float(s[x / 2][x % 2 * 16]);
 #pragma unroll
-          for (int e = 1; e < 31; e += 2) best[x] = fmaxf(fmaxf(best[x], __uint_as_float(s[x][e])), __uint_as_float(s[x][e + 1]));
-          best[x] = fmaxf(best[x], __uint_as_float(s[x][31]));
+          for (int e = 1; e < 15; e += 2)
+            best[x] = fmaxf(fmaxf(best[x], __uint_as_float(s[x / 2][x % 2 * 16 + e])), __uint_as_float(s[x / 2][x % 2 * 16 + e + 1]));
+          best[x] = fmaxf(best[x], __uint_as_float(s[x / 2][x % 2 * 16 + 15]));
         }
-        const float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+        float top = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+        *mine = top;
+        meeting();
+        top = fmaxf(top, *other);
         const bool move = top > limit;
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? exp2Fast((m - top) * p.c) : 1.f;
@@ -355,9 +366,9 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
             limit = top + slack;
             l *= f;
           }
-          if (any) {
+          if (any) {  // this thread's half of the row's answer
 #pragma unroll 1
-            for (int x = 0; x < HD / 16; x++) {
+            for (int x = 0; x < HD / 32; x++) {
               uint32_t o[16];
               tmemLoad16(tO + x * 16, o);
               tmemLoadWait();
@@ -370,14 +381,14 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         any = true;
         const float off = m == -INFINITY ? 0.f : m * p.c;
         const F2 c2 = makeF2(p.c, p.c), off2 = makeF2(-off, -off);
-        F2 sum[4] = {makeF2(l, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f), makeF2(0.f, 0.f)};
+        F2 sum[2] = {makeF2(l, 0.f), makeF2(0.f, 0.f)};
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
+        for (int x = 0; x < 2; x++) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) {
             const F2 pr = exp2F2(fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2));
-            sum[e & 3] = addF2(sum[e & 3], pr);
+            sum[e & 1] = addF2(sum[e & 1], pr);
             w[e] = pack2(pr);
           }
           tmemStore16(tS + x * 16, w);
@@ -387,43 +398,47 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         __syncwarp();
         if (lane == 0) mbarArrive(&pReady[t]);
         float upper;
-        splitF2(addF2(addF2(sum[0], sum[1]), addF2(sum[2], sum[3])), l, upper);
+        splitF2(addF2(sum[0], sum[1]), l, upper);
         l += upper;
       }
       if (!ok || !(ok = mbarWait(&oDone[t], oPhase, err, ERR_FWD_SOFTMAX))) break;
       oPhase ^= 1;
       tcFenceAfter();
+      *mine = l;  // the other's maximum was read before the last weights were handed over
+      meeting();
+      l += *other;
       const bool live = row < it.L;
-      if (a.lse) a.lse[((size_t)it.b * a.H + it.h) * a.padded() + row] = live ? -(m * p.c + log2f(l)) : -INFINITY;
+      if (a.lse && side == 0) a.lse[((size_t)it.b * a.H + it.h) * a.padded() + row] = live ? -(m * p.c + log2f(l)) : -INFINITY;
       const float inv = live ? 1.f / l : 0.f;
 #pragma unroll
-      for (int x = 0; x < HD / 32; x++) {
+      for (int x = 0; x < HD / 64; x++) {
         uint32_t o[32], w[16];
         tmemLoad32(tO + x * 32, o);
         tmemLoadWait();
-        if (x == HD / 32 - 1) {
+        if (x == HD / 64 - 1) {
           tcFenceBefore();
           __syncwarp();
           if (lane == 0) mbarArrive(&oFree[t]);
         }
-        const int words = a.D / 2 - x * 16;
+        const int col = side * (HD / 2) + x * 32, words = (a.D - col) / 2;
 #pragma unroll
         for (int e = 0; e < 32; e++) o[e] = live ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
 #pragma unroll
         for (int e = 0; e < 16; e++) w[e] = pack2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-        if (row < a.S) storeRow16(a.out.at(it.b, it.h, row) + x * 32, w, words, p.wide);
+        if (row < a.S) storeRow16(a.out.at(it.b, it.h, row) + col, w, words, p.wide);
         if (a.rest.p) {
 #pragma unroll
           for (int e = 0; e < 16; e++)
             w[e] = pack2(__uint_as_float(o[2 * e]) - __uint_as_float(w[e] << 16), __uint_as_float(o[2 * e + 1]) - __uint_as_float(w[e] & 0xffff0000u));
-          if (row < a.S) storeRow16(a.rest.at(it.b, it.h, row) + x * 32, w, words, p.wide);
+          if (row < a.S) storeRow16(a.rest.at(it.b, it.h, row) + col, w, words, p.wide);
         }
       }
+      meeting();  // the sums are read before the next item's maxima are written
     }
   }
   tcFenceBefore();
   __syncthreads();
-  if (warp == 9) tmemDealloc(tmem, C::kTmemCols);
+  if (warp == C::kMath + 1) tmemDealloc(tmem, C::kTmemCols);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------
