@@ -18,6 +18,8 @@ using namespace rows;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4, kUnrollBack = 2;  // rows of a lane whose loads are under way together
+constexpr int kCtasPerSm = 2;                // backward
 
 struct Shape {
   long long tokens;  // batch * seq
@@ -39,10 +41,9 @@ __global__ void __launch_bounds__(kThreads) forwardKernel(const __nv_bfloat16* _
   const int lane = threadIdx.x & 31, j = lane % LANES, group = lane / LANES;
   const int half = sh.D >> 1, rot = sh.heads + sh.kv, all = rot + sh.kv;
   const bool in = 8 * j < sh.D;
-  const long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const long long t = item / sh.split;
+  const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), t = item / (uint32_t)sh.split;
   if (t >= sh.tokens) return;
-  const int part = (int)(item % sh.split);
+  const int part = item - t * sh.split;
   float w[2][8];
   float2 cs[4] = {};
   if (in) {
@@ -52,41 +53,52 @@ __global__ void __launch_bounds__(kThreads) forwardKernel(const __nv_bfloat16* _
       w[0][4 + e] = toFloat(wq[half + 4 * j + e]);
       w[1][e] = toFloat(wk[4 * j + e]);
       w[1][4 + e] = toFloat(wk[half + 4 * j + e]);
-      cs[e] = table[(size_t)(t % sh.seq) * half + 4 * j + e];
+      cs[e] = table[(size_t)(t % (uint32_t)sh.seq) * half + 4 * j + e];
     }
   }
-  for (int h0 = part * kGroups; h0 < rot; h0 += sh.split * kGroups) {
-    const int h = h0 + group;
-    const bool live = in && h < rot;
-    float a[4] = {}, b[4] = {};
-    if (live) {
-      const __nv_bfloat16* row = x + ((size_t)t * all + h) * sh.D + 4 * j;
-      unpack4(*reinterpret_cast<const uint2*>(row), a);
-      unpack4(*reinterpret_cast<const uint2*>(row + half), b);
-    }
-    float ss = 0.f;
+  const int step = sh.split * kGroups;
+  for (int h0 = part * kGroups + group; h0 - group < rot; h0 += kUnroll * step) {
+    uint2 raw[kUnroll][2];
 #pragma unroll
-    for (int e = 0; e < 4; e++) ss += a[e] * a[e] + b[e] * b[e];
-    const float r = rsqrtf(laneSum<LANES>(ss) / (float)sh.D + sh.eps);
-    if (live) {
-      const int which = h >= sh.heads;
-      float ya[4], yb[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float na = a[e] * r * (which ? w[1][e] : w[0][e]), nb = b[e] * r * (which ? w[1][4 + e] : w[0][4 + e]);
-        ya[e] = na * cs[e].x - nb * cs[e].y;
-        yb[e] = nb * cs[e].x + na * cs[e].y;
+    for (int u = 0; u < kUnroll; u++) {
+      const int h = h0 + u * step;
+      raw[u][0] = raw[u][1] = make_uint2(0, 0);
+      if (in && h < rot) {
+        const __nv_bfloat16* row = x + ((size_t)t * all + h) * sh.D + 4 * j;
+        raw[u][0] = *reinterpret_cast<const uint2*>(row);
+        raw[u][1] = *reinterpret_cast<const uint2*>(row + half);
       }
-      __nv_bfloat16* out = (which ? k + ((size_t)t * sh.kv + h - sh.heads) * sh.D : q + ((size_t)t * sh.heads + h) * sh.D) + 4 * j;
-      *reinterpret_cast<uint2*>(out) = pack4(ya);
-      *reinterpret_cast<uint2*>(out + half) = pack4(yb);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      const int h = h0 + u * step;
+      float a[4], b[4];
+      unpack4(raw[u][0], a);
+      unpack4(raw[u][1], b);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; e++) ss += a[e] * a[e] + b[e] * b[e];
+      const float r = rsqrtf(laneSum<LANES>(ss) / (float)sh.D + sh.eps);
+      if (in && h < rot) {
+        const int which = h >= sh.heads;
+        float ya[4], yb[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float na = a[e] * r * (which ? w[1][e] : w[0][e]), nb = b[e] * r * (which ? w[1][4 + e] : w[0][4 + e]);
+          ya[e] = na * cs[e].x - nb * cs[e].y;
+          yb[e] = nb * cs[e].x + na * cs[e].y;
+        }
+        __nv_bfloat16* out = (which ? k + ((size_t)t * sh.kv + h - sh.heads) * sh.D : q + ((size_t)t * sh.heads + h) * sh.D) + 4 * j;
+        *reinterpret_cast<uint2*>(out) = pack4(ya);
+        *reinterpret_cast<uint2*>(out + half) = pack4(yb);
+      }
     }
   }
 }
 
 // partials [CTAs][2][D]: every CTA's share of the weights' gradients, summed by weightSum in a fixed order.
 template <int LANES, typename W>
-__global__ void __launch_bounds__(kThreads) backwardKernel(Grad dq, Grad dk, Grad dv, const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq,
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) backwardKernel(Grad dq, Grad dk, Grad dv, const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq,
                                                            const W* __restrict__ wk, const float2* __restrict__ table, __nv_bfloat16* __restrict__ dx,
                                                            float* __restrict__ partials, Shape sh) {
   constexpr int kGroups = 32 / LANES;
@@ -104,65 +116,73 @@ __global__ void __launch_bounds__(kThreads) backwardKernel(Grad dq, Grad dk, Gra
       w[1][4 + e] = toFloat(wk[half + 4 * j + e]);
     }
   }
-  const long long items = sh.tokens * sh.split;
-  for (long long item = (long long)blockIdx.x * kWarps + warp; item < items; item += (long long)gridDim.x * kWarps) {
-    const long long t = item / sh.split, batch = t / sh.seq;
-    const int pos = (int)(t % sh.seq);
+  const uint32_t items = (uint32_t)sh.tokens * sh.split;
+  for (uint32_t item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
+    const uint32_t t = item / (uint32_t)sh.split, batch = t / (uint32_t)sh.seq;
+    const int pos = t - batch * sh.seq;
     float2 cs[4] = {};
     if (in)
 #pragma unroll
       for (int e = 0; e < 4; e++) cs[e] = table[(size_t)pos * half + 4 * j + e];
-    for (int h0 = (int)(item % sh.split) * kGroups; h0 < all; h0 += sh.split * kGroups) {
-      const int h = h0 + group;
-      const bool live = in && h < all;
-      const int which = h < sh.heads ? 0 : h < rot ? 1 : 2;
-      float a[4] = {}, b[4] = {}, ga[4] = {}, gb[4] = {};
-      uint2 rawA = make_uint2(0, 0), rawB = make_uint2(0, 0);
-      const size_t off = ((size_t)t * all + h) * sh.D + 4 * j;
-      if (live) {
-        const __nv_bfloat16* g = (which == 0 ? dq.at(batch, h, pos) : which == 1 ? dk.at(batch, h - sh.heads, pos) : dv.at(batch, h - rot, pos)) + 4 * j;
-        rawA = *reinterpret_cast<const uint2*>(g);
-        rawB = *reinterpret_cast<const uint2*>(g + half);
-        if (which < 2) {
-          unpack4(*reinterpret_cast<const uint2*>(x + off), a);
-          unpack4(*reinterpret_cast<const uint2*>(x + off + half), b);
-          float ya[4], yb[4];
-          unpack4(rawA, ya);
-          unpack4(rawB, yb);
+    const int step = sh.split * kGroups;
+    for (int h0 = (item - t * sh.split) * kGroups + group; h0 - group < all; h0 += kUnrollBack * step) {
+      uint2 grad[kUnrollBack][2], row[kUnrollBack][2];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            ga[e] = ya[e] * cs[e].x + yb[e] * cs[e].y;
-            gb[e] = yb[e] * cs[e].x - ya[e] * cs[e].y;
+      for (int u = 0; u < kUnrollBack; u++) {
+        const int h = h0 + u * step;
+        grad[u][0] = grad[u][1] = row[u][0] = row[u][1] = make_uint2(0, 0);
+        if (in && h < all) {
+          const __nv_bfloat16* g = (h < sh.heads ? dq.at(batch, h, pos) : h < rot ? dk.at(batch, h - sh.heads, pos) : dv.at(batch, h - rot, pos)) + 4 * j;
+          grad[u][0] = *reinterpret_cast<const uint2*>(g);
+          grad[u][1] = *reinterpret_cast<const uint2*>(g + half);
+          if (h < rot) {
+            const __nv_bfloat16* p = x + ((size_t)t * all + h) * sh.D + 4 * j;
+            row[u][0] = *reinterpret_cast<const uint2*>(p);
+            row[u][1] = *reinterpret_cast<const uint2*>(p + half);
           }
         }
       }
-      const int wi = which & 1;
-      float ss = 0.f, dot = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        ss += a[e] * a[e] + b[e] * b[e];
-        dot += ga[e] * (wi ? w[1][e] : w[0][e]) * a[e] + gb[e] * (wi ? w[1][4 + e] : w[0][4 + e]) * b[e];
-      }
-      const float r = rsqrtf(laneSum<LANES>(ss) / (float)sh.D + sh.eps);
-      const float c = laneSum<LANES>(dot) * r * r / (float)sh.D;
-      if (live && which < 2) {
-        float oa[4], ob[4];
+      for (int u = 0; u < kUnrollBack; u++) {
+        const int h = h0 + u * step;
+        const bool key = h >= sh.heads, rotated = h < rot;  // (values: all sums below are zeros)
+        float a[4], b[4], ya[4], yb[4], ga[4], gb[4], wa[4], wb[4];
+        unpack4(row[u][0], a);
+        unpack4(row[u][1], b);
+        unpack4(grad[u][0], ya);
+        unpack4(grad[u][1], yb);
+        float ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          oa[e] = r * (ga[e] * (wi ? w[1][e] : w[0][e]) - a[e] * c);
-          ob[e] = r * (gb[e] * (wi ? w[1][4 + e] : w[0][4 + e]) - b[e] * c);
-          const float da = ga[e] * a[e] * r, db = gb[e] * b[e] * r;
-          dw[0][e] += which == 0 ? da : 0.f;
-          dw[0][4 + e] += which == 0 ? db : 0.f;
-          dw[1][e] += which == 1 ? da : 0.f;
-          dw[1][4 + e] += which == 1 ? db : 0.f;
+          ga[e] = ya[e] * cs[e].x + yb[e] * cs[e].y;
+          gb[e] = yb[e] * cs[e].x - ya[e] * cs[e].y;
+          wa[e] = key ? w[1][e] : w[0][e];
+          wb[e] = key ? w[1][4 + e] : w[0][4 + e];
+          ss += a[e] * a[e] + b[e] * b[e];
+          dot += ga[e] * wa[e] * a[e] + gb[e] * wb[e] * b[e];
         }
-        rawA = pack4(oa);
-        rawB = pack4(ob);
-      }
-      if (live) {
-        *reinterpret_cast<uint2*>(dx + off) = rawA;
-        *reinterpret_cast<uint2*>(dx + off + half) = rawB;
+        const float r = rsqrtf(laneSum<LANES>(ss) / (float)sh.D + sh.eps);
+        const float c = laneSum<LANES>(dot) * r * r / (float)sh.D;
+        if (in && h < all) {
+          if (rotated) {
+            float oa[4], ob[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              oa[e] = r * (ga[e] * wa[e] - a[e] * c);
+              ob[e] = r * (gb[e] * wb[e] - b[e] * c);
+              const float da = ga[e] * a[e] * r, db = gb[e] * b[e] * r;
+              dw[0][e] += key ? 0.f : da;
+              dw[0][4 + e] += key ? 0.f : db;
+              dw[1][e] += key ? da : 0.f;
+              dw[1][4 + e] += key ? db : 0.f;
+            }
+            grad[u][0] = pack4(oa);
+            grad[u][1] = pack4(ob);
+          }
+          __nv_bfloat16* out = dx + ((size_t)t * all + h) * sh.D + 4 * j;
+          *reinterpret_cast<uint2*>(out) = grad[u][0];
+          *reinterpret_cast<uint2*>(out + half) = grad[u][1];
+        }
       }
     }
   }
@@ -227,18 +247,18 @@ template <int LANES, typename W>
 cudaError_t forward(const void* x, const void* wq, const void* wk, const float* table, void* q, void* k, Shape sh, cudaStream_t s) {
   sh.split = splitFor(sh.tokens, sh.heads + sh.kv, 32 / LANES);
   const long long ctas = (sh.tokens * sh.split + kWarps - 1) / kWarps;
-  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (ctas * kWarps > 0x7fffffffLL) return cudaErrorInvalidValue;
   forwardKernel<LANES, W><<<(unsigned)ctas, kThreads, 0, s>>>((const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)q,
                                                              (__nv_bfloat16*)k, sh);
   return cudaGetLastError();
 }
 
-constexpr int kCtasPerSm = 2;
 template <int LANES, typename W>
 cudaError_t backward(Grad dq, Grad dk, Grad dv, const void* x, const void* wq, const void* wk, const float* table, void* dx, float* partials, void* dwq, void* dwk,
                      Shape sh, cudaStream_t s) {
   sh.split = splitFor(sh.tokens, sh.heads + 2 * sh.kv, 32 / LANES);
   const long long need = (sh.tokens * sh.split + kWarps - 1) / kWarps;
+  if (need * kWarps > 0x3fffffffLL) return cudaErrorInvalidValue;
   const int ctas = (int)(need < kCtasPerSm * smCount() ? need : kCtasPerSm * smCount());
   backwardKernel<LANES, W><<<ctas, kThreads, 0, s>>>(dq, dk, dv, (const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)dx, partials, sh);
   weightSum<W><<<(2 * sh.D + 31) / 32, 1024, 0, s>>>(partials, (W*)dwq, (W*)dwk, ctas, sh.D);

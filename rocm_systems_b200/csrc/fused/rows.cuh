@@ -45,6 +45,28 @@ __device__ __forceinline__ F2 exp2F2(F2 x) {
   splitF2(x, a, b);
   return makeF2(exp2Fast(a), exp2Fast(b));
 }
+// 2^x without the special-function unit, whose 16 results per clock and SM are what a softmax runs out of first: x = n + f with n the nearest
+// whole number (added and taken off again at a scale where fp32 has no fraction left), 2^f for |f| <= 1/2 by the polynomial of degree 4
+// with the smallest largest relative error (2.7e-6; Remez exchange), n added to its exponent. Below -126 the result is 2^-126; a NaN stays
+// something that is not finite or larger than any weight.
+__device__ __forceinline__ F2 exp2Poly(F2 x) {
+  float a, b;
+  splitF2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = makeF2(a, b);
+  const auto both = [](float v) { return makeF2(v, v); };
+  const F2 n = addF2(x, both(12582912.f));  // 1.5 * 2^23
+  const F2 f = fmaF2(addF2(n, both(-12582912.f)), both(-1.f), x);
+  F2 p = fmaF2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+  p = fmaF2(p, f, both(0.240247443318367f));
+  p = fmaF2(p, f, both(0.6931217908859253f));
+  p = fmaF2(p, f, both(0.9999992847442627f));
+  float na, nb;
+  splitF2(n, na, nb);
+  splitF2(p, a, b);
+  return makeF2(__int_as_float(__float_as_int(a) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(nb) << 23)));
+}
 // Two bf16 values of a 32-bit word.
 __device__ __forceinline__ F2 unpackF2(uint32_t w) { return makeF2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
