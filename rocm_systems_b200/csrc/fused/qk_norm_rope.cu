@@ -6,10 +6,13 @@
 //             has to be read anyway. The values' gradient is copied beside them, so that one launch writes the whole packed gradient.
 //
 // A head's row belongs to 8, 16 or 32 lanes; lane j holds elements [4j, 4j + 4) and their partners at + D / 2, so the rotation needs no
-// exchange and the sums take three to five shuffles. A warp stays with one token, whose cosines and sines it keeps in registers, and walks a
-// share of its heads.
-// Both directions are bound by memory traffic.
+// exchange and the sums take three to five shuffles. A warp stays with a few heads of one kind, whose weights (and the sums of their
+// gradients) it keeps in registers, and goes from token to token; the rows of a token's heads are loaded together, as what bounds both
+// directions is how many loads are under way: with one row at a time the backward pass took 59 us where it moves 142 MB (4096 tokens, 32/8
+// heads of 128).
 #include "rows.cuh"
+
+#include <type_traits>
 
 namespace b200 {
 namespace qkn {
@@ -18,13 +21,12 @@ using namespace rows;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 4, kUnrollBack = 2;  // rows of a lane whose loads are under way together
-constexpr int kCtasPerSm = 2;                // backward
+constexpr int kUnrollFwd = 4, kUnrollBwd = 2;  // rows of a lane whose loads are under way together
+constexpr int kCtasFwd = 3, kCtasBwd = 3;  // per SM
 
 struct Shape {
-  long long tokens;  // batch * seq
-  int seq, heads, kv, D;
-  int split;         // warps that share a token's heads
+  uint32_t tokens, seq;  // tokens = batch * seq
+  int heads, kv, D;
   float eps;
 };
 // Element strides of a gradient [batch, heads, seq, D] whose last dimension is dense.
@@ -34,44 +36,64 @@ struct Grad {
   __device__ const __nv_bfloat16* at(long long batch, int head, int pos) const { return p + batch * b + head * h + pos * s; }
 };
 
+// The heads that a warp stays with, and its tokens: kind 0 queries, 1 keys, 2 values.
+template <int LANES, int kUnroll> struct Share {
+  static constexpr int kHeads = 32 / LANES * kUnroll;
+  int kind, first, end, before;  // heads [first, end) of the kind; heads of a token before the kind's
+  uint32_t token, step;
+  __host__ __device__ static int count(int heads, int kv, bool values) { return (heads + kHeads - 1) / kHeads + (values ? 2 : 1) * ((kv + kHeads - 1) / kHeads); }
+  __device__ Share(const Shape& sh, bool values) {
+    const uint32_t n = count(sh.heads, sh.kv, values), warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int nq = (sh.heads + kHeads - 1) / kHeads, nk = (sh.kv + kHeads - 1) / kHeads;
+    step = gridDim.x * kWarps / n;
+    token = warp / n;
+    int c = warp - token * n;
+    if (token >= step) token = sh.tokens;  // a warp that is left over
+    kind = c < nq ? 0 : c < nq + nk ? 1 : 2;
+    c -= kind == 0 ? 0 : kind == 1 ? nq : nq + nk;
+    first = c * kHeads;
+    end = min(first + kHeads, kind == 0 ? sh.heads : sh.kv);
+    before = kind == 0 ? 0 : kind == 1 ? sh.heads : sh.heads + sh.kv;
+  }
+};
+
 template <int LANES, typename W>
-__global__ void __launch_bounds__(kThreads) forwardKernel(const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq, const W* __restrict__ wk,
-                                                          const float2* __restrict__ table, __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ k, Shape sh) {
+__global__ void __launch_bounds__(kThreads, kCtasFwd) forwardKernel(const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq, const W* __restrict__ wk,
+                                                                    const float2* __restrict__ table, __nv_bfloat16* __restrict__ q,
+                                                                    __nv_bfloat16* __restrict__ k, Shape sh) {
   constexpr int kGroups = 32 / LANES;
-  const int lane = threadIdx.x & 31, j = lane % LANES, group = lane / LANES;
-  const int half = sh.D >> 1, rot = sh.heads + sh.kv, all = rot + sh.kv;
+  const int lane = threadIdx.x & 31, j = lane % LANES, group = lane / LANES, half = sh.D >> 1, all = sh.heads + 2 * sh.kv;
   const bool in = 8 * j < sh.D;
-  const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), t = item / (uint32_t)sh.split;
-  if (t >= sh.tokens) return;
-  const int part = item - t * sh.split;
-  float w[2][8];
-  float2 cs[4] = {};
-  if (in) {
+  const Share<LANES, kUnrollFwd> mine(sh, false);
+  const W* w = mine.kind ? wk : wq;
+  float wa[4] = {}, wb[4] = {};
+  if (in)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      w[0][e] = toFloat(wq[4 * j + e]);
-      w[0][4 + e] = toFloat(wq[half + 4 * j + e]);
-      w[1][e] = toFloat(wk[4 * j + e]);
-      w[1][4 + e] = toFloat(wk[half + 4 * j + e]);
-      cs[e] = table[(size_t)(t % (uint32_t)sh.seq) * half + 4 * j + e];
+      wa[e] = toFloat(w[4 * j + e]);
+      wb[e] = toFloat(w[half + 4 * j + e]);
     }
-  }
-  const int step = sh.split * kGroups;
-  for (int h0 = part * kGroups + group; h0 - group < rot; h0 += kUnroll * step) {
-    uint2 raw[kUnroll][2];
+  __nv_bfloat16* const to = mine.kind ? k : q;
+  const int toHeads = mine.kind ? sh.kv : sh.heads;
+  for (uint32_t t = mine.token; t < sh.tokens; t += mine.step) {
+    uint2 raw[kUnrollFwd][2];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-      const int h = h0 + u * step;
+    for (int u = 0; u < kUnrollFwd; u++) {
+      const int h = mine.first + u * kGroups + group;
       raw[u][0] = raw[u][1] = make_uint2(0, 0);
-      if (in && h < rot) {
-        const __nv_bfloat16* row = x + ((size_t)t * all + h) * sh.D + 4 * j;
+      if (in && h < mine.end) {
+        const __nv_bfloat16* row = x + ((size_t)t * all + mine.before + h) * sh.D + 4 * j;
         raw[u][0] = *reinterpret_cast<const uint2*>(row);
         raw[u][1] = *reinterpret_cast<const uint2*>(row + half);
       }
     }
+    float2 cs[4] = {};
+    if (in)
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-      const int h = h0 + u * step;
+      for (int e = 0; e < 4; e++) cs[e] = table[(size_t)(t % sh.seq) * half + 4 * j + e];
+#pragma unroll
+    for (int u = 0; u < kUnrollFwd; u++) {
+      const int h = mine.first + u * kGroups + group;
       float a[4], b[4];
       unpack4(raw[u][0], a);
       unpack4(raw[u][1], b);
@@ -79,16 +101,15 @@ __global__ void __launch_bounds__(kThreads) forwardKernel(const __nv_bfloat16* _
 #pragma unroll
       for (int e = 0; e < 4; e++) ss += a[e] * a[e] + b[e] * b[e];
       const float r = rsqrtf(laneSum<LANES>(ss) / (float)sh.D + sh.eps);
-      if (in && h < rot) {
-        const int which = h >= sh.heads;
+      if (in && h < mine.end) {
         float ya[4], yb[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float na = a[e] * r * (which ? w[1][e] : w[0][e]), nb = b[e] * r * (which ? w[1][4 + e] : w[0][4 + e]);
+          const float na = a[e] * r * wa[e], nb = b[e] * r * wb[e];
           ya[e] = na * cs[e].x - nb * cs[e].y;
           yb[e] = nb * cs[e].x + na * cs[e].y;
         }
-        __nv_bfloat16* out = (which ? k + ((size_t)t * sh.kv + h - sh.heads) * sh.D : q + ((size_t)t * sh.heads + h) * sh.D) + 4 * j;
+        __nv_bfloat16* out = to + ((size_t)t * toHeads + h) * sh.D + 4 * j;
         *reinterpret_cast<uint2*>(out) = pack4(ya);
         *reinterpret_cast<uint2*>(out + half) = pack4(yb);
       }
@@ -98,55 +119,51 @@ __global__ void __launch_bounds__(kThreads) forwardKernel(const __nv_bfloat16* _
 
 // partials [CTAs][2][D]: every CTA's share of the weights' gradients, summed by weightSum in a fixed order.
 template <int LANES, typename W>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) backwardKernel(Grad dq, Grad dk, Grad dv, const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq,
-                                                           const W* __restrict__ wk, const float2* __restrict__ table, __nv_bfloat16* __restrict__ dx,
-                                                           float* __restrict__ partials, Shape sh) {
+__global__ void __launch_bounds__(kThreads, kCtasBwd) backwardKernel(Grad dq, Grad dk, Grad dv, const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq,
+                                                                       const W* __restrict__ wk, const float2* __restrict__ table, __nv_bfloat16* __restrict__ dx,
+                                                                       float* __restrict__ partials, Shape sh) {
   constexpr int kGroups = 32 / LANES;
-  __shared__ float part[kWarps][2][8 * LANES];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane % LANES, group = lane / LANES;
-  const int half = sh.D >> 1, rot = sh.heads + sh.kv, all = rot + sh.kv;
+  __shared__ float part[kWarps][8 * LANES];
+  __shared__ int kinds[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane % LANES, group = lane / LANES, half = sh.D >> 1, all = sh.heads + 2 * sh.kv;
   const bool in = 8 * j < sh.D;
-  float w[2][8] = {}, dw[2][8] = {};
-  if (in) {
+  const Share<LANES, kUnrollBwd> mine(sh, true);
+  const W* w = mine.kind ? wk : wq;
+  const Grad from = mine.kind == 0 ? dq : mine.kind == 1 ? dk : dv;
+  float wa[4] = {}, wb[4] = {}, dwa[4] = {}, dwb[4] = {};
+  if (in && mine.kind < 2)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      w[0][e] = toFloat(wq[4 * j + e]);
-      w[0][4 + e] = toFloat(wq[half + 4 * j + e]);
-      w[1][e] = toFloat(wk[4 * j + e]);
-      w[1][4 + e] = toFloat(wk[half + 4 * j + e]);
+      wa[e] = toFloat(w[4 * j + e]);
+      wb[e] = toFloat(w[half + 4 * j + e]);
     }
-  }
-  const uint32_t items = (uint32_t)sh.tokens * sh.split;
-  for (uint32_t item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
-    const uint32_t t = item / (uint32_t)sh.split, batch = t / (uint32_t)sh.seq;
+  for (uint32_t t = mine.token; t < sh.tokens; t += mine.step) {
+    const uint32_t batch = t / sh.seq;
     const int pos = t - batch * sh.seq;
-    float2 cs[4] = {};
-    if (in)
+    uint2 grad[kUnrollBwd][2], row[kUnrollBwd][2];
 #pragma unroll
-      for (int e = 0; e < 4; e++) cs[e] = table[(size_t)pos * half + 4 * j + e];
-    const int step = sh.split * kGroups;
-    for (int h0 = (item - t * sh.split) * kGroups + group; h0 - group < all; h0 += kUnrollBack * step) {
-      uint2 grad[kUnrollBack][2], row[kUnrollBack][2];
-#pragma unroll
-      for (int u = 0; u < kUnrollBack; u++) {
-        const int h = h0 + u * step;
-        grad[u][0] = grad[u][1] = row[u][0] = row[u][1] = make_uint2(0, 0);
-        if (in && h < all) {
-          const __nv_bfloat16* g = (h < sh.heads ? dq.at(batch, h, pos) : h < rot ? dk.at(batch, h - sh.heads, pos) : dv.at(batch, h - rot, pos)) + 4 * j;
-          grad[u][0] = *reinterpret_cast<const uint2*>(g);
-          grad[u][1] = *reinterpret_cast<const uint2*>(g + half);
-          if (h < rot) {
-            const __nv_bfloat16* p = x + ((size_t)t * all + h) * sh.D + 4 * j;
-            row[u][0] = *reinterpret_cast<const uint2*>(p);
-            row[u][1] = *reinterpret_cast<const uint2*>(p + half);
-          }
+    for (int u = 0; u < kUnrollBwd; u++) {
+      const int h = mine.first + u * kGroups + group;
+      grad[u][0] = grad[u][1] = row[u][0] = row[u][1] = make_uint2(0, 0);
+      if (in && h < mine.end) {
+        const __nv_bfloat16* g = from.at(batch, h, pos) + 4 * j;
+        grad[u][0] = *reinterpret_cast<const uint2*>(g);
+        grad[u][1] = *reinterpret_cast<const uint2*>(g + half);
+        if (mine.kind < 2) {
+          const __nv_bfloat16* p = x + ((size_t)t * all + mine.before + h) * sh.D + 4 * j;
+          row[u][0] = *reinterpret_cast<const uint2*>(p);
+          row[u][1] = *reinterpret_cast<const uint2*>(p + half);
         }
       }
+    }
+    if (mine.kind < 2) {
+      float2 cs[4] = {};
+      if (in)
 #pragma unroll
-      for (int u = 0; u < kUnrollBack; u++) {
-        const int h = h0 + u * step;
-        const bool key = h >= sh.heads, rotated = h < rot;  // (values: all sums below are zeros)
-        float a[4], b[4], ya[4], yb[4], ga[4], gb[4], wa[4], wb[4];
+        for (int e = 0; e < 4; e++) cs[e] = table[(size_t)pos * half + 4 * j + e];
+#pragma unroll
+      for (int u = 0; u < kUnrollBwd; u++) {
+        float a[4], b[4], ya[4], yb[4], ga[4], gb[4];
         unpack4(row[u][0], a);
         unpack4(row[u][1], b);
         unpack4(grad[u][0], ya);
@@ -156,45 +173,45 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) backwardKernel(Grad dq, 
         for (int e = 0; e < 4; e++) {
           ga[e] = ya[e] * cs[e].x + yb[e] * cs[e].y;
           gb[e] = yb[e] * cs[e].x - ya[e] * cs[e].y;
-          wa[e] = key ? w[1][e] : w[0][e];
-          wb[e] = key ? w[1][4 + e] : w[0][4 + e];
           ss += a[e] * a[e] + b[e] * b[e];
           dot += ga[e] * wa[e] * a[e] + gb[e] * wb[e] * b[e];
         }
         const float r = rsqrtf(laneSum<LANES>(ss) / (float)sh.D + sh.eps);
         const float c = laneSum<LANES>(dot) * r * r / (float)sh.D;
-        if (in && h < all) {
-          if (rotated) {
-            float oa[4], ob[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              oa[e] = r * (ga[e] * wa[e] - a[e] * c);
-              ob[e] = r * (gb[e] * wb[e] - b[e] * c);
-              const float da = ga[e] * a[e] * r, db = gb[e] * b[e] * r;
-              dw[0][e] += key ? 0.f : da;
-              dw[0][4 + e] += key ? 0.f : db;
-              dw[1][e] += key ? da : 0.f;
-              dw[1][4 + e] += key ? db : 0.f;
-            }
-            grad[u][0] = pack4(oa);
-            grad[u][1] = pack4(ob);
-          }
-          __nv_bfloat16* out = dx + ((size_t)t * all + h) * sh.D + 4 * j;
-          *reinterpret_cast<uint2*>(out) = grad[u][0];
-          *reinterpret_cast<uint2*>(out + half) = grad[u][1];
+        for (int e = 0; e < 4; e++) {  // of a head that does not exist zeros
+          dwa[e] += ga[e] * a[e] * r;
+          dwb[e] += gb[e] * b[e] * r;
+          ga[e] = r * (ga[e] * wa[e] - a[e] * c);
+          gb[e] = r * (gb[e] * wb[e] - b[e] * c);
         }
+        grad[u][0] = pack4(ga);
+        grad[u][1] = pack4(gb);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnrollBwd; u++) {
+      const int h = mine.first + u * kGroups + group;
+      if (in && h < mine.end) {
+        __nv_bfloat16* out = dx + ((size_t)t * all + mine.before + h) * sh.D + 4 * j;
+        *reinterpret_cast<uint2*>(out) = grad[u][0];
+        *reinterpret_cast<uint2*>(out + half) = grad[u][1];
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int e = 0; e < 4; e++) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      float v = dw[i][e];
-#pragma unroll
-      for (int o = LANES; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (group == 0) part[warp][i][8 * j + e] = v;
+    for (int o = LANES; o < 32; o <<= 1) {
+      dwa[e] += __shfl_xor_sync(0xffffffffu, dwa[e], o);
+      dwb[e] += __shfl_xor_sync(0xffffffffu, dwb[e], o);
     }
+    if (group == 0) {
+      part[warp][8 * j + e] = dwa[e];
+      part[warp][8 * j + 4 + e] = dwb[e];
+    }
+  }
+  if (lane == 0) kinds[warp] = mine.kind;
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * sh.D; c += kThreads) {
     const int i = c / sh.D, d = c % sh.D;
@@ -202,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) backwardKernel(Grad dq, 
     const int slot = 8 * (dd >> 2) + 4 * hi + (dd & 3);
     float v = 0.f;
 #pragma unroll
-    for (int wp = 0; wp < kWarps; wp++) v += part[wp][i][slot];
+    for (int wp = 0; wp < kWarps; wp++) v += kinds[wp] == i ? part[wp][slot] : 0.f;
     partials[(size_t)blockIdx.x * 2 * sh.D + c] = v;
   }
 }
@@ -236,36 +253,32 @@ int smCount() {
   return n[dev] ? n[dev] : 148;
 }
 
-// Warps that share a token's heads: one, unless there are too few tokens to give every SM 32 warps.
-int splitFor(long long tokens, int heads, int groups) {
-  const long long want = 32LL * smCount(), most = (heads + groups - 1) / groups;
-  long long s = (want + tokens - 1) / tokens;
-  return (int)(s < 1 ? 1 : s > most ? most : s);
+// A warp per token and share of its heads, as long as every SM takes them all at once.
+template <typename S> unsigned ctasFor(const Shape& sh, bool values) {
+  const long long need = ((long long)sh.tokens * S::count(sh.heads, sh.kv, values) + kWarps - 1) / kWarps, most = (long long)(values ? kCtasBwd : kCtasFwd) * smCount();
+  const long long least = (S::count(sh.heads, sh.kv, values) + kWarps - 1) / kWarps;  // every share has a warp
+  return (unsigned)(need < most ? need : most > least ? most : least);
 }
 
 template <int LANES, typename W>
-cudaError_t forward(const void* x, const void* wq, const void* wk, const float* table, void* q, void* k, Shape sh, cudaStream_t s) {
-  sh.split = splitFor(sh.tokens, sh.heads + sh.kv, 32 / LANES);
-  const long long ctas = (sh.tokens * sh.split + kWarps - 1) / kWarps;
-  if (ctas * kWarps > 0x7fffffffLL) return cudaErrorInvalidValue;
-  forwardKernel<LANES, W><<<(unsigned)ctas, kThreads, 0, s>>>((const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)q,
-                                                             (__nv_bfloat16*)k, sh);
+cudaError_t forward(const void* x, const void* wq, const void* wk, const float* table, void* q, void* k, const Shape& sh, cudaStream_t s) {
+  forwardKernel<LANES, W><<<ctasFor<Share<LANES, kUnrollFwd>>(sh, false), kThreads, 0, s>>>((const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)q,
+                                                                        (__nv_bfloat16*)k, sh);
   return cudaGetLastError();
 }
 
 template <int LANES, typename W>
 cudaError_t backward(Grad dq, Grad dk, Grad dv, const void* x, const void* wq, const void* wk, const float* table, void* dx, float* partials, void* dwq, void* dwk,
-                     Shape sh, cudaStream_t s) {
-  sh.split = splitFor(sh.tokens, sh.heads + 2 * sh.kv, 32 / LANES);
-  const long long need = (sh.tokens * sh.split + kWarps - 1) / kWarps;
-  if (need * kWarps > 0x3fffffffLL) return cudaErrorInvalidValue;
-  const int ctas = (int)(need < kCtasPerSm * smCount() ? need : kCtasPerSm * smCount());
+                     const Shape& sh, cudaStream_t s) {
+  const unsigned ctas = ctasFor<Share<LANES, kUnrollBwd>>(sh, true);
   backwardKernel<LANES, W><<<ctas, kThreads, 0, s>>>(dq, dk, dv, (const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)dx, partials, sh);
-  weightSum<W><<<(2 * sh.D + 31) / 32, 1024, 0, s>>>(partials, (W*)dwq, (W*)dwk, ctas, sh.D);
+  weightSum<W><<<(2 * sh.D + 31) / 32, 1024, 0, s>>>(partials, (W*)dwq, (W*)dwk, (int)ctas, sh.D);
   return cudaGetLastError();
 }
 
-bool good(const Shape& sh) { return sh.tokens >= 0 && sh.seq > 0 && sh.heads > 0 && sh.kv > 0 && sh.D >= 8 && sh.D <= 256 && sh.D % 8 == 0; }
+bool good(long long tokens, int seq, const Shape& sh) {
+  return tokens >= 0 && tokens < (1LL << 30) && seq > 0 && sh.heads > 0 && sh.kv > 0 && sh.D >= 8 && sh.D <= 256 && sh.D % 8 == 0 && (long long)sh.heads + 2LL * sh.kv < (1 << 14);
+}
 
 }  // namespace qkn
 }  // namespace b200
@@ -278,8 +291,8 @@ extern "C" {
 // [>= seq, D / 2] (cos, sin).
 int b200ops_qk_norm_rope_fwd(const void* x, const void* wq, const void* wk, int wBf16, const float* table, void* q, void* k, long long tokens, int seq, int heads,
                              int kv, int D, float eps, cudaStream_t s) {
-  const Shape sh{tokens, seq, heads, kv, D, 1, eps};
-  if (!good(sh)) return (int)cudaErrorInvalidValue;
+  const Shape sh{(uint32_t)tokens, (uint32_t)seq, heads, kv, D, eps};
+  if (!good(tokens, seq, sh)) return (int)cudaErrorInvalidValue;
   if (tokens == 0) return 0;
   const auto go = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
@@ -289,14 +302,17 @@ int b200ops_qk_norm_rope_fwd(const void* x, const void* wq, const void* wk, int 
 }
 
 // fp32 words of scratch for the backward call.
-long long b200ops_qk_norm_rope_bwd_scratch(int D) { return (long long)kCtasPerSm * smCount() * 2 * D; }
+long long b200ops_qk_norm_rope_bwd_scratch(int D, int heads, int kv) {
+  const long long most = (long long)kCtasBwd * smCount(), least = ((long long)heads + 2LL * kv + kWarps - 1) / kWarps;
+  return (most > least ? most : least) * 2 * D;
+}
 
 // strides: batch, head and position strides (elements, multiples of 4) of dq, dk, dv in turn. dx like x; dwq, dwk [D] of the weights' type.
 int b200ops_qk_norm_rope_bwd(const void* dq, const void* dk, const void* dv, const long long* strides, const void* x, const void* wq, const void* wk, int wBf16,
                              const float* table, void* dx, float* scratch, void* dwq, void* dwk, long long tokens, int seq, int heads, int kv, int D, float eps,
                              cudaStream_t s) {
-  const Shape sh{tokens, seq, heads, kv, D, 1, eps};
-  if (!good(sh) || tokens == 0) return (int)cudaErrorInvalidValue;
+  const Shape sh{(uint32_t)tokens, (uint32_t)seq, heads, kv, D, eps};
+  if (!good(tokens, seq, sh) || tokens == 0) return (int)cudaErrorInvalidValue;
   const auto grad = [&](const void* p, int i) { return Grad{(const __nv_bfloat16*)p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
   const auto go = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;

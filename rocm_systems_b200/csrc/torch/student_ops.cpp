@@ -12,7 +12,7 @@
 
 extern "C" {
 int b200ops_qk_norm_rope_fwd(const void*, const void*, const void*, int, const float*, void*, void*, long long, int, int, int, int, float, cudaStream_t);
-long long b200ops_qk_norm_rope_bwd_scratch(int);
+long long b200ops_qk_norm_rope_bwd_scratch(int, int, int);
 int b200ops_qk_norm_rope_bwd(const void*, const void*, const void*, const long long*, const void*, const void*, const void*, int, const float*, void*, float*, void*, void*,
                              long long, int, int, int, int, float, cudaStream_t);
 int b200ops_window_attention_fwd(const void*, const void*, const void*, void*, float*, void*, const int*, const long long*, int, int, int, int, int, int, int, float,
@@ -98,7 +98,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     c10::cuda::OptionalCUDAGuard guard(qkv.device());
     const Tensor dq = rows16(grads[0]), dk = rows16(grads[1]), dv = rows16(grads[2]);
     const Tensor dqkv = at::empty_like(qkv), dwq = at::empty_like(wq), dwk = at::empty_like(wk);
-    const Tensor scratch = at::empty({(int64_t)b200ops_qk_norm_rope_bwd_scratch((int)D)}, qkv.options().dtype(at::kFloat));
+    const Tensor scratch = at::empty({(int64_t)b200ops_qk_norm_rope_bwd_scratch((int)D, (int)heads, (int)kv)}, qkv.options().dtype(at::kFloat));
     const auto st = strides<3>({&dq, &dk, &dv});
     check(b200ops_qk_norm_rope_bwd(ptr(dq), ptr(dk), ptr(dv), st.data(), ptr(qkv), ptr(wq), ptr(wk), wq.scalar_type() == at::kBFloat16, (const float*)ptr(table), out(dqkv),
                                    (float*)out(scratch), out(dwq), out(dwk), B * S, (int)S, (int)heads, (int)kv, (int)D, (float)ctx->saved_data["eps"].toDouble(), stream()),
@@ -118,7 +118,7 @@ std::tuple<Tensor, Tensor, Tensor> qkNormRope(const Tensor& qkv, const Tensor& w
   need(table.dim() == 3 && table.size(0) >= S && table.size(1) == D / 2 && table.size(2) == 2, "table: [at least S, D / 2, 2]");
   need(table.scalar_type() == at::kFloat && table.is_contiguous() && (reinterpret_cast<uintptr_t>(ptr(table)) & 15) == 0, "table: contiguous fp32");
   need(eps >= 0 && std::isfinite(eps), "eps: finite, not negative");
-  need(S < (1LL << 31) && heads + 2 * kv < (1LL << 31), "too many positions or heads");
+  need(qkv.size(0) * S < (1LL << 30) && heads + 2 * kv < (1LL << 14), "too many positions or heads");
   need(onOneDevice(qkv, {&wq, &wk, &table}), "tensors on one CUDA device expected");
   variable_list r;
   if (at::GradMode::is_enabled() && (qkv.requires_grad() || wq.requires_grad() || wk.requires_grad()))
