@@ -64,7 +64,9 @@ template <size_t N> std::array<long long, 3 * N> strides(const std::array<const 
   return s;
 }
 // [B, heads, S, D] whose memory is [B, S, heads, D], the layout the projections read and write.
-Tensor byToken(int64_t B, int64_t heads, int64_t S, int64_t D, const Tensor& like) { return at::empty({B, S, heads, D}, like.options()).transpose(1, 2); }
+Tensor byToken(int64_t B, int64_t heads, int64_t S, int64_t D, const Tensor& like) {
+  return at::empty_strided({B, heads, S, D}, {S * heads * D, D, heads * D, 1}, like.options());
+}
 
 const void* ptr(const Tensor& t) { return t.const_data_ptr(); }
 void* out(const Tensor& t) { return t.mutable_data_ptr(); }

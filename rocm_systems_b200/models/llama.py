@@ -7,25 +7,30 @@ stream (see :mod:`rocm_systems_b200.parallel.fsdp`). Every linear layer's three 
 gradient, weight gradient) run on this package's tcgen05 CTA-pair kernel, which reads row-major and
 transposed operands alike, with the weight gradient written straight into the unit's flat gradient
 buffer (``set_gemm("library")`` switches them to cuBLAS through ``torch.mm`` for comparison);
-attention is the library SDPA kernel; norms, rotary embedding, SwiGLU, the loss, the embedding
+attention is the library SDPA kernel, or with ``LlamaConfig.window`` this package's windowed one
+(:mod:`rocm_systems_b200.ops.attention`); norms, rotary embedding, SwiGLU, the loss, the embedding
 and AdamW are this package's CUDA kernels (:mod:`rocm_systems_b200.ops.train_ops`).
 """
 from __future__ import annotations
 
 import os
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 
+from ..ops import attention
 from ..ops import train_ops as ops
 from ..parallel.fsdp import AdamWConfig, FlatUnit, FSDPEngine, ParamSpec
 
 
 @dataclass
 class LlamaConfig:
-    """Shape of a Llama-style decoder (grouped-query attention, SwiGLU MLP, RMSNorm, rotary embedding, untied output matrix)."""
+    """Shape of a Llama-style decoder (grouped-query attention, SwiGLU MLP, RMSNorm, rotary embedding, untied output matrix).
+
+    ``qk_norm``: every query and key head is normalised (RMSNorm over the head, with one weight vector each for queries and keys) before the
+    rotation. ``window``: a token sees the last ``window`` tokens, itself among them, and the first ``sinks`` ones; 0: all earlier ones."""
 
     vocab: int = 128256
     hidden: int = 4096
@@ -37,6 +42,9 @@ class LlamaConfig:
     eps: float = 1e-5
     seq_len: int = 4096
     init_std: float = 0.02
+    qk_norm: bool = False
+    window: int = 0
+    sinks: int = 0
 
     @property
     def head_dim(self) -> int:
@@ -92,6 +100,7 @@ class LlamaConfig:
     def param_count(self) -> int:
         d = self.head_dim
         per_layer = self.hidden * (self.heads + 2 * self.kv_heads) * d + self.hidden * self.hidden + 3 * self.hidden * self.ffn + 2 * self.hidden
+        per_layer += 2 * d if self.qk_norm else 0
         return 2 * self.vocab * self.hidden + self.layers * per_layer + self.hidden
 
     def flops_per_token(self) -> float:
@@ -99,6 +108,11 @@ class LlamaConfig:
         d = self.head_dim
         gemm_params = self.layers * (self.hidden * (self.heads + 2 * self.kv_heads) * d + self.hidden * self.hidden + 3 * self.hidden * self.ffn) + self.vocab * self.hidden
         attn = self.layers * 6 * self.seq_len * self.hidden  # 2*S*H fwd for QK^T and PV, halved by causality, x3 for fwd+bwd
+        if 0 < self.window < self.seq_len:
+            # tokens that a token sees on average: the window is short at the start; the sinks count where the window has left them behind
+            S, w = self.seq_len, self.window
+            seen = w - w * (w - 1) / (2 * S) + sum(min(self.sinks, i + 1 - w) for i in range(w, S)) / S
+            attn = self.layers * 12 * self.hidden * seen
         return 6.0 * gemm_params + attn
 
 
@@ -173,8 +187,18 @@ class _SplitQKV(torch.autograd.Function):
         return out, None, None
 
 
+@dataclass
+class DistillConfig:
+    """How a teacher's stored logits enter the loss: ``(1 - weight)`` of cross-entropy and ``weight`` of the divergence from them at
+    ``temperature`` (:func:`rocm_systems_b200.ops.train_ops.distill_loss`)."""
+
+    weight: float = 0.5
+    temperature: float = 1.0
+
+
 def layer_specs(cfg: LlamaConfig) -> List[ParamSpec]:
     d = cfg.head_dim
+    norms = [ParamSpec("q_norm", (d,), "ones"), ParamSpec("k_norm", (d,), "ones")] if cfg.qk_norm else []
     return [
         ParamSpec("attn_norm", (cfg.hidden,), "ones"),
         ParamSpec("wqkv", ((cfg.heads + 2 * cfg.kv_heads) * d, cfg.hidden), std=cfg.init_std),
@@ -182,6 +206,7 @@ def layer_specs(cfg: LlamaConfig) -> List[ParamSpec]:
         ParamSpec("mlp_norm", (cfg.hidden,), "ones"),
         ParamSpec("w13", (2 * cfg.ffn, cfg.hidden), std=cfg.init_std),  # gate rows then up rows
         ParamSpec("w2", (cfg.hidden, cfg.ffn), std=cfg.init_std),
+        *norms,
     ]
 
 
@@ -192,9 +217,15 @@ def layer_forward(p: dict, x: torch.Tensor, cfg: LlamaConfig, rope: torch.Tensor
     d, nh, nkv = cfg.head_dim, cfg.heads, cfg.kv_heads
     h = ops.rmsnorm(x, p["attn_norm"], cfg.eps)
     qkv = linear(h, p["wqkv"]).view(T, nh + 2 * nkv, d)
-    qkv = ops.rope_(qkv, rope, nh + nkv)
-    q, k, v = _SplitQKV.apply(qkv.view(batch, S, nh + 2 * nkv, d), nh, nkv)
-    a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=nkv != nh)
+    if cfg.qk_norm:
+        q, k, v = attention.qk_norm_rope(qkv.view(batch, S, nh + 2 * nkv, d), p["q_norm"], p["k_norm"], rope, nh, nkv, cfg.eps)
+    else:
+        qkv = ops.rope_(qkv, rope, nh + nkv)
+        q, k, v = _SplitQKV.apply(qkv.view(batch, S, nh + 2 * nkv, d), nh, nkv)
+    if cfg.window:
+        a = attention.window_attention(q, k, v, cfg.window, cfg.sinks)
+    else:
+        a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=nkv != nh)
     a = a.transpose(1, 2).reshape(T, nh * d)
     x = x + linear(a, p["wo"])
     h = ops.rmsnorm(x, p["mlp_norm"], cfg.eps)
@@ -204,11 +235,14 @@ def layer_forward(p: dict, x: torch.Tensor, cfg: LlamaConfig, rope: torch.Tensor
 
 class LlamaTrainer:
     """The public training API: ``loss = trainer.step(tokens, targets)`` with host tensors in
-    pinned memory or device tensors; ``loss`` is a host float when ``return_loss`` is set."""
+    pinned memory or device tensors; ``loss`` is a host float when ``return_loss`` is set. With ``distill``,
+    ``step(tokens, targets, teacher=(ids, logits))`` learns from a teacher's stored logits too."""
 
     def __init__(self, cfg: LlamaConfig, comm=None, device: Optional[torch.device] = None, opt: Optional[AdamWConfig] = None,
-                 seed: int = 0, fused_rs: bool = True, sym_shards: bool = True, overlap: bool = True, copy_engine_gather: Optional[bool] = None):
+                 seed: int = 0, fused_rs: bool = True, sym_shards: bool = True, overlap: bool = True, copy_engine_gather: Optional[bool] = None,
+                 distill: Optional[DistillConfig] = None):
         self.cfg = cfg
+        self.distill = distill
         self.comm = comm
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         rank = comm.rank if comm is not None else 0
@@ -230,9 +264,17 @@ class LlamaTrainer:
         self._loss_host = torch.zeros(1, dtype=torch.float32).pin_memory() if torch.cuda.is_available() else torch.zeros(1)
 
     # ---- one optimisation step ---------------------------------------------------------------------
-    def step(self, tokens: torch.Tensor, targets: torch.Tensor, return_loss: bool = True):
+    def step(self, tokens: torch.Tensor, targets: torch.Tensor, return_loss: bool = True,
+             teacher: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+        """One optimisation step on ``tokens`` and ``targets`` [batch, seq]. ``teacher``: the ids (int64 or int32) and logits (fp32 or bf16) of a
+        teacher's top entries, both [batch, seq, K]; the trainer then needs a :class:`DistillConfig`."""
         cfg, eng = self.cfg, self.engine
+        assert (teacher is None) == (self.distill is None), "a teacher's logits in every step, or no DistillConfig"
+        if teacher is not None:
+            assert all(t.dim() == 3 and t.shape[:2] == tokens.shape for t in teacher), "teacher: ids and logits [batch, seq, K]"
         with torch.cuda.device(self.device):
+            if teacher is not None:
+                teacher = tuple(t.to(self.device, non_blocking=True) for t in teacher)
             if not tokens.is_cuda:
                 if self._tok_dev is None or self._tok_dev.shape != tokens.shape:
                     self._tok_dev = torch.empty(tokens.shape, dtype=torch.int64, device=self.device)
@@ -272,7 +314,12 @@ class LlamaTrainer:
                 hn = ops.rmsnorm(hin, self.head.params["norm"], cfg.eps)
             w_out = self.head.params["out"].detach()  # the head GEMMs are differentiated by hand below
             logits = mm_nt(hn.detach(), w_out)
-            loss_rows = ops.cross_entropy_inplace(logits, tgt, 1.0 / T)
+            if teacher is None:
+                loss_rows = ops.cross_entropy_inplace(logits, tgt, 1.0 / T)
+            else:
+                K = teacher[0].shape[-1]
+                loss_rows, _ = ops.distill_loss(logits, tgt, teacher[0].reshape(T, K), teacher[1].reshape(T, K), self.distill.weight,
+                                                self.distill.temperature, 1.0 / T, grad=logits)
             loss = loss_rows.mean()
             # What no token of this batch touches of the embedding is updated beside the backward pass.
             by_rows = eng.updates_rows and cfg.vocab * cfg.hidden >= eng.rows_from

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ..ops import train_ops
+from ..ops import attention, train_ops
 
 _done = False
 
@@ -284,11 +284,13 @@ class TensorParallelAttention:
     rotary embedding and causal attention for those heads are local; the row-parallel output projection runs inside the
     reduce-scatter (``b200collGemmRs``) and leaves this rank's rows of the result. Together with
     :class:`TensorParallelMLP` this is a whole layer with two fused kernels per half and no stand-alone collective.
+    With ``window`` a token sees the last ``window`` tokens and the first ``sinks`` ones (:func:`rocm_systems_b200.ops.attention.window_attention`).
     """
 
     def __init__(self, comm, rows_per_rank: int, hidden: int, heads: int, kv_heads: int, seq_len: int, device=None, rope_theta: float = 500000.0,
-                 std: float = 0.02, seed: int = 0, comm_ctas: int = 0):
+                 std: float = 0.02, seed: int = 0, comm_ctas: int = 0, window: int = 0, sinks: int = 0):
         self.comm = comm
+        self.window, self.sinks = window, sinks
         self.n, self.rank = comm.nranks, comm.rank
         assert heads % self.n == 0 and kv_heads % self.n == 0, "heads and kv_heads must divide by the tensor-parallel size"
         self.rows, self.hidden, self.seq = rows_per_rank, hidden, seq_len
@@ -325,7 +327,10 @@ class TensorParallelAttention:
         q = t[:, :self.hq].reshape(B, self.seq, self.hq, self.d).transpose(1, 2)
         k = t[:, self.hq:self.hq + self.hkv].reshape(B, self.seq, self.hkv, self.d).transpose(1, 2)
         v = t[:, self.hq + self.hkv:].reshape(B, self.seq, self.hkv, self.d).transpose(1, 2)
-        o = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.hq != self.hkv)
+        if self.window:
+            o = attention.window_attention(q, k, v, self.window, self.sinks)
+        else:
+            o = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.hq != self.hkv)
         return o.transpose(1, 2).reshape(self.M, self.hq * self.d)
 
     def _attend(self, qkv: torch.Tensor, out: torch.Tensor) -> None:
