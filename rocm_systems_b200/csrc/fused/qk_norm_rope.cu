@@ -7,9 +7,11 @@
 //
 // A head's row belongs to 8, 16 or 32 lanes; lane j holds elements [4j, 4j + 4) and their partners at + D / 2, so the rotation needs no
 // exchange and the sums take three to five shuffles. A warp stays with a few heads of one kind, whose weights (and the sums of their
-// gradients) it keeps in registers, and goes from token to token; the rows of a token's heads are loaded together, as what bounds both
-// directions is how many loads are under way: with one row at a time the backward pass took 59 us where it moves 142 MB (4096 tokens, 32/8
-// heads of 128).
+// gradients) it keeps in registers, and goes from token to token. Forward, the rows of four heads per lane group are loaded together;
+// backward, where a row needs twice the registers, rows travel through shared memory, six tokens deep (a row at a time: 59 us).
+//
+// 4096 tokens, 32 + 8 + 8 heads of 128: forward 19 us for 84 MB (4.4 TB/s), backward 45 us for 142 MB (3.1 TB/s) and 5 for the weights' sums.
+// The backward pass is bound by its instructions (about 290 per pair of rows, issued in half of the cycles) rather than by memory.
 #include "rows.cuh"
 
 #include <type_traits>
@@ -21,8 +23,9 @@ using namespace rows;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnrollFwd = 4, kUnrollBwd = 2;  // rows of a lane whose loads are under way together
-constexpr int kCtasFwd = 3, kCtasBwd = 3;  // per SM
+constexpr int kUnrollFwd = 4, kUnrollBwd = 2;  // rows of a lane that are dealt with together
+constexpr int kStages = 6;                     // backward: tokens whose rows are on their way or in shared memory
+constexpr int kCtasFwd = 3, kCtasBwd = 2;  // per SM
 
 struct Shape {
   uint32_t tokens, seq;  // tokens = batch * seq
@@ -117,6 +120,10 @@ __global__ void __launch_bounds__(kThreads, kCtasFwd) forwardKernel(const __nv_b
   }
 }
 
+__device__ __forceinline__ void copyAsync16(void* smem, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(src) : "memory");
+}
+
 // partials [CTAs][2][D]: every CTA's share of the weights' gradients, summed by weightSum in a fixed order.
 template <int LANES, typename W>
 __global__ void __launch_bounds__(kThreads, kCtasBwd) backwardKernel(Grad dq, Grad dk, Grad dv, const __nv_bfloat16* __restrict__ x, const W* __restrict__ wq,
@@ -137,37 +144,58 @@ __global__ void __launch_bounds__(kThreads, kCtasBwd) backwardKernel(Grad dq, Gr
       wa[e] = toFloat(w[4 * j + e]);
       wb[e] = toFloat(w[half + 4 * j + e]);
     }
+  // The rows of the next tokens are on their way into shared memory meanwhile: [stage][row][gradient, x] of this lane's group.
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr uint32_t kRow = 16 * LANES, kStage = kUnrollBwd * 2 * kGroups * kRow;
+  uint8_t* const rows = ring + warp * kStages * kStage + group * kRow;
+  const __nv_bfloat16* const fromHead = from.p + (mine.first + group) * from.h + 8 * j;
+  const __nv_bfloat16* const xHead = x + (size_t)(mine.before + mine.first + group) * sh.D + 8 * j;
+  const auto fetch = [&](uint32_t t, int stage) {
+    if (t < sh.tokens && in) {
+      const uint32_t batch = t / sh.seq, pos = t - batch * sh.seq;
+      const __nv_bfloat16* g = fromHead + batch * from.b + pos * from.s;
+      const __nv_bfloat16* p = xHead + (size_t)t * all * sh.D;
+#pragma unroll
+      for (int u = 0; u < kUnrollBwd; u++)
+        if (mine.first + u * kGroups + group < mine.end) {
+          uint8_t* to = rows + stage * kStage + u * 2 * kGroups * kRow + 16 * j;
+          copyAsync16(to, g + u * kGroups * from.h);
+          if (mine.kind < 2) copyAsync16(to + kGroups * kRow, p + u * kGroups * sh.D);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int n = 0; n < kStages - 1; n++) fetch(mine.token + n * mine.step, n);
+  int stage = 0;
   for (uint32_t t = mine.token; t < sh.tokens; t += mine.step) {
-    const uint32_t batch = t / sh.seq;
-    const int pos = t - batch * sh.seq;
-    uint2 grad[kUnrollBwd][2], row[kUnrollBwd][2];
+    fetch(t + (kStages - 1) * mine.step, stage == 0 ? kStages - 1 : stage - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    float2 cs[4] = {};
+    if (in && mine.kind < 2)
+#pragma unroll
+      for (int e = 0; e < 4; e++) cs[e] = table[(size_t)(t % sh.seq) * half + 4 * j + e];
 #pragma unroll
     for (int u = 0; u < kUnrollBwd; u++) {
       const int h = mine.first + u * kGroups + group;
-      grad[u][0] = grad[u][1] = row[u][0] = row[u][1] = make_uint2(0, 0);
-      if (in && h < mine.end) {
-        const __nv_bfloat16* g = from.at(batch, h, pos) + 4 * j;
-        grad[u][0] = *reinterpret_cast<const uint2*>(g);
-        grad[u][1] = *reinterpret_cast<const uint2*>(g + half);
+      const bool live = in && h < mine.end;
+      const uint8_t* at = rows + stage * kStage + u * 2 * kGroups * kRow + 8 * j;
+      uint2 ra = make_uint2(0, 0), rb = ra, xa = ra, xb = ra;
+      if (live) {
+        ra = *reinterpret_cast<const uint2*>(at);
+        rb = *reinterpret_cast<const uint2*>(at + sh.D);
         if (mine.kind < 2) {
-          const __nv_bfloat16* p = x + ((size_t)t * all + mine.before + h) * sh.D + 4 * j;
-          row[u][0] = *reinterpret_cast<const uint2*>(p);
-          row[u][1] = *reinterpret_cast<const uint2*>(p + half);
+          xa = *reinterpret_cast<const uint2*>(at + kGroups * kRow);
+          xb = *reinterpret_cast<const uint2*>(at + kGroups * kRow + sh.D);
         }
       }
-    }
-    if (mine.kind < 2) {
-      float2 cs[4] = {};
-      if (in)
-#pragma unroll
-        for (int e = 0; e < 4; e++) cs[e] = table[(size_t)pos * half + 4 * j + e];
-#pragma unroll
-      for (int u = 0; u < kUnrollBwd; u++) {
+      if (mine.kind < 2) {
         float a[4], b[4], ya[4], yb[4], ga[4], gb[4];
-        unpack4(row[u][0], a);
-        unpack4(row[u][1], b);
-        unpack4(grad[u][0], ya);
-        unpack4(grad[u][1], yb);
+        unpack4(xa, a);
+        unpack4(xb, b);
+        unpack4(ra, ya);
+        unpack4(rb, yb);
         float ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -185,20 +213,19 @@ __global__ void __launch_bounds__(kThreads, kCtasBwd) backwardKernel(Grad dq, Gr
           ga[e] = r * (ga[e] * wa[e] - a[e] * c);
           gb[e] = r * (gb[e] * wb[e] - b[e] * c);
         }
-        grad[u][0] = pack4(ga);
-        grad[u][1] = pack4(gb);
+        ra = pack4(ga);
+        rb = pack4(gb);
       }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnrollBwd; u++) {
-      const int h = mine.first + u * kGroups + group;
-      if (in && h < mine.end) {
+      if (live) {
         __nv_bfloat16* out = dx + ((size_t)t * all + mine.before + h) * sh.D + 4 * j;
-        *reinterpret_cast<uint2*>(out) = grad[u][0];
-        *reinterpret_cast<uint2*>(out + half) = grad[u][1];
+        *reinterpret_cast<uint2*>(out) = ra;
+        *reinterpret_cast<uint2*>(out + half) = rb;
       }
     }
+    __syncwarp();  // the stage is read before it is filled again
+    if (++stage == kStages) stage = 0;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
   for (int e = 0; e < 4; e++) {
 #pragma unroll
@@ -271,7 +298,16 @@ template <int LANES, typename W>
 cudaError_t backward(Grad dq, Grad dk, Grad dv, const void* x, const void* wq, const void* wk, const float* table, void* dx, float* partials, void* dwq, void* dwk,
                      const Shape& sh, cudaStream_t s) {
   const unsigned ctas = ctasFor<Share<LANES, kUnrollBwd>>(sh, true);
-  backwardKernel<LANES, W><<<ctas, kThreads, 0, s>>>(dq, dk, dv, (const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)dx, partials, sh);
+  constexpr int kSmem = kWarps * kStages * kUnrollBwd * 2 * (32 / LANES) * 16 * LANES;  // 64 KB
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(backwardKernel<LANES, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  backwardKernel<LANES, W><<<ctas, kThreads, kSmem, s>>>(dq, dk, dv, (const __nv_bfloat16*)x, (const W*)wq, (const W*)wk, (const float2*)table, (__nv_bfloat16*)dx, partials, sh);
   weightSum<W><<<(2 * sh.D + 31) / 32, 1024, 0, s>>>(partials, (W*)dwq, (W*)dwk, (int)ctas, sh.D);
   return cudaGetLastError();
 }
