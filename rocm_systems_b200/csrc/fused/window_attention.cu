@@ -48,7 +48,7 @@ template <typename K> static cudaError_t allowSmem(K kernel, size_t bytes, bool 
   return e;
 }
 
-template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
+template <int HD, bool FINE> static cudaError_t forward(const Args& a, cudaStream_t s) {
   static bool done[64] = {};
   bindContext();
   FwdParams p{};
@@ -63,9 +63,9 @@ template <int HD> static cudaError_t forward(const Args& a, cudaStream_t s) {
   const int ctas = (int)(items < gemm::smCount() ? items : gemm::smCount());  // one per SM
   if (items > 0x3fffffffLL || !headMap(&p.q, a.q, a.B, a.H, a.S, a.D) || !headMap(&p.k, a.k, a.B, a.KV, a.S, a.D) || !headMap(&p.v, a.v, a.B, a.KV, a.S, a.D))
     return cudaErrorInvalidValue;
-  const cudaError_t e = allowSmem(forwardKernel<HD>, FwdCfg<HD>::kSmem, done);
+  const cudaError_t e = allowSmem(forwardKernel<HD, FINE>, FwdCfg<HD>::kSmem, done);
   if (e != cudaSuccess) return e;
-  forwardKernel<HD><<<ctas, FwdCfg<HD>::kThreads, FwdCfg<HD>::kSmem, s>>>(p);
+  forwardKernel<HD, FINE><<<ctas, FwdCfg<HD>::kThreads, FwdCfg<HD>::kSmem, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -141,7 +141,8 @@ int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, vo
   a.scale = scale;
   a.rest = packed(rest, a);
   if (!good(a) || !aligned(a.q) || !aligned(a.k) || !aligned(a.v) || !aligned(a.out) || ((uintptr_t)rest & 15)) return (int)cudaErrorInvalidValue;
-  return (int)(D <= 64 ? forward<64>(a, s) : forward<128>(a, s));
+  if (a.S <= kFineKeys || a.window <= kFineKeys - a.sinks) return (int)(D <= 64 ? forward<64, true>(a, s) : forward<128, true>(a, s));
+  return (int)(D <= 64 ? forward<64, false>(a, s) : forward<128, false>(a, s));
 }
 
 // strides: of q, k, v, out, dout, dq, dk, dv in turn. lse and rest as the forward call left them; scratch: as many fp32

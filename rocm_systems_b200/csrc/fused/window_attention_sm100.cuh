@@ -59,6 +59,11 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
   return j0 + kTile - 1 <= r0 && (rLast - j0 < a.window || j0 + kTile <= a.sinks);
 }
 
+// Where a row sees at most so many keys, weights are handed to the tensor cores as the sum of two bf16 values. A weight rounded to bf16 is off by
+// 2^-9 of itself; over many keys that averages out, but where a row sees two or three, the gradient is a small difference of such weights: 3
+// tokens, dK off by 0.0052 of its norm instead of 0.0025. It costs half as many products again, in calls that are not bound by them.
+constexpr int kFineKeys = 128;
+
 template <int HD> struct FwdCfg {
   static constexpr int kMath = 16;                       // warps 0-7 and 8-15 are the two tiles' softmax
   static constexpr int kThreads = 32 * (kMath + 4);      // launched with 96 registers each, split as 4 x 128 x 104 and 128 x 64
@@ -93,7 +98,8 @@ __device__ __forceinline__ void zeroOut(const Tensor& t, int b, int h, int row0,
   }
 }
 
-template <int HD>
+// FINE: weights as the sum of two bf16 values.
+template <int HD, bool FINE>
 __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const __grid_constant__ FwdParams p) {
   using C = FwdCfg<HD>;
   using namespace sm100;
@@ -249,6 +255,11 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
               for (int kk = 0; kk < kTile / 16; kk++)
                 mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + (kk / 4) * 64 + (kk % 4) * 8, descV + ((slotV * C::kTileBytes + kk * 2048) >> 4), idescO,
                                started[t] || kk != 0);
+              if constexpr (FINE)
+#pragma unroll
+                for (int kk = 0; kk < kTile / 16; kk++)
+                  mmaF16FromTmem(tmem + C::kTmemO + t * HD, tmem + C::kTmemS + t * kTile + (kk / 4) * 64 + 32 + (kk % 4) * 8,
+                                 descV + ((slotV * C::kTileBytes + kk * 2048) >> 4), idescO, 1);
               if (last) mmaCommit(&oDone[t]);
             }
             if (t == 1) mmaCommit(&empty[slotV]);
@@ -385,20 +396,21 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         F2 sum[2] = {makeF2(l, 0.f), makeF2(0.f, 0.f)};
         const auto weights = [&](auto all) {
 #pragma unroll
-          for (int x = 0; x < 2; x++) {
+          for (int x = 0; x < (FINE ? 4 : 2); x++) {  // FINE: once more for what rounding took (formed again, registers are short)
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-              const F2 v = fmaF2(makeF2(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), c2, off2);
+              const F2 v = fmaF2(makeF2(__uint_as_float(s[x & 1][2 * e]), __uint_as_float(s[x & 1][2 * e + 1])), c2, off2);
               const F2 pr = decltype(all)::value && e % kPoly == kPoly - 1 ? exp2Poly(v) : exp2F2(v);
-              sum[e & 1] = addF2(sum[e & 1], pr);
+              if (x < 2) sum[e & 1] = addF2(sum[e & 1], pr);
               w[e] = pack2(pr);
+              if (x >= 2) w[e] = pack2(fmaF2(unpackF2(w[e]), makeF2(-1.f, -1.f), pr));
             }
             tmemStore16(tS + x * 16, w);
           }
         };
         // Masked scores have to become zeros, which the polynomial does not give.
-        if (every) weights(std::true_type{});
+        if (!FINE && every) weights(std::true_type{});
         else weights(std::false_type{});
         tmemStoreWait();
         tcFenceBefore();

@@ -22,12 +22,16 @@ def hidden_keys(S, window, sinks, device):
 
 
 def attention(q, k, v, window, sinks, lengths, scale, dout=None):
-    """Windowed attention by its definition: {"out"} and with ``dout`` {"dq", "dk", "dv"}, and under "tol" how far each may be off."""
+    """Windowed attention by its definition: {"out"} and with ``dout`` {"dq", "dk", "dv"}, and under "tol" how far each may be off.
+
+    Where no row sees more than 128 keys the forward pass's weights are sums of two bf16 values, each off by at most 2^-16 of itself."""
     B, H, S, D = q.shape
     KV = k.shape[1]
     G = H // KV
     dev = q.device
     hid = hidden_keys(S, window, sinks, dev)
+    few = S <= 128 or 0 < window and window + sinks <= 128
+    weight = BF * BF if few else BF
     names = ("out",) if dout is None else ("out", "dq", "dk", "dv")
     like = {"out": q, "dq": q, "dk": k, "dv": k}
     res = {n: torch.zeros(like[n].shape, dtype=DT, device=dev) for n in names}
@@ -46,8 +50,9 @@ def attention(q, k, v, window, sinks, lengths, scale, dout=None):
             O = P @ V
             A = P @ V.abs()
             res["out"][b, h, :L] = O
-            # every weight rounded to bf16, the answer rounded once more
-            tO = BF * (A + O.abs()) + (2 * ds_abs + sums) * A + TINY * V.abs().sum(0)
+            # every weight rounded, the answer rounded once more; what rounding took from the answer is kept, rounded to bf16 itself, for delta
+            raw = weight * A + (2 * ds_abs + sums) * A + TINY * V.abs().sum(0)
+            tO = raw + BF * O.abs()
             tol["out"][b, h, :L] = tO
             if dout is None:
                 continue
@@ -55,8 +60,8 @@ def attention(q, k, v, window, sinks, lengths, scale, dout=None):
             dP = dO @ V.T
             delta = (dP * P).sum(1, keepdim=True)
             dS = P * (dP - delta)
-            # delta is formed from the rounded answer; dS is rounded to bf16 after fp32 arithmetic
-            E = (dO.abs() * tO).sum(1, keepdim=True) + (D / 16 + 8) * 2.0 ** -22 * (dO.abs() @ V.abs().T).amax(1, keepdim=True)
+            # delta is formed from the answer in two bf16 parts, dS is rounded to bf16 after fp32 arithmetic
+            E = (dO.abs() * (raw + BF * BF * O.abs())).sum(1, keepdim=True) + (D / 16 + 8) * 2.0 ** -22 * (dO.abs() @ V.abs().T).amax(1, keepdim=True)
             eP = (BF + 2 * ds_abs) * P + TINY
             eS = (BF + 2 * ds_abs) * dS.abs() + P * E + TINY * (dP.abs() + delta.abs() + E)
             res["dq"][b, h, :L] = dS @ K * scale
