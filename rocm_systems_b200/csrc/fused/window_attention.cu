@@ -69,15 +69,21 @@ template <int HD, bool FINE> static cudaError_t forward(const Args& a, cudaStrea
   return cudaGetLastError();
 }
 
-// How the sinks' far queries are split: every key tile that holds sinks and is not through with its window's queries.
+// How the sinks' far queries are split: every key tile that holds sinks and is not through with its window's queries. With kMostSplits such
+// tiles there is work for all SMs without, and the partial sums stay below 2 kMostSplits blocks (268 MB at D = 128).
+constexpr int kMostSplits = 1024;
 static void splitSinks(const Args& a, BwdParams& p) {
   p.tiles = (a.S + kTile - 1) / kTile;
   if (a.sinks == 0 || a.window >= a.S) return;
   const int near = (kTile + a.window - 2) / kTile + 1;  // query tiles that see a key tile through the window
   const int far = p.tiles - near;                       // of the first tile; the others have fewer
   if (far <= 0) return;
-  p.sinkTiles = (a.sinks + kTile - 1) / kTile;
-  p.farChunk = near < 4 ? 4 : near;
+  const long long sinkTiles = (a.sinks + kTile - 1) / kTile, splits = kMostSplits / (sinkTiles * a.B * a.KV);
+  if (splits == 0) return;
+  p.sinkTiles = (int)sinkTiles;
+  p.farChunk = (int)((far + splits - 1) / splits);
+  if (p.farChunk < near) p.farChunk = near;
+  if (p.farChunk < 4) p.farChunk = 4;
   p.farCount = (far + p.farChunk - 1) / p.farChunk;
 }
 static long long partialWords(const Args& a, const BwdParams& p) {
@@ -124,7 +130,8 @@ using namespace b200::wattn;
 extern "C" {
 
 // q, out [B, H, S, D], k, v [B, KV, S, D] bf16, 16-byte aligned, with strides (batch, head, position) of q, k, v, out in turn (elements,
-// multiples of 8). lse (fp32 [B, H, S rounded up to 128]) and rest (bf16 [B, S, H, D], what rounding took from out) are for the backward call, or nullptr. lengths: int32 [B] on the device, or nullptr. window 0: no window.
+// multiples of 8). lse (fp32 [B, H, S rounded up to 128]) and rest (bf16 [B, S, H, D], what rounding took from out) are for the backward call,
+// or nullptr. lengths: int32 [B] on the device, or nullptr. window 0: no window.
 int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int* lengths, const long long* strides, int B, int H, int KV,
                                  int S, int D, int window, int sinks, float scale, cudaStream_t s) {
   const auto tensor = [&](const void* p, int i) { return Tensor{(const __nv_bfloat16*)p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
@@ -136,7 +143,7 @@ int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, vo
   a.lse = lse;
   a.lengths = lengths;
   a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
-  a.window = window == 0 ? S : window;
+  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
   a.sinks = sinks < S ? sinks : S;
   a.scale = scale;
   a.rest = packed(rest, a);
@@ -164,7 +171,7 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
   a.stat = reinterpret_cast<__nv_bfloat16*>(scratch);
   a.lengths = lengths;
   a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
-  a.window = window == 0 ? S : window;
+  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
   a.sinks = sinks < S ? sinks : S;
   a.scale = scale;
   a.rest = packed(rest, a);
@@ -178,7 +185,7 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
 long long b200ops_window_attention_bwd_scratch(int B, int H, int KV, int S, int D, int window, int sinks) {
   Args a{};
   a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
-  a.window = window == 0 ? S : window;
+  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
   a.sinks = sinks < S ? sinks : S;
   if (!good(a)) return -1;
   BwdParams p{};

@@ -196,3 +196,17 @@ def test_oracle_gradients_are_those_of_the_definitions():
     ref = oracle.distill(z, tgt, ids, values, 0.3, 2.0, 0.5)
     assert torch.allclose(loss(z), ref["loss"])
     assert torch.allclose(torch.autograd.grad(loss(z).sum(), z)[0] * 0.5, ref["grad"])
+
+
+@pytest.mark.parametrize("B, H, KV, S, D, window, sinks", [(1, 32, 8, 4096, 128, 1024, 4), (1, 32, 8, 131072, 128, 1024, 131072), (1, 32, 8, 131072, 128, 128, 4096),
+                                                           (4, 32, 8, 8192, 128, 128, 2000), (64, 32, 8, 8192, 64, 1, 300), (1, 1, 1, 1 << 20, 128, 1, 1)])
+def test_window_attention_backward_scratch_is_bounded(B, H, KV, S, D, window, sinks):
+    """However many sinks there are: rows' statistics, and at most 2048 blocks of 128 rows of two gradients for the sinks' partial sums."""
+    import ctypes
+
+    from rocm_systems_b200 import _lib
+
+    words = _lib.load().b200ops_window_attention_bwd_scratch
+    words.argtypes, words.restype = [ctypes.c_int] * 7, ctypes.c_longlong
+    stats = B * H * ((S + 127) // 128 * 128) * 4
+    assert stats <= words(B, H, KV, S, D, window, sinks) <= stats + 2048 * 2 * 128 * D

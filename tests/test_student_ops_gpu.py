@@ -106,6 +106,12 @@ def test_window_attention_heads(B, H, KV, S, D, window, sinks):
     _check_attention(*_attention_inputs(S + D, B, H, KV, S, D), window, sinks)
 
 
+@pytest.mark.parametrize("B, S, window, sinks", [(24, 1400, 100, 200), (64, 600, 40, 300), (2, 700, 1, 700)])
+def test_window_attention_many_sinks(B, S, window, sinks):
+    """As many key tiles with sinks as need no splitting of their later queries, or little of it."""
+    _check_attention(*_attention_inputs(B, B, 8, 8, S, 64), window, sinks)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("window, sinks", [(300, 4), (0, 0), (513, 129)])
 def test_window_attention_many_tiles(D, window, sinks):
