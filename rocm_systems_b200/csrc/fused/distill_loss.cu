@@ -29,6 +29,9 @@ constexpr int kMaxEntries = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kSlice = 16384;      // elements of a slice, as long as a cluster of eight can hold the row
 constexpr int kMaxSlice = 104 * 1024;
+// Scores are scaled by 1 / tau before their maximum is taken off, in fp32: below kMinTau the rounding of that maximum shows (logits of 100: 1e-3
+// of a probability). The divergence is of the size of 1 / tau^2 and multiplied by tau^2: above kMaxTau little is left of it.
+constexpr float kMinTau = 0.01f, kMaxTau = 100.f;
 constexpr int kErrLoad = 31, kErrMeet = 32;
 
 struct Args {
@@ -308,7 +311,7 @@ extern "C" {
 int b200ops_distill_loss(const void* logits, void* grad, const long long* targets, const void* ids, int idBytes, const void* values, int valueBytes, float* loss,
                          long long T, int V, int K, long long stride, long long gradStride, float a, float tau, float gradScale, cudaStream_t s) {
   using namespace b200::distill;
-  if (T < 0 || V <= 0 || V > kMaxCluster * kMaxSlice || K <= 0 || K > kMaxEntries || !(tau > 0.f) || !(a >= 0.f && a <= 1.f) || stride < V || gradStride < V ||
+  if (T < 0 || V <= 0 || V > kMaxCluster * kMaxSlice || K <= 0 || K > kMaxEntries || !(tau >= kMinTau && tau <= kMaxTau) || !(a >= 0.f && a <= 1.f) || stride < V || gradStride < V ||
       (idBytes != 4 && idBytes != 8) || (valueBytes != 2 && valueBytes != 4) || (((uintptr_t)logits | (uintptr_t)grad) & 1))
     return (int)cudaErrorInvalidValue;
   if (T == 0) return 0;

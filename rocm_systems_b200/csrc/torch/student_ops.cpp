@@ -218,7 +218,7 @@ std::tuple<Tensor, Tensor> distillLoss(const Tensor& logits, const Tensor& targe
   need(K >= 1 && K <= 1024, "1 to 1024 teacher entries per row");
   const auto it = teacherIds.scalar_type(), vt = teacherLogits.scalar_type();
   need((it == at::kLong || it == at::kInt) && (vt == at::kFloat || vt == at::kBFloat16), "int64 or int32 ids, fp32 or bf16 logits");
-  need(weight >= 0 && weight <= 1 && temperature > 0 && std::isfinite(temperature) && std::isfinite(gradScale), "0 <= weight <= 1, temperature above 0");
+  need(weight >= 0 && weight <= 1 && temperature >= 0.01 && temperature <= 100 && std::isfinite(gradScale), "0 <= weight <= 1, temperature from 0.01 to 100");
   need(T < (1LL << 28), "too many rows");
   if (gradIn) {
     const Tensor& g = *gradIn;

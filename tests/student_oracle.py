@@ -134,7 +134,10 @@ def distill(logits, targets, ids, values, weight, tau, scale):
         # threads or more side by side) and of the tree behind them
         seq = (V / 256 + 16) * 2.0 ** -24
         far = (z[t] - z[t].max()).abs().nan_to_num(posinf=0.0) * 1.45 / min(tau, 1.0) * 2.0 ** -22 + 2.0 ** -20 + seq
-        m = g * far
+        # the exponents' offset, maximum / tau in powers of two, is rounded to 2^-24 of itself: once where a slice's sums are made and once for
+        # the gradient
+        shift = z[t].abs().nan_to_num(posinf=0.0).max() * 1.45 / min(tau, 1.0) * 2.0 ** -23
+        m = g * (far + shift)
         g[y] -= 1 - weight
         ltol[t] = (1 - weight) * (2.0 ** -21 * (z[t].abs().nan_to_num(posinf=0.0).max() + 16) + seq)
         if a:
@@ -144,7 +147,7 @@ def distill(logits, targets, ids, values, weight, tau, scale):
             loss[t] += a * tau ** 2 * (p[part] * (logp[part] - logq[i[part]])).sum()
             g.index_add_(0, i, -a * tau * p)
             m.index_add_(0, i, a * tau * p * (2.0 ** -18 + (u - u.max()).abs().nan_to_num(posinf=0.0) * 2.0 ** -21))
-            ltol[t] += a * tau ** 2 * (2.0 ** -18 * (p[part] * (logp[part].abs() + logq[i[part]].abs() + 16)).sum() + seq)
+            ltol[t] += a * tau ** 2 * (2.0 ** -18 * (p[part] * (logp[part].abs() + logq[i[part]].abs() + 16)).sum() + seq + shift)
         m[y] += 2.0 ** -22
         grad[t] = g * scale
         # the smallest results are rounded to a fixed step: half of bf16's smallest

@@ -210,3 +210,12 @@ def test_window_attention_backward_scratch_is_bounded(B, H, KV, S, D, window, si
     words.argtypes, words.restype = [ctypes.c_int] * 7, ctypes.c_longlong
     stats = B * H * ((S + 127) // 128 * 128) * 4
     assert stats <= words(B, H, KV, S, D, window, sinks) <= stats + 2048 * 2 * 128 * D
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-6, 0.0099, 101.0, 1e6, 1e30, float("nan")])
+def test_distill_loss_refuses_temperatures_beyond_its_arithmetic(temperature):
+    """Scores are scaled by 1 / temperature in fp32, and the divergence by its square."""
+    from rocm_systems_b200.ops import train_ops
+
+    with pytest.raises(AssertionError, match="temperature"):
+        train_ops.distill_loss(**_loss_args(temperature=temperature))

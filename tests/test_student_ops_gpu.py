@@ -231,6 +231,11 @@ def test_distill_loss(T, V, K, weight, tau):
     _check_distill(*_distill_inputs(T + V, T, V, K), weight, tau, 1 / T)
 
 
+@pytest.mark.parametrize("weight, tau", [(0.5, 0.01), (1.0, 0.01), (0.5, 0.1), (0.5, 30.0), (0.5, 100.0), (1.0, 100.0)])
+def test_distill_loss_temperature_range(weight, tau):
+    _check_distill(*_distill_inputs(11, 4, 33000, 20), weight, tau, 0.25)
+
+
 @pytest.mark.parametrize("ids, values", [(torch.int32, torch.float32), (torch.int32, bf), (torch.int64, bf)])
 def test_distill_loss_types(ids, values):
     _check_distill(*_distill_inputs(7, 6, 2048, 20, ids, values), 0.7, 0.5, -3.0)
