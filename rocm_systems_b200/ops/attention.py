@@ -1,7 +1,8 @@
 """Attention of a decoder layer on hand-written kernels: per-head norms of queries and keys with the rotation to their positions
 (``csrc/fused/qk_norm_rope.cu``) and causal attention with a sliding window and sink tokens (``csrc/fused/window_attention.cu``).
 
-bf16 tensors, fp32 arithmetic, forward and backward. The calls enqueue on the current stream of the tensors' device and return at once;
+bf16 tensors, fp32 arithmetic, forward and backward. The calls enqueue on the current stream of the tensors' device and return at once (the
+first one on a device allocates an error word and should come before any stream capture);
 :func:`rocm_systems_b200.ops.train_ops.gemm_take_error` reports a kernel that gave up a wait."""
 from __future__ import annotations
 
