@@ -69,6 +69,9 @@ template <int HD, bool FINE> static cudaError_t forward(const Args& a, cudaStrea
   return cudaGetLastError();
 }
 
+// Whether weights and their gradients are held as two bf16 values.
+static bool fine(const Args& a) { return a.S <= kFineSeq || a.window <= kFineKeys - a.sinks; }
+
 // How the sinks' far queries are split: every key tile that holds sinks and is not through with its window's queries. With kMostSplits such
 // tiles there is work for all SMs without, and the partial sums stay below 2 kMostSplits blocks (268 MB at D = 128).
 constexpr int kMostSplits = 1024;
@@ -90,7 +93,7 @@ static long long partialWords(const Args& a, const BwdParams& p) {
   return (long long)a.B * a.KV * p.sinkTiles * (1 + p.farCount) * 2 * (a.sinks < kTile ? a.sinks : kTile) * a.D;
 }
 
-template <int HD> static cudaError_t backward(const Args& a, float* partials, cudaStream_t s) {
+template <int HD, bool FINE> static cudaError_t backward(const Args& a, float* partials, cudaStream_t s) {
   static bool doneQ[64] = {}, doneK[64] = {};
   using Q = BwdCfg<HD, kQueries>;
   using K = BwdCfg<HD, kKeys>;
@@ -112,12 +115,12 @@ template <int HD> static cudaError_t backward(const Args& a, float* partials, cu
       !headMap(&p.out, a.out, a.B, a.H, a.S, a.D) || !headMap(&p.rest, a.rest, a.B, a.H, a.S, a.D))
     return cudaErrorInvalidValue;
   k.x1 = p.y1, k.x2 = p.y2, k.y1 = p.x1, k.y2 = p.x2;
-  cudaError_t e = allowSmem(backwardKernel<HD, kQueries>, Q::kSmem, doneQ);
-  if (e == cudaSuccess) e = allowSmem(backwardKernel<HD, kKeys>, K::kSmem, doneK);
+  cudaError_t e = allowSmem(backwardKernel<HD, kQueries, FINE>, Q::kSmem, doneQ);
+  if (e == cudaSuccess) e = allowSmem(backwardKernel<HD, kKeys, FINE>, K::kSmem, doneK);
   if (e != cudaSuccess) return e;
   const auto ctas = [](long long items) { return (unsigned)(items < gemm::smCount() ? items : gemm::smCount()); };  // one per SM
-  backwardKernel<HD, kQueries><<<ctas(itemsQ), Q::kThreads, Q::kSmem, s>>>(p);
-  backwardKernel<HD, kKeys><<<ctas(itemsK), K::kThreads, K::kSmem, s>>>(k);
+  backwardKernel<HD, kQueries, FINE><<<ctas(itemsQ), Q::kThreads, Q::kSmem, s>>>(p);
+  backwardKernel<HD, kKeys, FINE><<<ctas(itemsK), K::kThreads, K::kSmem, s>>>(k);
   if (p.sinkTiles) joinSinks<<<dim3(a.sinks, a.B * a.KV), 128, 0, s>>>(k);
   return cudaGetLastError();
 }
@@ -148,7 +151,7 @@ int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, vo
   a.scale = scale;
   a.rest = packed(rest, a);
   if (!good(a) || !aligned(a.q) || !aligned(a.k) || !aligned(a.v) || !aligned(a.out) || ((uintptr_t)rest & 15)) return (int)cudaErrorInvalidValue;
-  if (a.S <= kFineKeys || a.window <= kFineKeys - a.sinks) return (int)(D <= 64 ? forward<64, true>(a, s) : forward<128, true>(a, s));
+  if (fine(a)) return (int)(D <= 64 ? forward<64, true>(a, s) : forward<128, true>(a, s));
   return (int)(D <= 64 ? forward<64, false>(a, s) : forward<128, false>(a, s));
 }
 
@@ -179,7 +182,8 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
   for (const Tensor* t : {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv})
     if (!aligned(*t)) return (int)cudaErrorInvalidValue;
   float* partials = scratch + (size_t)B * H * a.padded() * 4;
-  return (int)(D <= 64 ? backward<64>(a, partials, s) : backward<128>(a, partials, s));
+  if (fine(a)) return (int)(D <= 64 ? backward<64, true>(a, partials, s) : backward<128, true>(a, partials, s));
+  return (int)(D <= 64 ? backward<64, false>(a, partials, s) : backward<128, false>(a, partials, s));
 }
 
 long long b200ops_window_attention_bwd_scratch(int B, int H, int KV, int S, int D, int window, int sinks) {

@@ -64,10 +64,13 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
   return j0 + kTile - 1 <= r0 && (rLast - j0 < a.window || j0 + kTile <= a.sinks);
 }
 
-// Where a row sees at most so many keys, weights are handed to the tensor cores as the sum of two bf16 values. A weight rounded to bf16 is off by
-// 2^-9 of itself; over many keys that averages out, but where a row sees two or three, the gradient is a small difference of such weights: 3
-// tokens, dK off by 0.0052 of its norm instead of 0.0025. It costs half as many products again, in calls that are not bound by them.
-constexpr int kFineKeys = 128;
+// Weights and their gradients (P and dS) go to the tensor cores in bf16, each off by 2^-9 of itself. Over many keys that averages out: dQ and dK
+// are 0.0024 of their norm off, 0.0017 of which is their own rounding. Where rows see a few keys the gradient is a small difference of such
+// numbers (3 tokens: 0.0039 to 0.0052). So in sequences of at most kFineSeq tokens (also a padded batch's, whose lengths are not known here), and
+// where no row sees more than kFineKeys keys, they are handed over as the sum of two bf16 values, which leaves 0.0017. Measured, 32 query and 8
+// key heads of 128: a window of 128 keys over 4096 tokens takes 47 us forward and 159 backward, and would take 55 and 239; 64 sequences of 129
+// tokens take 100 and 374 instead of 90 and 303.
+constexpr int kFineSeq = 256, kFineKeys = 64;
 
 template <int HD> struct FwdCfg {
   static constexpr int kMath = 16;                       // warps 0-7 and 8-15 are the two tiles' softmax
@@ -102,6 +105,9 @@ __device__ __forceinline__ void zeroOut(const Tensor& t, int b, int h, int row0,
     if (r < S) reinterpret_cast<uint4*>(t.at(b, h, r))[n % (D / 8)] = make_uint4(0, 0, 0, 0);
   }
 }
+
+// What rounding to two bf16 values (`packed`) took from `v`.
+__device__ __forceinline__ F2 remainder(F2 v, uint32_t packed) { return fmaF2(unpackF2(packed), makeF2(-1.f, -1.f), v); }
 
 // FINE: weights as the sum of two bf16 values.
 template <int HD, bool FINE>
@@ -409,7 +415,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
               const F2 pr = decltype(all)::value && e % kPoly == kPoly - 1 ? exp2Poly(v) : exp2F2(v);
               if (x < 2) sum[e & 1] = addF2(sum[e & 1], pr);
               w[e] = pack2(pr);
-              if (x >= 2) w[e] = pack2(fmaF2(unpackF2(w[e]), makeF2(-1.f, -1.f), pr));
+              if (x >= 2) w[e] = pack2(remainder(pr, w[e]));
             }
             tmemStore16(tS + x * 16, w);
           }
@@ -521,7 +527,9 @@ template <int HD, Side SIDE> struct BwdCfg {
   static constexpr uint32_t kX1 = 0, kX2 = 64, kS = SIDE == kQueries ? 128 : 0, kDp = kS + 128, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
 };
 
-template <int HD, Side SIDE>
+// FINE: P and dS as the sum of two bf16 values. What rounding took goes where the queries' kernel has P's columns free and where the keys'
+// kernel has had S, which then is not made a tile ahead.
+template <int HD, Side SIDE, bool FINE>
 __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(const __grid_constant__ BwdParams p) {
   using C = BwdCfg<HD, SIDE>;
   using namespace sm100;
@@ -710,11 +718,15 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         else mmaF16(tmem + d, descX + ((x * C::kTileBytes + o) >> 4), y, idescS, kk != 0);
       }
     };
-    const auto gather = [&](uint32_t acc, uint32_t w, int s, bool first) {  // acc += W Y, W: two halves of the tile's columns, each packed into half of its own
+    // acc += W Y, W: two halves of the tile's columns, each packed into half of its own; FINE: and what rounding took from W
+    const auto gather = [&](uint32_t acc, uint32_t w, uint32_t rest, int s, bool first) {
       constexpr int kSteps = kTile / 32;
+#pragma unroll 1
+      for (int part = 0; part < (FINE ? 2 : 1); part++, w = rest)
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; kk++)
-        mmaF16FromTmem(tmem + acc, tmem + w + (kk / kSteps) * (kTile / 2) + (kk % kSteps) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc, !first || kk != 0);
+        for (int kk = 0; kk < kTile / 16; kk++)
+          mmaF16FromTmem(tmem + acc, tmem + w + (kk / kSteps) * (kTile / 2) + (kk % kSteps) * 8, descSum + ((s * C::kTileBytes + kk * 2048) >> 4), idescAcc,
+                         !first || part != 0 || kk != 0);
     };
     const auto further = [&](uint32_t d, int x, uint32_t g) {  // keys: the step of lse or delta
       const uint32_t at = smemAddr(extra);
@@ -748,21 +760,25 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       __syncwarp();
       for (int n = 0; n < it.count && all; n++, g++) {
         const bool more = n + 1 < it.count;
-        if (more) {
+        constexpr bool kAhead = !(FINE && SIDE == kKeys);  // the next tile's scores may be made while this one's place is in use
+        if (more && kAhead) {
           wait(sTaken, g & 1);
           tcFenceAfter();
           if (electOne()) scores(g + 1);
           __syncwarp();
         }
         wait(dsReady, g & 1);
+        if (more && !kAhead) wait(sTaken, g & 1);
         tcFenceAfter();
         if (electOne()) {
           if constexpr (SIDE == kKeys) {
-            gather(C::kAcc1, C::kDp, slot2(g), n == 0);
+            gather(C::kAcc1, C::kDp, C::kS, slot2(g), n == 0);
             mmaCommit(&empty[slot2(g)]);
           }
-          gather(SIDE == kQueries ? C::kAcc1 : C::kAcc2, SIDE == kQueries ? C::kDp : C::kDp + 32, slot1(g), n == 0);
+          if constexpr (SIDE == kQueries) gather(C::kAcc1, C::kDp, C::kDp + 32, slot1(g), n == 0);
+          else gather(C::kAcc2, C::kDp + 32, C::kS + 32, slot1(g), n == 0);
           mmaCommit(&empty[slot1(g)]);
+          if (more && !kAhead) scores(g + 1);
           if (more) grads(g + 1);
           else {
             mmaCommit(done);
@@ -956,6 +972,15 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           if (every) weights(std::true_type{});
           else weights(std::false_type{});
         }
+        if constexpr (FINE && SIDE == kKeys) {
+#pragma unroll
+          for (int x = 0; x < kCols / 32; x++) {
+            uint32_t o[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] = pack2(remainder(w[x * 16 + e], pack2(w[x * 16 + e])));
+            tmemStore16(base + C::kS + cols + x * 16, o);
+          }
+        }
         if (!(ok = mbarWait(dpFull, g & 1, err, ERR_BWD_MATH))) break;
         tcFenceAfter();
         {
@@ -982,8 +1007,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
                 F2 v = mulF2(w[x * 16 + e], SIDE == kQueries ? addF2(dp, rowDelta) : dp);
                 if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
                 o[e] = pack2(v);
+                if constexpr (FINE) d[x][e] = pack2(remainder(v, o[e]));
               }
               tmemStore16(base + C::kDp + cols + (SIDE == kKeys ? 32 : 0) + x * 16, o);
+              if constexpr (FINE) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[e] = d[x][e];
+                tmemStore16(base + (SIDE == kKeys ? C::kS : C::kDp) + 32 + cols + x * 16, o);
+              }
             }
           };
           if (every) gradients(std::true_type{});

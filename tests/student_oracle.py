@@ -24,13 +24,14 @@ def hidden_keys(S, window, sinks, device):
 def attention(q, k, v, window, sinks, lengths, scale, dout=None):
     """Windowed attention by its definition: {"out"} and with ``dout`` {"dq", "dk", "dv"}, and under "tol" how far each may be off.
 
-    Where no row sees more than 128 keys the forward pass's weights are sums of two bf16 values, each off by at most 2^-16 of itself."""
+    Up to 256 tokens, and where no row sees more than 64 keys, the weights and their gradients are sums of two bf16 values, off by at most 2^-16
+    of themselves."""
     B, H, S, D = q.shape
     KV = k.shape[1]
     G = H // KV
     dev = q.device
     hid = hidden_keys(S, window, sinks, dev)
-    few = S <= 128 or 0 < window and window + sinks <= 128
+    few = S <= 256 or 0 < window and window + sinks <= 64
     weight = BF * BF if few else BF
     names = ("out",) if dout is None else ("out", "dq", "dk", "dv")
     like = {"out": q, "dq": q, "dk": k, "dv": k}
@@ -62,8 +63,8 @@ def attention(q, k, v, window, sinks, lengths, scale, dout=None):
             dS = P * (dP - delta)
             # delta is formed from the answer in two bf16 parts, dS is rounded to bf16 after fp32 arithmetic
             E = (dO.abs() * (raw + BF * BF * O.abs())).sum(1, keepdim=True) + (D / 16 + 8) * 2.0 ** -22 * (dO.abs() @ V.abs().T).amax(1, keepdim=True)
-            eP = (BF + 2 * ds_abs) * P + TINY
-            eS = (BF + 2 * ds_abs) * dS.abs() + P * E + TINY * (dP.abs() + delta.abs() + E)
+            eP = (weight + 2 * ds_abs) * P + TINY
+            eS = (weight + 2 * ds_abs) * dS.abs() + P * E + TINY * (1 + dP.abs() + delta.abs() + E)
             res["dq"][b, h, :L] = dS @ K * scale
             tol["dq"][b, h, :L] = BF * res["dq"][b, h, :L].abs() + scale * ((eS + sums * dS.abs()) @ K.abs())
             res["dk"][b, g, :L] += dS.T @ Q * scale

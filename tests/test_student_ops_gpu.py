@@ -144,7 +144,8 @@ def test_window_attention_large_scores():
     _check_attention(q, k, v, dout, 150, 3, scale=0.0)
 
 
-@pytest.mark.parametrize("S, window, sinks", [(2, 0, 0), (3, 1, 2), (5, 0, 0), (40, 2, 0), (700, 2, 1), (700, 100, 28), (700, 100, 29)])
+@pytest.mark.parametrize("S, window, sinks", [(2, 0, 0), (3, 1, 2), (5, 0, 0), (40, 2, 0), (700, 2, 1), (700, 100, 28), (700, 100, 29), (700, 60, 4), (700, 60, 5), (1100, 1, 1),
+                                              (256, 0, 0), (256, 9, 3), (257, 0, 0)])
 def test_window_attention_rows_that_see_few_keys(S, window, sinks):
     """Peaked rows of a few keys, where a gradient is a small difference of weights (the tolerance knows how the weights are rounded)."""
     q, k, v, dout = _attention_inputs(S + window, 2, 4, 2, S, 64)
