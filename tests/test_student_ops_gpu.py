@@ -333,3 +333,89 @@ def test_norms_rotation_and_attention_in_a_row():
     for n, t in zip(("dqkv", "dwq", "dwk"), back):
         oracle.off(n, t, ref)
     assert train_ops.gemm_take_error() == 0
+
+
+def _big(*shape):
+    return torch.empty(*shape, device="cuda", dtype=bf).normal_(generator=_gen(1))
+
+
+def test_offsets_beyond_32_bits_attention():
+    """The last sequence of a batch of more than 2^31 elements is what it is alone."""
+    from rocm_systems_b200.ops import attention
+
+    B, H, S, D = 2101, 8, 1024, 128
+    q, dout = _big(B, S, H, D).transpose(1, 2), _big(B, S, H, D).transpose(1, 2)
+    k, v = (_big(B, S, 1, D).transpose(1, 2) for _ in range(2))
+    assert q.numel() > 2 ** 31
+    lengths = torch.full((B,), S, device="cuda", dtype=torch.int32)
+    lengths[-1] = 777
+
+    def run(n):
+        leaves = [t[n:].detach().requires_grad_(True) for t in (q, k, v)]
+        out = attention.window_attention(*leaves, 300, 0, lengths[n:])
+        return [t[-1] for t in (out, *torch.autograd.grad(out, leaves, dout[n:]))]
+
+    for got, want in zip(run(0), run(B - 1)):
+        assert torch.equal(got, want)
+
+
+def test_offsets_beyond_32_bits_norms():
+    from rocm_systems_b200.ops import attention, train_ops
+
+    B, S, H, KV, D = 1030, 1024, 14, 1, 128
+    qkv = _big(B, S, H + 2 * KV, D)
+    assert qkv.numel() > 2 ** 31
+    w = torch.ones(D, device="cuda", dtype=bf)
+    table = train_ops.rope_table(S, D, 10000.0, "cuda")
+    grads = [_big(S, n, D).transpose(0, 1).expand(B, n, S, D) for n in (H, KV, KV)]
+
+    def run(n):
+        x = qkv[n:].detach().requires_grad_(True)
+        out = attention.qk_norm_rope(x, w, w, table, H, KV)
+        dx, = torch.autograd.grad(out, (x,), [g[n:] for g in grads])
+        return [t[-1] for t in (*out, dx)]
+
+    for got, want in zip(run(0), run(B - 1)):
+        assert torch.equal(got, want)
+
+
+def test_offsets_beyond_32_bits_loss():
+    from rocm_systems_b200.ops import train_ops
+
+    T, V, K = 17000, 128256, 8
+    logits = _big(T, V)
+    assert logits.numel() > 2 ** 31
+    tgt = torch.randint(0, V, (T,), device="cuda", generator=_gen(2))
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=_gen(3))
+    values = torch.randn(T, K, device="cuda", generator=_gen(4))
+    alone = train_ops.distill_loss(logits[-2:].clone(), tgt[-2:], ids[-2:], values[-2:], 0.5, 2.0, 0.125)
+    loss, grad = train_ops.distill_loss(logits, tgt, ids, values, 0.5, 2.0, 0.125, grad=logits)
+    assert torch.equal(loss[-2:], alone[0]) and torch.equal(grad[-2:], alone[1])
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call has its own scratch: what runs beside it on another stream changes nothing."""
+    from rocm_systems_b200.ops import attention, train_ops
+
+    q, k, v, dout = _attention_inputs(5, 2, 8, 2, 900, 128)
+    logits, tgt, ids, values = _distill_inputs(6, 64, 32000, 16)
+    g = _gen(7)
+    qkv, w = _rand(g, 2, 900, 12, 128).requires_grad_(True), torch.ones(128, device="cuda", dtype=bf).requires_grad_(True)
+    table = train_ops.rope_table(900, 128, 10000.0, "cuda")
+
+    def run():
+        out = attention.window_attention(q, k, v, 200, 3)
+        n = attention.qk_norm_rope(qkv, w, w, table, 8, 2)
+        return [out, *torch.autograd.grad(out, (q, k, v), dout), *n, *torch.autograd.grad(n, (qkv, w), [torch.ones_like(t) for t in n]),
+                *train_ops.distill_loss(logits, tgt, ids, values, 0.5, 2.5, 1.0)]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
