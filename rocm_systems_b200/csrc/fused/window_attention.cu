@@ -69,7 +69,7 @@ template <int HD, bool FINE> static cudaError_t forward(const Args& a, cudaStrea
   return cudaGetLastError();
 }
 
-// Whether weights and their gradients are held as two bf16 values.
+// Whether the weights and their gradients of all rows are held as two bf16 values.
 static bool fine(const Args& a) { return a.S <= kFineSeq || a.window <= kFineKeys - a.sinks; }
 
 // How the sinks' far queries are split: every key tile that holds sinks and is not through with its window's queries. With kMostSplits such

@@ -64,13 +64,17 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
   return j0 + kTile - 1 <= r0 && (rLast - j0 < a.window || j0 + kTile <= a.sinks);
 }
 
-// Weights and their gradients (P and dS) go to the tensor cores in bf16, each off by 2^-9 of itself. Over many keys that averages out: dQ and dK
-// are 0.0024 of their norm off, 0.0017 of which is their own rounding. Where rows see a few keys the gradient is a small difference of such
-// numbers (3 tokens: 0.0039 to 0.0052). So in sequences of at most kFineSeq tokens (also a padded batch's, whose lengths are not known here), and
-// where no row sees more than kFineKeys keys, they are handed over as the sum of two bf16 values, which leaves 0.0017. Measured, 32 query and 8
-// key heads of 128: a window of 128 keys over 4096 tokens takes 47 us forward and 159 backward, and would take 55 and 239; 64 sequences of 129
-// tokens take 100 and 374 instead of 90 and 303.
-constexpr int kFineSeq = 256, kFineKeys = 64;
+// Weights and their gradients (P and dS) go to the tensor cores in bf16, each off by 2^-9 of itself. Over many keys that averages out. Where rows
+// see a few keys the gradient is a small difference of such numbers (3 tokens: 0.0039 to 0.0052 of its norm). So for the first kFineSeq queries
+// of a sequence, and where no row sees more than kFineKeys keys, they are handed over as the sum of two bf16 values, which leaves the
+// result's own rounding. The rule looks at a query's position alone: what a sequence answers does not hang on the batch that it is padded in.
+//
+// Kernels for calls of such rows only (FINE) multiply by both values in one step. In the others the first tiles are streamed a second time, for
+// what rounding took: the same products in the same order, so the same bits, and the issuing warp need not know. (A question in each of its
+// steps made the windowed passes 5 to 7% slower, whatever the answer was.) 4096 tokens, 32 query and 8 key heads of 128, device time with the
+// first tiles streamed twice and once: window 1024 and 4 sinks, forward 88 and 84 us, backward 255 and 246; all earlier keys 136 and 133, 426 and 422.
+// A window of 128 keys throughout as two values would take 55 instead of 47 us forward and 239 instead of 159 backward.
+constexpr int kFineSeq = 2 * kTile, kFineKeys = 64;  // kFineSeq: a pair of query tiles, so that a forward item is of one kind
 
 template <int HD> struct FwdCfg {
   static constexpr int kMath = 16;                       // warps 0-7 and 8-15 are the two tiles' softmax
@@ -109,7 +113,7 @@ __device__ __forceinline__ void zeroOut(const Tensor& t, int b, int h, int row0,
 // What rounding to two bf16 values (`packed`) took from `v`.
 __device__ __forceinline__ F2 remainder(F2 v, uint32_t packed) { return fmaF2(unpackF2(packed), makeF2(-1.f, -1.f), v); }
 
-// FINE: weights as the sum of two bf16 values.
+// FINE: all weights as the sum of two bf16 values.
 template <int HD, bool FINE>
 __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const __grid_constant__ FwdParams p) {
   using C = FwdCfg<HD>;
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 
   // A pair of query tiles of one head and its key tiles.
   struct Item {
-    int h, b, kh, r0, L, count, nSinks;
+    int h, b, kh, r0, L, count, nSinks, twice;  // twice: 1 where every tile comes a second time
     bool two;
     KeyRange own0, own1;
     __device__ Item(const FwdParams& p, uint32_t item) : own0(p.a, 0, 0), own1(p.a, 0, 0) {
@@ -175,13 +179,18 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       L = lengthOf(a, b);
       count = nSinks = 0;
       two = r0 + kTile < L;
+      twice = !FINE && r0 < kFineSeq;
       if (r0 >= L) return;
       own0 = KeyRange(a, r0, min(r0 + kTile, L) - 1);
       own1 = KeyRange(a, two ? r0 + kTile : r0, min(r0 + 2 * kTile, L) - 1);
       nSinks = min(own0.sinkTiles, own0.first);
-      count = nSinks + own1.last - own0.first + 1;
+      count = (nSinks + own1.last - own0.first + 1) << twice;
     }
-    __device__ int tileOf(int n) const { return n < nSinks ? n : own0.first + n - nSinks; }
+    __device__ int tileOf(int n) const {
+      n >>= twice;
+      return n < nSinks ? n : own0.first + n - nSinks;
+    }
+    __device__ bool again(int n) const { return !FINE && (n & twice); }
     __device__ bool active(int t, int n) const { return t == 0 ? own0.has(tileOf(n)) : two && own1.has(tileOf(n)); }
     __device__ bool straddles(int n) const { return L - tileOf(n) * kTile < kTile; }
   };
@@ -250,7 +259,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         const int slotV = after(slotK), slotNext = after(slotV);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const bool now = it.active(t, n), next = more && it.active(t, n + 1), last = it.tileOf(n) == (t ? it.own1.last : it.own0.last);
+          const bool now = it.active(t, n), next = more && it.active(t, n + 1), last = it.tileOf(n) == (t ? it.own1.last : it.own0.last) && (FINE || (n & it.twice) == it.twice);
           if (now) {
             if (!started[t]) {
               wait(&oFree[t], oTurn[t]);
@@ -405,24 +414,25 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         const float off = m == -INFINITY ? 0.f : m * p.c;
         const F2 c2 = makeF2(p.c, p.c), off2 = makeF2(-off, -off);
         F2 sum[2] = {makeF2(l, 0.f), makeF2(0.f, 0.f)};
-        const auto weights = [&](auto all) {
+        const auto weights = [&](auto poly, auto rest) {
 #pragma unroll
           for (int x = 0; x < (FINE ? 4 : 2); x++) {  // FINE: once more for what rounding took (formed again, registers are short)
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               const F2 v = fmaF2(makeF2(__uint_as_float(s[x & 1][2 * e]), __uint_as_float(s[x & 1][2 * e + 1])), c2, off2);
-              const F2 pr = decltype(all)::value && e % kPoly == kPoly - 1 ? exp2Poly(v) : exp2F2(v);
-              if (x < 2) sum[e & 1] = addF2(sum[e & 1], pr);
+              const F2 pr = decltype(poly)::value && e % kPoly == kPoly - 1 ? exp2Poly(v) : exp2F2(v);
               w[e] = pack2(pr);
-              if (x >= 2) w[e] = pack2(remainder(pr, w[e]));
+              if (x >= 2 || decltype(rest)::value) w[e] = pack2(remainder(pr, w[e]));
+              else sum[e & 1] = addF2(sum[e & 1], pr);
             }
             tmemStore16(tS + x * 16, w);
           }
         };
         // Masked scores have to become zeros, which the polynomial does not give.
-        if (!FINE && every) weights(std::true_type{});
-        else weights(std::false_type{});
+        if (!FINE && every && !it.twice) weights(std::true_type{}, std::false_type{});
+        else if (!it.again(n)) weights(std::false_type{}, std::false_type{});
+        else weights(std::false_type{}, std::true_type{});
         tmemStoreWait();
         tcFenceBefore();
         __syncwarp();
@@ -527,7 +537,7 @@ template <int HD, Side SIDE> struct BwdCfg {
   static constexpr uint32_t kX1 = 0, kX2 = 64, kS = SIDE == kQueries ? 128 : 0, kDp = kS + 128, kAcc1 = SIDE == kQueries ? 384 : 256, kAcc2 = 384;
 };
 
-// FINE: P and dS as the sum of two bf16 values. What rounding took goes where the queries' kernel has P's columns free and where the keys'
+// FINE: P and dS of all rows as the sum of two bf16 values. What rounding took goes where the queries' kernel has P's columns free and where the keys'
 // kernel has had S, which then is not made a tile ahead.
 template <int HD, Side SIDE, bool FINE>
 __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(const __grid_constant__ BwdParams p) {
@@ -570,7 +580,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         sinkTiles = min(r.sinkTiles, r.first);
         yTiles = sinkTiles + r.last - r.first + 1;
         yh = xh / a.group();
-        count = x0 < L ? yTiles : 0;
+        count = x0 < L ? (!FINE && x0 < kFineSeq ? 2 * yTiles : yTiles) : 0;
       } else {
         xTile = turn < p.tiles ? turn : (turn - p.tiles) / p.farCount;
         if (turn >= p.tiles) far = (turn - p.tiles) % p.farCount;
@@ -587,15 +597,19 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         }
         if (x0 >= L || yTiles < 0) yTiles = 0;
         yh = xh * a.group();
-        count = yTiles * a.group();
+        count = (yTiles + (FINE ? 0 : max(0, min(kFineSeq / kTile, yFirst + yTiles) - yFirst))) * a.group();
         if (xTile < p.sinkTiles) partRows = min(kTile, a.sinks - x0);
       }
     }
-    // The streamed tiles in their order.
+    // The streamed tiles in their order; `again`: the second time, for what rounding took.
     __device__ int firstTile() const { return SIDE == kQueries && sinkTiles ? 0 : yFirst; }
-    __device__ int nextTile(int tile) const {
+    __device__ void next(int& tile, bool& again) const {
+      if constexpr (!FINE) {
+        again = !again && (SIDE == kQueries ? x0 : tile * kTile) < kFineSeq;
+        if (again) return;
+      }
       const int end = SIDE == kQueries ? sinkTiles : yFirst + yTiles;  // queries: from the sinks to the window; keys: to the next head's first
-      return tile + 1 == end ? yFirst : tile + 1;
+      tile = tile + 1 == end ? yFirst : tile + 1;
     }
     __device__ bool straddles(int tile) const { return L - tile * kTile < kTile; }
     // Where the sums of this item's sinks go: dK's rows, then dV's.
@@ -670,6 +684,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           tmaLoad4d(smemX + C::kTileBytes + x * kBox, &p.x2, x * 64, it.x0, it.xh, it.b, xFull);
         }
         int tile = it.firstTile(), h = it.yh;
+        bool again = false;
         // Queries: the answer and what rounding took from it take the place of X when that is in tensor memory, delta is made of them; behind as many
         // streamed tiles as the ring takes meanwhile.
         const auto answer = [&]() {
@@ -694,8 +709,8 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
             mbarArriveExpectTx(&full[s], C::kTileBytes);
             for (int x = 0; x < C::kBoxes; x++) tmaLoad4d(ring + s * C::kTileBytes + x * kBox, w ? &p.y2 : &p.y1, x * 64, y0, h, it.b, &full[s]);
           }
-          tile = it.nextTile(tile);
-          if (SIDE == kKeys && tile == it.yFirst) h++;
+          it.next(tile, again);
+          if (SIDE == kKeys && tile == it.yFirst && !again) h++;
           if (SIDE == kQueries && ok && n == min(1, it.count - 1)) answer();
         }
       }
@@ -805,6 +820,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       const Item it(p, itemOf(k));
       if (it.count == 0) continue;
       int tile = it.firstTile();
+      bool again = false;
       if (SIDE == kKeys) {
         ok = ok && mbarWait(xFull, xPhase, err, ERR_BWD_MMA);
         xPhase ^= 1;
@@ -813,7 +829,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       landed(it, tile, g, 1);
       if (lane == 0) mbarArrive(xReady);
       for (int n = 0; n < it.count && ok; n++, g++) {
-        tile = it.nextTile(tile);
+        it.next(tile, again);
         if (n + 1 < it.count) landed(it, tile, g + 1, 0);
         if (lane == 0) mbarArrive(sTaken);
         if (n + 1 < it.count) landed(it, tile, g + 1, 1);
@@ -925,11 +941,13 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
       }
       const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
       int tile = it.firstTile();
+      bool second = false;
       for (int n = 0; n < it.count; n++, g++) {
         const int y0 = tile * kTile;
-        tile = it.nextTile(tile);
-        const bool every = SIDE == kQueries ? it.x0 + kTile <= it.L && seesAll(a, it.x0, it.x0 + kTile - 1, y0)
-                                            : y0 + kTile <= it.L && seesAll(a, y0, y0 + kTile - 1, it.x0);
+        const bool again = second;
+        it.next(tile, second);
+        const bool every = !again && (SIDE == kQueries ? it.x0 + kTile <= it.L && seesAll(a, it.x0, it.x0 + kTile - 1, y0)
+                                                       : y0 + kTile <= it.L && seesAll(a, y0, y0 + kTile - 1, it.x0));
         uint32_t bits[kCols / 32];
         if (!every) {
 #pragma unroll
@@ -994,10 +1012,13 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
               uint32_t o[16];
 #pragma unroll
               for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
+              if (!FINE && again)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[e] = pack2(remainder(w[x * 16 + e], o[e]));
               tmemStore16(base + C::kDp + cols + x * 16, o);
             }
           }
-          const auto gradients = [&](auto all) {
+          const auto gradients = [&](auto all, auto rest) {
 #pragma unroll
             for (int x = 0; x < kCols / 32; x++) {
               uint32_t o[16];
@@ -1008,6 +1029,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
                 if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
                 o[e] = pack2(v);
                 if constexpr (FINE) d[x][e] = pack2(remainder(v, o[e]));
+                if constexpr (decltype(rest)::value) o[e] = pack2(remainder(v, o[e]));
               }
               tmemStore16(base + C::kDp + cols + (SIDE == kKeys ? 32 : 0) + x * 16, o);
               if constexpr (FINE) {
@@ -1017,8 +1039,9 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
               }
             }
           };
-          if (every) gradients(std::true_type{});
-          else gradients(std::false_type{});
+          if (!FINE && again) gradients(std::false_type{}, std::true_type{});
+          else if (every) gradients(std::true_type{}, std::false_type{});
+          else gradients(std::false_type{}, std::false_type{});
         }
         tmemStoreWait();
         tcFenceBefore();

@@ -1,0 +1,74 @@
+"""The student decoder's operators where their variants meet: padded batches and odd head dimensions beyond the shortest sequences, values that
+are not finite, small losses, what autograd may do with a call."""
+import math
+
+import pytest
+import torch
+
+import student_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+bf = torch.bfloat16
+NAMES = ("out", "dq", "dk", "dv")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _rand(g, *shape, scale=1.0):
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(bf)
+
+
+def _inputs(seed, B, H, KV, S, D):
+    g = _gen(seed)
+    packed = _rand(g, B, S, H + 2 * KV, D)
+    q, k, v = (packed[:, :, a:b].transpose(1, 2).detach() for a, b in ((0, H), (H, H + KV), (H + KV, H + 2 * KV)))
+    return q, k, v, _rand(g, B, S, H, D).transpose(1, 2)
+
+
+def _both_ways(q, k, v, dout, window=0, sinks=0, lengths=None):
+    from rocm_systems_b200.ops import attention
+
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    out = attention.window_attention(q, k, v, window, sinks, lengths)
+    return dict(zip(NAMES, (out.detach(), *torch.autograd.grad(out, (q, k, v), dout))))
+
+
+def _against_the_oracle(q, k, v, dout, window, sinks, lengths=None):
+    got = _both_ways(q, k, v, dout, window, sinks, lengths)
+    ref = oracle.attention(q, k, v, window, sinks, lengths, 1 / math.sqrt(q.shape[-1]), dout)
+    for n in NAMES:
+        oracle.off(n, got[n], ref)
+    return got
+
+
+# ---- how weights are rounded -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [0, 40, 64, 65, 300])
+def test_padding_changes_no_bit_of_a_sequence(D, window):
+    """A sequence in a padded batch has the answer and the gradients that it has alone, however long the others are."""
+    lengths = (700, 3, 130, 256, 257, 1, 0)
+    q, k, v, dout = _inputs(7, len(lengths), 4, 2, 700, D)
+    got = _both_ways(q, k, v, dout, window, 0, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    for b, n in enumerate(lengths):
+        if n == 0:
+            continue
+        alone = _both_ways(*(t[b:b + 1, :, :n] for t in (q, k, v, dout)), window)
+        for name in NAMES:
+            assert torch.equal(got[name][b:b + 1, :, :n], alone[name]), (name, n)
+
+
+@pytest.mark.parametrize("S, window, sinks", [(300, 0, 0), (700, 0, 0), (700, 200, 5), (1100, 70, 150)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_long_sequences_first_rows_are_as_exact_as_a_short_one(S, D, window, sinks):
+    """Their gradient is a difference of few weights. Answers and gradients of the first 256 rows do not depend on what follows; the keys' gradients do
+    not where the later rows' gradient is zero. So the bounds of a sequence of 256 tokens hold."""
+    q, k, v, dout = _inputs(S + D, 2, 4, 2, S, D)
+    q = q * 2
+    dout = torch.where(torch.arange(S, device="cuda").view(S, 1) < 256, dout, torch.zeros_like(dout))
+    got = _both_ways(q, k, v, dout, window, sinks)
+    ref = oracle.attention(*(t[:, :, :256] for t in (q, k, v)), window, sinks, None, 1 / math.sqrt(D), dout[:, :, :256])
+    for n in NAMES:
+        oracle.off(n, got[n][:, :, :256], ref)
+    assert not got["dk"][:, :, 256:].any() and not got["dv"][:, :, 256:].any()
