@@ -47,8 +47,8 @@ __device__ __forceinline__ F2 exp2F2(F2 x) {
 }
 // 2^x without the special-function unit, whose 16 results per clock and SM are what a softmax runs out of first: x = n + f with n the nearest
 // whole number (added and taken off again at a scale where fp32 has no fraction left), 2^f for |f| <= 1/2 by the polynomial of degree 4
-// with the smallest largest relative error (2.7e-6; Remez exchange), n added to its exponent. Below -126 the result is 2^-126; a NaN stays
-// something that is not finite or larger than any weight.
+// with the smallest largest relative error (2.7e-6 in fp32; Remez exchange), times 2^n, whose bits n is shifted into. Below -126 the result is 2^-126. A NaN
+// stays one by that product (n added to the exponent's bits made it the largest finite number).
 __device__ __forceinline__ F2 exp2Poly(F2 x) {
   float a, b;
   splitF2(x, a, b);
@@ -62,10 +62,8 @@ __device__ __forceinline__ F2 exp2Poly(F2 x) {
   p = fmaF2(p, f, both(0.240247443318367f));
   p = fmaF2(p, f, both(0.6931217908859253f));
   p = fmaF2(p, f, both(0.9999992847442627f));
-  float na, nb;
-  splitF2(n, na, nb);
-  splitF2(p, a, b);
-  return makeF2(__int_as_float(__float_as_int(a) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(nb) << 23)));
+  splitF2(n, a, b);
+  return mulF2(p, makeF2(__int_as_float((__float_as_int(a) << 23) + 0x3f800000), __int_as_float((__float_as_int(b) << 23) + 0x3f800000)));
 }
 // Two bf16 values of a 32-bit word.
 __device__ __forceinline__ F2 unpackF2(uint32_t w) { return makeF2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }

@@ -72,3 +72,43 @@ def test_a_long_sequences_first_rows_are_as_exact_as_a_short_one(S, D, window, s
     for n in NAMES:
         oracle.off(n, got[n][:, :, :256], ref)
     assert not got["dk"][:, :, 256:].any() and not got["dv"][:, :, 256:].any()
+
+
+# ---- values that are not finite ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("S, D", [(200, 64), (500, 64), (500, 128)])
+def test_window_attention_a_key_that_is_not_a_number(S, D):
+    """Rows that see it answer NaN, whichever of a tile's columns it is in; the others do not notice."""
+    B = 128
+    q, k, v, dout = _inputs(S, B, 1, 1, S, D)
+    at = torch.arange(B, device="cuda")
+    k[at, 0, at, 5] = math.nan
+    got = _both_ways(q, k, v, dout)
+    sees = torch.arange(S, device="cuda")[None, :] >= at[:, None]
+    assert bool(torch.isnan(got["out"][:, 0][sees]).all()) and bool(torch.isfinite(got["out"][:, 0][~sees]).all())
+    assert bool(torch.isnan(got["dq"][:, 0][sees]).all())
+    assert bool(torch.isnan(got["dk"]).all()) and bool(torch.isnan(got["dv"]).all())  # the last row sees all of them
+
+
+def test_window_attention_a_key_that_is_infinite():
+    """A score of plus infinity leaves no number; one of minus infinity is a key that counts nothing."""
+    B, S, D = 128, 500, 64
+    q, k, v, dout = _inputs(3, B, 1, 1, S, D)
+    at = torch.arange(B, device="cuda")
+    k[at, 0, at, 0] = math.inf
+    sign = torch.where(torch.rand(B, S, device="cuda", generator=_gen(1)) < 0.5, 1.0, -1.0)
+    q[:, 0, :, 0] = sign.to(bf)
+    out = _both_ways(q, k, v, dout)["out"][:, 0]
+    rows = torch.arange(S, device="cuda")
+    sees = rows[None, :] >= at[:, None]
+    nothing = (at[:, None] == 0) & (rows[None, :] == 0)  # no other key
+    bad = (sees & (sign > 0)) | nothing
+    assert bool(torch.isnan(out[bad]).all())
+    k[at, 0, at, 0] = 0
+    scores = q[:, 0].double() @ k[:, 0].double().transpose(1, 2) / math.sqrt(D)
+    scores.masked_fill_(rows[None, :] > rows[:, None], -math.inf)
+    scores[at, :, at] = -math.inf
+    P = torch.softmax(scores, -1)
+    # every weight is rounded to bf16 and the answer again; the scores' own errors are far smaller
+    tol = 2.0 ** -8 * (P @ v[:, 0].double()).abs() + (2.0 ** -8 + 2.0 ** -12) * (P @ v[:, 0].double().abs())
+    good = sees & ~bad
+    assert bool(((out.double() - P @ v[:, 0].double()).abs() <= tol)[good].all())
