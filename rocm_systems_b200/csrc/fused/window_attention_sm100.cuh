@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       l += *other;
       const bool live = row < it.L;
       if (a.lse && side == 0) a.lse[((size_t)it.b * a.H + it.h) * a.padded() + row] = live ? -(m * p.c + log2f(l)) : -INFINITY;
-      const float inv = live ? 1.f / l : 0.f;
+      // (A row whose every score is minus infinity has no softmax; what the polynomial gave for such scores is no answer.)
+      const float inv = !live ? 0.f : m == -INFINITY ? NAN : 1.f / l;
 #pragma unroll
       for (int x = 0; x < HD / 64; x++) {
         uint32_t o[32], w[16];

@@ -112,3 +112,15 @@ def test_window_attention_a_key_that_is_infinite():
     tol = 2.0 ** -8 * (P @ v[:, 0].double()).abs() + (2.0 ** -8 + 2.0 ** -12) * (P @ v[:, 0].double().abs())
     good = sees & ~bad
     assert bool(((out.double() - P @ v[:, 0].double()).abs() <= tol)[good].all())
+
+
+@pytest.mark.parametrize("S", [100, 700])
+def test_window_attention_rows_of_nothing_but_minus_infinity(S):
+    """Rows all of whose visible scores are minus infinity have no softmax."""
+    q, k, v, _ = _inputs(5, 1, 2, 1, S, 64)
+    k[..., 0] = -k[..., 0].abs() - 0.5
+    q[0, 1, S // 2:, 0] = math.inf
+    from rocm_systems_b200.ops import attention
+
+    out = attention.window_attention(q, k, v)
+    assert bool(torch.isnan(out[0, 1, S // 2:]).all()) and bool(torch.isfinite(out[0, 0]).all()) and bool(torch.isfinite(out[0, 1, :S // 2]).all())
