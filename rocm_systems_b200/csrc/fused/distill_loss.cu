@@ -146,12 +146,12 @@ __global__ void __launch_bounds__(kThreads, 6) distillKernel(const Args p, int c
     float best = -INFINITY, norm = 0.f;
     for (int k = lane; k < p.K; k += 32) best = fmaxf(best, prob[k]);
     best = laneMax<32>(best);
-    if (best > -INFINITY)
-      for (int k = lane; k < p.K; k += 32)
-        if (id[k] >= 0) norm += exp2Fast((prob[k] - best) * kLog2e);
+    // Entries of minus infinity have no weight, also where nothing is larger; a value that is not a number (the maximum passes over it) shows.
+    for (int k = lane; k < p.K; k += 32)
+      if (id[k] >= 0 && prob[k] != -INFINITY) norm += exp2Fast((prob[k] - best) * kLog2e);
     norm = laneSum<32>(norm);
     const float logNorm = logf(norm);
-    for (int k = lane; k < p.K; k += 32) prob[k] = id[k] >= 0 && norm != 0.f ? exp2Fast((prob[k] - best - logNorm) * kLog2e) : 0.f;
+    for (int k = lane; k < p.K; k += 32) prob[k] = id[k] >= 0 && prob[k] != -INFINITY ? exp2Fast((prob[k] - best - logNorm) * kLog2e) : 0.f;
     if (lane == 0) teacher[0] = best, teacher[1] = logNorm, teacher[2] = norm == 0.f ? 0.f : 1.f;
   }
 

@@ -124,3 +124,21 @@ def test_window_attention_rows_of_nothing_but_minus_infinity(S):
 
     out = attention.window_attention(q, k, v)
     assert bool(torch.isnan(out[0, 1, S // 2:]).all()) and bool(torch.isfinite(out[0, 0]).all()) and bool(torch.isfinite(out[0, 1, :S // 2]).all())
+
+
+@pytest.mark.parametrize("K", [1, 5, 40])
+def test_distill_loss_a_teacher_that_is_not_a_number(K):
+    """It is not a row without entries: the loss, and the gradient of the entries' logits, are not numbers either."""
+    from rocm_systems_b200.ops import train_ops
+
+    g = _gen(K)
+    logits, tgt = _rand(g, 4, 300), torch.arange(4, device="cuda")
+    ids = torch.stack([torch.randperm(300, device="cuda", generator=g)[:K] for _ in range(4)])
+    values = torch.randn(4, K, device="cuda", generator=g)
+    values[1] = math.nan
+    values[2, K - 1] = math.nan
+    values[3] = -math.inf      # entries of no weight: a row without any
+    for weight in (0.5, 1.0):
+        loss, grad = train_ops.distill_loss(logits, tgt, ids, values, weight, 2.0)
+        assert torch.isnan(loss).tolist() == [False, True, True, False]
+        assert torch.isnan(grad.gather(1, ids)).all(-1).tolist() == [False, True, True, False] and bool(torch.isfinite(grad[[0, 3]]).all())
