@@ -158,10 +158,16 @@ __global__ void __launch_bounds__(kThreads, 6) distillKernel(const Args p, int c
   // ---- the slice's sums, relative to its own maximum: one exchange with the cluster is enough
   const float soft = MODE == kOne && p.a == 0.f ? kLog2e : kLog2e / p.tau, one = kLog2e;
   const F2 soft2 = makeF2(soft, soft), one2 = makeF2(one, one);
+  // Exponents are v soft + off with off = -(top soft) rounded, so that each is (v - top) soft and, for all of a slice alike, what that rounding took.
+  // It is taken out of the sums again: of 100 / 0.01 in powers of two it is up to 2^-11.
   F2 offSoft, offOne;
+  float tookSoft, tookOne;
+  constexpr float kPower = MODE == kPower2 ? 2.f : MODE == kPower3 ? 3.f : 4.f;
   const auto relativeTo = [&](float top) {
     offSoft = makeF2(-top * soft, -top * soft);
     offOne = makeF2(-top * one, -top * one);
+    tookSoft = fmaf(top, soft, -top * soft);
+    tookOne = MODE >= kPower2 ? kPower * tookSoft : MODE == kTwo ? fmaf(top, one, -top * one) : tookSoft;
   };
   const auto powers = [&](F2 v, F2& q, F2& c) {
     q = exp2F2(fmaF2(v, soft2, offSoft));
@@ -196,7 +202,9 @@ __global__ void __launch_bounds__(kThreads, 6) distillKernel(const Args p, int c
   float sumSoft, sumOne, upper, upperOne;
   splitF2(partSoft, sumSoft, upper);
   splitF2(partOne, sumOne, upperOne);
-  const float2 both = blockSum(make_float2(sumSoft + upper, sumOne + upperOne), sums);
+  float2 both = blockSum(make_float2(sumSoft + upper, sumOne + upperOne), sums);
+  both.x *= exp2f(-tookSoft);
+  both.y *= exp2f(-tookOne);
   // Each CTA tells all of them, and goes on when all have told it: then they have also read the logits that they look up, which the gradient
   // may be about to take the place of.
   clusterWait();
@@ -213,10 +221,12 @@ __global__ void __launch_bounds__(kThreads, 6) distillKernel(const Args p, int c
   }
   if (MODE == kOne) sumOne = sumSoft;
   relativeTo(m);
+  // The gradient's powers have the row's own rounding in them, so its factors have the sums with it.
+  const float gradSoft = sumSoft * exp2f(tookSoft), gradOne = sumOne * exp2f(tookOne);
   const float a = teacher[2] == 0.f ? 0.f : p.a;
 
   // ---- the gradient, in the logits' place
-  const float fOne = p.a < 1.f ? (1.f - p.a) / sumOne * p.gradScale : 0.f, fSoft = a == 0.f ? 0.f : a * p.tau / sumSoft * p.gradScale;
+  const float fOne = p.a < 1.f ? (1.f - p.a) / gradOne * p.gradScale : 0.f, fSoft = a == 0.f ? 0.f : a * p.tau / gradSoft * p.gradScale;
   const F2 fOne2 = makeF2(fOne, fOne), fSoft2 = MODE == kOne ? makeF2(fOne + fSoft, fOne + fSoft) : makeF2(fSoft, fSoft);
   const auto dense = [&](F2 v) {
     F2 q, c;
@@ -271,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 6) distillKernel(const Args p, int c
     kl = laneSum<32>(kl);
     if (lane == 0) {
       float loss = a == 0.f ? 0.f : a * p.tau * p.tau * kl;
-      if (p.a < 1.f) loss += (1.f - p.a) * (m + logf(sumOne) - teacher[3]);
+      if (p.a < 1.f) loss += (1.f - p.a) * ((m - teacher[3]) + logf(sumOne));
       p.loss[row] = loss;
     }
   }

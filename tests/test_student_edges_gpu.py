@@ -142,3 +142,29 @@ def test_distill_loss_a_teacher_that_is_not_a_number(K):
         loss, grad = train_ops.distill_loss(logits, tgt, ids, values, weight, 2.0)
         assert torch.isnan(loss).tolist() == [False, True, True, False]
         assert torch.isnan(grad.gather(1, ids)).all(-1).tolist() == [False, True, True, False] and bool(torch.isfinite(grad[[0, 3]]).all())
+
+
+@pytest.mark.parametrize("weight, tau", [(0.0, 1.0), (0.0, 3.0), (1.0, 1.0), (1.0, 0.01), (1.0, 0.1), (0.5, 1.0), (0.5, 2.0), (0.5, 3.0), (0.5, 4.0), (0.5, 2.5), (0.5, 0.1)])
+@pytest.mark.parametrize("V", [500, 40000])
+def test_distill_loss_small_losses_of_large_logits(V, weight, tau):
+    """A student that is all but sure of what target and teacher say: the loss is the logarithm of a sum that hardly differs from one.
+
+    Each power of two is off by 2^-22 of itself, of the largest one that is the sum's error, once more where the slices' sums are joined; the logarithm adds
+    2^-23: below 2^-20 together, of each softmax. Nothing of it grows with the logits' size."""
+    from rocm_systems_b200.ops import train_ops
+
+    tops = torch.cat([torch.arange(16, 32, 0.125), torch.arange(32, 128, 0.5)]).to("cuda")
+    T = tops.numel()
+    g = _gen(V)
+    logits = _rand(g, T, V, scale=0.5)
+    tgt = torch.randint(0, V, (T,), device="cuda", generator=g)
+    logits[torch.arange(T), tgt] = tops.to(bf)
+    loss, _ = train_ops.distill_loss(logits, tgt, tgt[:, None].contiguous(), torch.zeros(T, 1, device="cuda"), weight, tau)
+    z = logits.double()
+    ce, kl = (-torch.log_softmax(z / t, -1).gather(1, tgt[:, None])[:, 0] for t in (1.0, tau))
+    want = (1 - weight) * ce + weight * tau ** 2 * kl
+    # sums over the row: one rounding per addition of a thread (128 of them side by side in each of up to 8 slices) and of the tree behind them
+    seq = (V / 128 + 16) * 2.0 ** -24
+    tol = (1 - weight) * (2.0 ** -20 + seq * ce) + weight * tau ** 2 * (2.0 ** -20 + seq * kl) + 2.0 ** -18 * want
+    over = (loss.double() - want).abs() - tol
+    assert bool((over <= 0).all()), (float(over.max()), float(want[over.argmax()]), float(tops[over.argmax()]))
