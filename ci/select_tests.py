@@ -31,11 +31,11 @@ RULES = [
     ("rocm_systems_b200/csrc/shmem/*", ["tests/test_api_cpu.py"], ["tests/test_gpu_fused_multi.py", "tests/test_shmem_dma_gpu.py"], True),
     ("rocm_systems_b200/csrc/fused/fsdp_kernels.cu", ["tests/test_fsdp_rscast_emulation_cpu.py", "tests/test_protocol_model_cpu.py"], ["tests/test_gpu_fused_multi.py"], True),
     ("rocm_systems_b200/csrc/fused/gemm_fp8*", ["tests/test_fp8_reference_cpu.py"], [], True),
-    ("rocm_systems_b200/csrc/fused/qk_norm_rope.cu", ["tests/test_student_ops_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
-    ("rocm_systems_b200/csrc/fused/window_attention*", ["tests/test_student_ops_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
-    ("rocm_systems_b200/csrc/fused/distill_loss.cu", ["tests/test_student_ops_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
-    ("rocm_systems_b200/csrc/fused/rows.cuh", ["tests/test_student_ops_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
-    ("rocm_systems_b200/csrc/torch/student_ops.cpp", ["tests/test_student_ops_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
+    ("rocm_systems_b200/csrc/fused/qk_norm_rope.cu", ["tests/test_student_ops_cpu.py", "tests/test_student_edges_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
+    ("rocm_systems_b200/csrc/fused/window_attention*", ["tests/test_student_ops_cpu.py", "tests/test_student_edges_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
+    ("rocm_systems_b200/csrc/fused/distill_loss.cu", ["tests/test_student_ops_cpu.py", "tests/test_student_edges_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
+    ("rocm_systems_b200/csrc/fused/rows.cuh", ["tests/test_student_ops_cpu.py", "tests/test_student_edges_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
+    ("rocm_systems_b200/csrc/torch/student_ops.cpp", ["tests/test_student_ops_cpu.py", "tests/test_student_edges_cpu.py", "tests/test_kernel_resources_cpu.py"], ["tests/test_student_ops_gpu.py", "tests/test_student_edges_gpu.py", "tests/test_llama_student_gpu.py"], True),
     ("rocm_systems_b200/csrc/fused/*", ["tests/test_kernel_resources_cpu.py"], ["tests/test_gemm_gpu.py", "tests/test_train_ops_gpu.py", "tests/test_gpu_fused_multi.py", "tests/test_zz_fused_single_gpu.py", "tests/test_zz_no_alloc.py"], True),
     ("rocm_systems_b200/csrc/torch/*", ["tests/test_dist_cpu.py"], ["tests/test_gpu_collectives.py"], True),
     ("rocm_systems_b200/csrc/trace/kokkosp.cc", ["tests/test_kokkosp_cpu.py", "tests/test_sanitizers_cpu.py"], [], True),

@@ -43,6 +43,11 @@ void check(int rc, const char* what, int launches) {
 }
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "this operator's gradient is not itself differentiable (create_graph)"); }
 
+// There is no forward-mode derivative here; without this a tangent would be dropped in silence, as its tensor need not require a gradient.
+void noTangent(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) need(!t->_fw_grad(/*level=*/0).defined(), "forward-mode derivatives are not implemented (an input is a dual tensor)");
+}
+
 bool onOneDevice(const Tensor& t, std::initializer_list<const Tensor*> others) {
   for (const Tensor* o : others)
     if (o->device() != t.device()) return false;
@@ -121,6 +126,7 @@ std::tuple<Tensor, Tensor, Tensor> qkNormRope(const Tensor& qkv, const Tensor& w
   need(table.scalar_type() == at::kFloat && table.is_contiguous() && (reinterpret_cast<uintptr_t>(ptr(table)) & 15) == 0, "table: contiguous fp32");
   need(eps >= 0 && std::isfinite(eps), "eps: finite, not negative");
   need(qkv.size(0) * S < (1LL << 30) && heads + 2 * kv < (1LL << 14), "too many positions or heads");
+  noTangent({&qkv, &wq, &wk, &table});
   need(onOneDevice(qkv, {&wq, &wk, &table}), "tensors on one CUDA device expected");
   variable_list r;
   if (at::GradMode::is_enabled() && (qkv.requires_grad() || wq.requires_grad() || wk.requires_grad()))
@@ -196,6 +202,7 @@ Tensor windowAttention(const Tensor& q, const Tensor& k, const Tensor& v, int64_
   need(!lengthsIn || (lengthsIn->dim() == 1 && lengthsIn->size(0) == B && lengthsIn->scalar_type() == at::kInt && lengthsIn->is_contiguous()),
        "lengths: contiguous int32 [B]");
   need(S < (1LL << 30) && B * k.size(1) < (1LL << 16) && B * H * ((S + 127) / 128) < (1LL << 31), "too many positions, heads or sequences");
+  noTangent({&q, &k, &v});
   const Tensor lengths = lengthsIn.value_or(Tensor());
   need(onOneDevice(q, {&k, &v}) && (!lengths.defined() || lengths.device() == q.device()), "tensors on one CUDA device expected");
   const Numbers n{std::min(window, S), std::min(sinks, S), scaleIn ? *scaleIn : 1.0 / std::sqrt((double)D)};
@@ -229,6 +236,7 @@ std::tuple<Tensor, Tensor> distillLoss(const Tensor& logits, const Tensor& targe
     if (T > 0 && !(from(g) == from(logits) && (T == 1 || g.stride(0) == logits.stride(0))))
       need(to(g) <= from(logits) || to(logits) <= from(g), "grad: logits itself, or memory apart from it");
   }
+  noTangent({&logits, &teacherLogits});
   need(onOneDevice(logits, {&targets, &teacherIds, &teacherLogits}) && (!gradIn || gradIn->device() == logits.device()), "tensors on one CUDA device expected");
   c10::cuda::OptionalCUDAGuard guard(logits.device());
   const Tensor grad = gradIn ? *gradIn : at::empty({T, V}, logits.options());
