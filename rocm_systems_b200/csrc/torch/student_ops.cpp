@@ -126,6 +126,7 @@ std::tuple<Tensor, Tensor, Tensor> qkNormRope(const Tensor& qkv, const Tensor& w
   need(table.scalar_type() == at::kFloat && table.is_contiguous() && (reinterpret_cast<uintptr_t>(ptr(table)) & 15) == 0, "table: contiguous fp32");
   need(eps >= 0 && std::isfinite(eps), "eps: finite, not negative");
   need(qkv.size(0) * S < (1LL << 30) && heads + 2 * kv < (1LL << 14), "too many positions or heads");
+  need(!at::GradMode::is_enabled() || !table.requires_grad(), "table: a gradient is not formed for it");
   noTangent({&qkv, &wq, &wk, &table});
   need(onOneDevice(qkv, {&wq, &wk, &table}), "tensors on one CUDA device expected");
   variable_list r;

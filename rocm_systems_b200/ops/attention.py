@@ -38,7 +38,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     """RMSNorm of every query and key head and the rotation to its position, in one pass over the packed projection.
 
     ``qkv`` [B, S, heads + 2 kv_heads, D] bf16: query, key and value heads of each token, D a multiple of 8 up to 256. ``q_weight`` and
-    ``k_weight`` [D], both bf16 or both fp32, scale the normalised elements; ``table`` [>= S, D / 2, 2] is :func:`train_ops.rope_table`'s.
+    ``k_weight`` [D], both bf16 or both fp32, scale the normalised elements; ``table`` [>= S, D / 2, 2] is :func:`train_ops.rope_table`'s and
+    takes no gradient.
     Returns ``q`` [B, heads, S, D], ``k`` and ``v`` [B, kv_heads, S, D]; ``v`` is a view of ``qkv``. The backward pass writes one packed
     gradient for ``qkv`` and the weights' gradients in their type, in a fixed order of summation."""
     return _ext().qk_norm_rope(qkv, q_weight, k_weight, table, heads, kv_heads, eps)

@@ -44,3 +44,13 @@ def test_forward_mode_derivatives_are_refused(op, args, dual, grad):
         args[dual] = forward_ad.make_dual(args[dual], torch.ones_like(args[dual]))
         with pytest.raises(AssertionError, match="forward-mode"):
             call(**args)
+
+
+def test_a_table_that_asks_for_a_gradient_is_refused():
+    from rocm_systems_b200.ops import attention
+
+    args = _norm_args(table=torch.zeros(8, 32, 2, requires_grad=True))
+    with pytest.raises(AssertionError, match="table: a gradient"):
+        attention.qk_norm_rope(**args)
+    with torch.no_grad(), pytest.raises(AssertionError, match="CUDA device"):  # nothing but the device is wrong
+        attention.qk_norm_rope(**args)
