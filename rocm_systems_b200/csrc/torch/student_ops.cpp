@@ -246,6 +246,7 @@ std::tuple<Tensor, Tensor> distillLoss(const Tensor& logits, const Tensor& targe
                              (float*)out(loss), T, (int)V, (int)K, std::max(logits.stride(0), V), std::max(grad.stride(0), V), (float)weight, (float)temperature,
                              (float)gradScale, stream()),
         "distill_loss", 1);
+  if (gradIn && !grad.is_inference()) grad.unsafeGetTensorImpl()->bump_version();  // written through its pointer: a graph that saved it has to notice
   return {loss, grad};
 }
 

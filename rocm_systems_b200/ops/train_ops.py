@@ -177,6 +177,8 @@ def cross_entropy_inplace(logits: torch.Tensor, targets: torch.Tensor, grad_scal
     T, V = logits.shape
     loss = torch.empty(T, dtype=torch.float32, device=logits.device)
     _ck(_lib_ops().b200ops_cross_entropy(logits.data_ptr(), targets.data_ptr(), loss.data_ptr(), T, V, logits.stride(0), grad_scale, _s()), "cross_entropy")
+    if not logits.is_inference():
+        torch.autograd.graph.increment_version(logits)  # written through its pointer: a graph that saved it has to notice
     return loss
 
 

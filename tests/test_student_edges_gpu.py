@@ -168,3 +168,29 @@ def test_distill_loss_small_losses_of_large_logits(V, weight, tau):
     tol = (1 - weight) * (2.0 ** -20 + seq * ce) + weight * tau ** 2 * (2.0 ** -20 + seq * kl) + 2.0 ** -18 * want
     over = (loss.double() - want).abs() - tol
     assert bool((over <= 0).all()), (float(over.max()), float(want[over.argmax()]), float(tops[over.argmax()]))
+
+
+@pytest.mark.parametrize("loss", ["distill", "cross_entropy"])
+def test_a_gradient_in_the_logits_place_is_seen_by_autograd(loss):
+    """A graph that saved the logits refuses its backward pass once the gradient has taken their place."""
+    from rocm_systems_b200.ops import train_ops
+
+    x = _rand(_gen(1), 4, 64).requires_grad_(True)
+    tgt, ids, values = torch.arange(4, device="cuda"), torch.zeros(4, 1, dtype=torch.int64, device="cuda"), torch.zeros(4, 1, device="cuda")
+    logits = x * 2
+    other = logits.square().sum()  # keeps the logits
+    version = logits._version
+    with torch.no_grad():
+        if loss == "distill":
+            train_ops.distill_loss(logits, tgt, ids, values, 0.5, 2.0)
+            assert logits._version == version
+            train_ops.distill_loss(logits, tgt, ids, values, 0.5, 2.0, grad=logits)
+        else:
+            train_ops.cross_entropy_inplace(logits, tgt, 1.0)
+    assert logits._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        other.backward()
+    with torch.inference_mode():  # tensors without versions
+        plain = torch.zeros(4, 64, dtype=bf, device="cuda")
+        train_ops.distill_loss(plain, tgt, ids, values, 0.5, 2.0, grad=plain)
+        train_ops.cross_entropy_inplace(plain, tgt, 1.0)
