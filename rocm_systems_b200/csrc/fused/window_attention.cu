@@ -18,6 +18,14 @@ static bool wide(const Tensor& t) { return ((uintptr_t)t.p & 31) == 0 && t.b % 1
 static Tensor packed(const void* p, const Args& a) { return {(const __nv_bfloat16*)p, (long long)a.S * a.H * a.D, a.D, (long long)a.H * a.D}; }
 static bool aligned(const Tensor& t) { return t.p && ((uintptr_t)t.p & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.s % 8 == 0; }
 
+static Args sizes(int B, int H, int KV, int S, int D, int window, int sinks) {
+  Args a{};
+  a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
+  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
+  a.sinks = sinks < S ? sinks : S;
+  return a;
+}
+
 // The device's context made current on this thread: encoding a tensor map asks for one, and a backward pass may be the first that its
 // thread does.
 static void bindContext() {
@@ -138,16 +146,13 @@ extern "C" {
 int b200ops_window_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int* lengths, const long long* strides, int B, int H, int KV,
                                  int S, int D, int window, int sinks, float scale, cudaStream_t s) {
   const auto tensor = [&](const void* p, int i) { return Tensor{(const __nv_bfloat16*)p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
-  Args a{};
+  Args a = sizes(B, H, KV, S, D, window, sinks);
   a.q = tensor(q, 0);
   a.k = tensor(k, 1);
   a.v = tensor(v, 2);
   a.out = tensor(out, 3);
   a.lse = lse;
   a.lengths = lengths;
-  a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
-  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
-  a.sinks = sinks < S ? sinks : S;
   a.scale = scale;
   a.rest = packed(rest, a);
   if (!good(a) || !aligned(a.q) || !aligned(a.k) || !aligned(a.v) || !aligned(a.out) || ((uintptr_t)rest & 15)) return (int)cudaErrorInvalidValue;
@@ -161,7 +166,7 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
                                  void* dv, const int* lengths, const long long* strides, int B, int H, int KV, int S, int D, int window, int sinks, float scale,
                                  cudaStream_t s) {
   const auto tensor = [&](const void* p, int i) { return Tensor{(const __nv_bfloat16*)p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
-  Args a{};
+  Args a = sizes(B, H, KV, S, D, window, sinks);
   a.q = tensor(q, 0);
   a.k = tensor(k, 1);
   a.v = tensor(v, 2);
@@ -173,9 +178,6 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
   a.lse = const_cast<float*>(lse);
   a.stat = reinterpret_cast<__nv_bfloat16*>(scratch);
   a.lengths = lengths;
-  a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
-  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
-  a.sinks = sinks < S ? sinks : S;
   a.scale = scale;
   a.rest = packed(rest, a);
   if (!good(a) || !lse || !scratch || !rest || (((uintptr_t)rest | (uintptr_t)lse | (uintptr_t)scratch) & 15)) return (int)cudaErrorInvalidValue;
@@ -187,14 +189,20 @@ int b200ops_window_attention_bwd(const void* q, const void* k, const void* v, co
 }
 
 long long b200ops_window_attention_bwd_scratch(int B, int H, int KV, int S, int D, int window, int sinks) {
-  Args a{};
-  a.B = B, a.H = H, a.KV = KV, a.S = S, a.D = D;
-  a.window = window == 0 || sinks >= S ? S : window;  // S or more: every earlier key
-  a.sinks = sinks < S ? sinks : S;
+  const Args a = sizes(B, H, KV, S, D, window, sinks);
   if (!good(a)) return -1;
   BwdParams p{};
   splitSinks(a, p);
   return (long long)B * H * a.padded() * 4 + partialWords(a, p);
+}
+
+// Kernels that the backward call launches: for the queries, for the keys and, where the sinks' queries are split, for their sums.
+int b200ops_window_attention_bwd_launches(int B, int H, int KV, int S, int D, int window, int sinks) {
+  const Args a = sizes(B, H, KV, S, D, window, sinks);
+  if (!good(a)) return -1;
+  BwdParams p{};
+  splitSinks(a, p);
+  return p.sinkTiles ? 3 : 2;
 }
 
 }  // extern "C"

@@ -18,6 +18,7 @@ int b200ops_qk_norm_rope_bwd(const void*, const void*, const void*, const long l
 int b200ops_window_attention_fwd(const void*, const void*, const void*, void*, float*, void*, const int*, const long long*, int, int, int, int, int, int, int, float,
                                  cudaStream_t);
 long long b200ops_window_attention_bwd_scratch(int, int, int, int, int, int, int);
+int b200ops_window_attention_bwd_launches(int, int, int, int, int, int, int);
 int b200ops_window_attention_bwd(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, const int*,
                                  const long long*, int, int, int, int, int, int, int, float, cudaStream_t);
 int b200ops_distill_loss(const void*, void*, const long long*, const void*, int, const void*, int, float*, long long, int, int, long long, long long, float, float, float,
@@ -186,7 +187,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     check(b200ops_window_attention_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(rest), ptr(g), (const float*)ptr(lse), (float*)out(scratch), out(dq), out(dk), out(dv),
                                        lengths.defined() ? (const int*)ptr(lengths) : nullptr, st.data(), B, H, KV, S, D, window, sinks,
                                        (float)ctx->saved_data["scale"].toDouble(), stream()),
-          "window_attention_bwd", 2);
+          "window_attention_bwd", b200ops_window_attention_bwd_launches(B, H, KV, S, D, window, sinks));
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -245,7 +246,7 @@ std::tuple<Tensor, Tensor> distillLoss(const Tensor& logits, const Tensor& targe
   check(b200ops_distill_loss(ptr(logits), out(grad), (const long long*)ptr(targets), ptr(ids), (int)ids.element_size(), ptr(values), (int)values.element_size(),
                              (float*)out(loss), T, (int)V, (int)K, std::max(logits.stride(0), V), std::max(grad.stride(0), V), (float)weight, (float)temperature,
                              (float)gradScale, stream()),
-        "distill_loss", 1);
+        "distill_loss", T > 0);
   if (gradIn && !grad.is_inference()) grad.unsafeGetTensorImpl()->bump_version();  // written through its pointer: a graph that saved it has to notice
   return {loss, grad};
 }

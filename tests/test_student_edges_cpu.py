@@ -54,3 +54,18 @@ def test_a_table_that_asks_for_a_gradient_is_refused():
         attention.qk_norm_rope(**args)
     with torch.no_grad(), pytest.raises(AssertionError, match="CUDA device"):  # nothing but the device is wrong
         attention.qk_norm_rope(**args)
+
+
+@pytest.mark.parametrize("S, window, sinks, launches", [(900, 0, 0, 2), (900, 100, 0, 2), (900, 100, 3, 3), (900, 0, 3, 2), (900, 900, 3, 2), (200, 100, 3, 2), (1, 1, 1, 2),
+                                                        (900, 100, 900, 2)])
+def test_window_attention_says_how_many_kernels_a_backward_call_launches(S, window, sinks, launches):
+    import ctypes
+
+    from rocm_systems_b200 import _lib
+
+    args = (1, 2, 1, S, 64, window, sinks)
+    count, words = _lib.load().b200ops_window_attention_bwd_launches, _lib.load().b200ops_window_attention_bwd_scratch
+    count.argtypes, words.argtypes, words.restype = [ctypes.c_int] * 7, [ctypes.c_int] * 7, ctypes.c_longlong
+    assert count(*args) == launches
+    assert (words(*args) > 2 * ((S + 127) // 128 * 128) * 4) == (launches == 3)  # partial sums, and the kernel that adds them up
+    assert count(1, 2, 1, S, 60, window, sinks) == -1

@@ -194,3 +194,33 @@ def test_a_gradient_in_the_logits_place_is_seen_by_autograd(loss):
         plain = torch.zeros(4, 64, dtype=bf, device="cuda")
         train_ops.distill_loss(plain, tgt, ids, values, 0.5, 2.0, grad=plain)
         train_ops.cross_entropy_inplace(plain, tgt, 1.0)
+
+def _norm_inputs(seed, B=2, S=37, heads=4, kv=2, D=64, weights=bf):
+    from rocm_systems_b200.ops import train_ops
+
+    g = _gen(seed)
+    qkv = _rand(g, B, S, heads + 2 * kv, D)
+    w = [(1 + 0.3 * torch.randn(D, device="cuda", generator=g)).to(weights) for _ in range(2)]
+    grads = tuple(_rand(g, B, S, n, D).transpose(1, 2) for n in (heads, kv, kv))
+    return (qkv, *w), train_ops.rope_table(S, D, 10000.0, "cuda"), grads
+
+def test_launches_are_counted():
+    from rocm_systems_b200.ops import attention, train_ops
+
+    def count(fn):
+        before = attention.launches()
+        fn()
+        return attention.launches() - before
+
+    q, k, v, dout = _inputs(2, 1, 2, 1, 900, 64)
+    assert count(lambda: attention.window_attention(q, k, v, 100, 3)) == 1
+    assert count(lambda: _both_ways(q, k, v, dout)) == 3
+    assert count(lambda: _both_ways(q, k, v, dout, 100, 3)) == 4      # the sinks' sums are joined
+    assert count(lambda: _both_ways(q, k, v, dout, 100, 0)) == 3
+    inputs, table, grads = _norm_inputs(1)
+    leaf = inputs[0].detach().requires_grad_(True)
+    assert count(lambda: attention.qk_norm_rope(*inputs, table, 4, 2)) == 1
+    assert count(lambda: torch.autograd.grad(attention.qk_norm_rope(leaf, *inputs[1:], table, 4, 2), leaf, grads)) == 3
+    logits, tgt, ids, values = _rand(_gen(1), 3, 64), torch.arange(3, device="cuda"), torch.zeros(3, 1, dtype=torch.int64, device="cuda"), torch.zeros(3, 1, device="cuda")
+    assert count(lambda: train_ops.distill_loss(logits, tgt, ids, values)) == 1
+    assert count(lambda: train_ops.distill_loss(logits[:0], tgt[:0], ids[:0], values[:0])) == 0
