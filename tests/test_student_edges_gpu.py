@@ -224,3 +224,97 @@ def test_launches_are_counted():
     logits, tgt, ids, values = _rand(_gen(1), 3, 64), torch.arange(3, device="cuda"), torch.zeros(3, 1, dtype=torch.int64, device="cuda"), torch.zeros(3, 1, device="cuda")
     assert count(lambda: train_ops.distill_loss(logits, tgt, ids, values)) == 1
     assert count(lambda: train_ops.distill_loss(logits[:0], tgt[:0], ids[:0], values[:0])) == 0
+
+
+# ---- what autograd may do with a call -----------------------------------------------------------------------------------
+def test_gradients_of_gradients_are_refused():
+    from rocm_systems_b200.ops import attention
+
+    q, k, v, dout = _inputs(1, 1, 2, 1, 20, 64)
+    q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not itself differentiable"):
+        torch.autograd.grad(attention.window_attention(q, k, v), q, dout, create_graph=True)
+    (qkv, wq, wk), table, grads = _norm_inputs(2)
+    qkv.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not itself differentiable"):
+        torch.autograd.grad(attention.qk_norm_rope(qkv, wq, wk, table, 4, 2), qkv, grads, create_graph=True)
+
+
+@pytest.mark.parametrize("S, window, sinks", [(150, 0, 0), (500, 90, 3)])
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (0, 2)])
+def test_a_gradient_of_some_inputs_only(S, window, sinks, which):
+    """The same bits as when all of them need one."""
+    from rocm_systems_b200.ops import attention
+
+    q, k, v, dout = _inputs(S, 2, 4, 2, S, 64)
+    want = _both_ways(q, k, v, dout, window, sinks)
+    leaves = [t.detach().requires_grad_(i in which) for i, t in enumerate((q, k, v))]
+    got = torch.autograd.grad(attention.window_attention(*leaves, window, sinks), [leaves[i] for i in which], dout)
+    for i, t in zip(which, got):
+        assert torch.equal(t, want[("dq", "dk", "dv")[i]])
+
+
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (0, 1)])
+def test_norms_a_gradient_of_some_inputs_only(which):
+    from rocm_systems_b200.ops import attention
+
+    inputs, table, grads = _norm_inputs(3)
+
+    def run(which):
+        leaves = [t.detach().requires_grad_(i in which) for i, t in enumerate(inputs)]
+        return torch.autograd.grad(attention.qk_norm_rope(*leaves, table, 4, 2), [leaves[i] for i in which], grads)
+
+    want = run((0, 1, 2))
+    assert all(torch.equal(t, want[i]) for i, t in zip(which, run(which)))
+
+
+# ---- padded batches and head dimensions beyond 256 tokens ----------------------------------------------------------------
+@pytest.mark.parametrize("lengths", [(700, 0, 1, 3), (127, 129, 700, 400), (257, 512, 640, 641)])
+@pytest.mark.parametrize("D, window, sinks", [(64, 0, 0), (96, 0, 0), (128, 0, 0), (64, 100, 4), (128, 100, 4), (72, 130, 140), (128, 130, 140), (96, 300, 600)])
+def test_padded_batches_of_longer_sequences(lengths, D, window, sinks):
+    """As for the short ones: NaN and infinities behind a sequence's end are not used; its rows answer zeros and get zero gradients, also where the
+    sinks' later queries are split and a sequence ends before them or among the sinks."""
+    S = 700
+    q, k, v, dout = _inputs(D + window, 4, 4, 2, S, D)
+    L = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for t in (q, k, v, dout):
+        for b, n in enumerate(lengths):
+            t[b, :, n:] = math.nan
+            t[b, :, n:, ::3] = math.inf
+    got = _against_the_oracle(q, k, v, dout, window, sinks, L)
+    for n, t in got.items():
+        for b, m in enumerate(lengths):
+            assert not t[b, :, m:].any(), n
+
+
+@pytest.mark.parametrize("lengths", [(1100, 3), (130, 1099), (0, 513)])
+@pytest.mark.parametrize("D, window, sinks", [(128, 100, 4), (64, 65, 300), (40, 0, 0)])
+def test_padded_batches_of_long_sequences(lengths, D, window, sinks):
+    S = 1100
+    q, k, v, dout = _inputs(D + window, 2, 2, 1, S, D)
+    L = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for t in (q, k, v, dout):
+        for b, n in enumerate(lengths):
+            t[b, :, n:] = math.nan
+    got = _against_the_oracle(q, k, v, dout, window, sinks, L)
+    for n, t in got.items():
+        for b, m in enumerate(lengths):
+            assert not t[b, :, m:].any(), n
+
+
+@pytest.mark.parametrize("B, H, KV, D", [(1, 1, 1, 8), (2, 3, 1, 128), (1, 4, 4, 104), (2, 6, 2, 96), (1, 8, 1, 40), (3, 2, 2, 16), (1, 5, 5, 72), (1, 7, 1, 120)])
+@pytest.mark.parametrize("S, window, sinks", [(400, 0, 0), (400, 90, 5), (641, 129, 1)])
+def test_head_dimensions_of_longer_sequences(B, H, KV, D, S, window, sinks):
+    _against_the_oracle(*_inputs(S + D, B, H, KV, S, D), window, sinks)
+
+
+@pytest.mark.parametrize("D", [64, 72, 128])
+def test_layouts_of_longer_sequences(D):
+    """Heads outside positions, rows off 16 bytes, one key head's memory for all, a transposed gradient, a gradient that is one number."""
+    B, H, KV, S = 2, 4, 2, 450
+    g = _gen(D)
+    q = _rand(g, B, H, S, D)
+    k = _rand(g, B * KV * S * D + 1)[1:].view(B, KV, S, D)
+    v = _rand(g, B, 1, S, D).expand(B, KV, S, D)
+    _against_the_oracle(q, k, v, _rand(g, B, H, D, S).transpose(2, 3), 133, 2)
+    _against_the_oracle(_rand(g, B, S, H, D + 8)[..., :D].transpose(1, 2), k, v, _rand(g, 1, 1, 1, 1).expand(B, H, S, D), 0, 0)
