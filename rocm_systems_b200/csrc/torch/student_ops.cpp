@@ -62,6 +62,14 @@ Tensor rows16(const Tensor& t) {
   for (int d = 0; d < 3; d++) fine = fine && (t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0));
   return fine ? t : t.clone(at::MemoryFormat::Contiguous);
 }
+// `t` if it is dense and starts on a 16-byte boundary; else a copy.
+Tensor dense16(const Tensor& t) {
+  return t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// A hook on saved tensors promises equal values; in which memory they come back is its own affair.
+void cameBack(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const Tensor& grad) {
+  TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == grad.device(), "a saved tensor came back as something else");
+}
 // (batch, head, position) strides of [B, heads, S, D] tensors in turn; of a dimension of one the stride is nothing.
 template <size_t N> std::array<long long, 3 * N> strides(const std::array<const Tensor*, N>& ts) {
   std::array<long long, 3 * N> s{};
@@ -96,14 +104,20 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     ctx->saved_data["heads"] = heads;
     ctx->saved_data["kv"] = kv;
     ctx->saved_data["eps"] = eps;
+    ctx->saved_data["wide"] = wq.scalar_type() == at::kFloat;
     return normForward(qkv, wq, wk, table, heads, kv, eps);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once();
     const auto saved = ctx->get_saved_variables();
-    const Tensor &qkv = saved[0], &wq = saved[1], &wk = saved[2], &table = saved[3];
-    const int64_t heads = ctx->saved_data["heads"].toInt(), kv = ctx->saved_data["kv"].toInt(), B = qkv.size(0), S = qkv.size(1), D = qkv.size(3);
-    c10::cuda::OptionalCUDAGuard guard(qkv.device());
+    const int64_t heads = ctx->saved_data["heads"].toInt(), kv = ctx->saved_data["kv"].toInt(), B = grads[0].size(0), S = grads[0].size(2), D = grads[0].size(3);
+    const auto weights = ctx->saved_data["wide"].toBool() ? at::kFloat : at::kBFloat16;
+    cameBack(saved[0], {B, S, heads + 2 * kv, D}, at::kBFloat16, grads[0]);
+    for (int i = 1; i < 3; i++) cameBack(saved[i], {D}, weights, grads[0]);
+    cameBack(saved[3], {saved[3].size(0), D / 2, 2}, at::kFloat, grads[0]);
+    TORCH_CHECK(saved[3].size(0) >= S, "a saved tensor came back as something else");
+    c10::cuda::OptionalCUDAGuard guard(grads[0].device());
+    const Tensor qkv = dense16(saved[0]), wq = saved[1].contiguous(), wk = saved[2].contiguous(), table = dense16(saved[3]);
     const Tensor dq = rows16(grads[0]), dk = rows16(grads[1]), dv = rows16(grads[2]);
     const Tensor dqkv = at::empty_like(qkv), dwq = at::empty_like(wq), dwk = at::empty_like(wk);
     const Tensor scratch = at::empty({(int64_t)b200ops_qk_norm_rope_bwd_scratch((int)D, (int)heads, (int)kv)}, qkv.options().dtype(at::kFloat));
@@ -170,17 +184,21 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["kv"] = k.size(1);
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once();
     const auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &rest = saved[4], &lse = saved[5];
-    const Tensor lengths = saved.size() > 6 ? saved[6] : Tensor();
-    const int B = (int)q.size(0), H = (int)q.size(1), KV = (int)k.size(1), S = (int)q.size(2), D = (int)q.size(3);
+    const int B = (int)grads[0].size(0), H = (int)grads[0].size(1), KV = (int)ctx->saved_data["kv"].toInt(), S = (int)grads[0].size(2), D = (int)grads[0].size(3);
+    for (int i = 0; i < 4; i++) cameBack(saved[i], {B, i == 1 || i == 2 ? KV : H, S, D}, at::kBFloat16, grads[0]);
+    cameBack(saved[4], {B, S, H, D}, at::kBFloat16, grads[0]);
+    cameBack(saved[5], {B, H, (S + 127) / 128 * 128}, at::kFloat, grads[0]);
+    if (saved.size() > 6) cameBack(saved[6], {B}, at::kInt, grads[0]);
     const int window = (int)ctx->saved_data["window"].toInt(), sinks = (int)ctx->saved_data["sinks"].toInt();
-    c10::cuda::OptionalCUDAGuard guard(q.device());
-    const Tensor g = rows16(grads[0]);
+    c10::cuda::OptionalCUDAGuard guard(grads[0].device());
+    const Tensor q = rows16(saved[0]), k = rows16(saved[1]), v = rows16(saved[2]), o = rows16(saved[3]), rest = dense16(saved[4]), lse = dense16(saved[5]);
+    const Tensor lengths = saved.size() > 6 ? saved[6].contiguous() : Tensor(), g = rows16(grads[0]);
     const Tensor dq = byToken(B, H, S, D, q), dk = byToken(B, KV, S, D, q), dv = byToken(B, KV, S, D, q);
     const Tensor scratch = at::empty({(int64_t)b200ops_window_attention_bwd_scratch(B, H, KV, S, D, window, sinks)}, lse.options());
     const auto st = strides<8>({&q, &k, &v, &o, &g, &dq, &dk, &dv});

@@ -195,6 +195,7 @@ def test_a_gradient_in_the_logits_place_is_seen_by_autograd(loss):
         train_ops.distill_loss(plain, tgt, ids, values, 0.5, 2.0, grad=plain)
         train_ops.cross_entropy_inplace(plain, tgt, 1.0)
 
+
 def _norm_inputs(seed, B=2, S=37, heads=4, kv=2, D=64, weights=bf):
     from rocm_systems_b200.ops import train_ops
 
@@ -318,3 +319,60 @@ def test_layouts_of_longer_sequences(D):
     v = _rand(g, B, 1, S, D).expand(B, KV, S, D)
     _against_the_oracle(q, k, v, _rand(g, B, H, D, S).transpose(2, 3), 133, 2)
     _against_the_oracle(_rand(g, B, S, H, D + 8)[..., :D].transpose(1, 2), k, v, _rand(g, 1, 1, 1, 1).expand(B, H, S, D), 0, 0)
+
+
+def _elsewhere(t):
+    """The same values in other memory: dimensions in another order, every row off its 16 bytes."""
+    if t.dim() < 2:
+        return torch.cat([t[:1], t])[1:]
+    room = torch.empty(tuple(reversed(t.shape[:-1])) + (t.shape[-1] + 1,), dtype=t.dtype, device=t.device)
+    room = room[..., 1:].permute(*reversed(range(t.dim() - 1)), t.dim() - 1)
+    return room.copy_(t)
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.clone(memory_format=torch.contiguous_format), _elsewhere])
+def test_saved_tensors_may_come_back_in_other_memory(unpack):
+    """A hook on saved tensors gives back equal values; where and in which order they lie is its own affair."""
+    from rocm_systems_b200.ops import attention
+
+    q, k, v, dout = _inputs(9, 2, 4, 2, 300, 64)
+    inputs, table, grads = _norm_inputs(4)
+    L = torch.tensor([300, 170], dtype=torch.int32, device="cuda")
+
+    def run():
+        a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        b = [t.detach().requires_grad_(True) for t in inputs]
+        out, normed = attention.window_attention(*a, 90, 3, L), attention.qk_norm_rope(*b, table, 4, 2)
+        return [*torch.autograd.grad(out, a, dout), *torch.autograd.grad(normed, b, grads)]
+
+    want = run()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: unpack(t)):
+        got = run()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_saved_tensors_kept_on_the_host():
+    from rocm_systems_b200.ops import attention
+
+    q, k, v, dout = _inputs(9, 2, 4, 2, 300, 64)
+    want = _both_ways(q, k, v, dout, 90, 3)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    with torch.autograd.graph.save_on_cpu():
+        out = attention.window_attention(*leaves, 90, 3)
+    for n, t in zip(NAMES[1:], torch.autograd.grad(out, leaves, dout)):
+        assert torch.equal(t, want[n]), n
+
+
+def test_saved_tensors_that_are_something_else_are_refused():
+    from rocm_systems_b200.ops import attention
+
+    q, k, v, dout = _inputs(9, 1, 2, 1, 40, 64)
+    inputs, table, grads = _norm_inputs(4)
+    for change in (lambda t: t.float() if t.dtype == bf else t.double() if t.dtype == torch.float32 else t, lambda t: t.cpu(), lambda t: t[..., :-1]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            a, b = q.detach().requires_grad_(True), inputs[0].detach().requires_grad_(True)
+            out, normed = attention.window_attention(a, k, v), attention.qk_norm_rope(b, *inputs[1:], table, 4, 2)
+        with pytest.raises(RuntimeError, match="saved"):
+            torch.autograd.grad(out, a, dout)
+        with pytest.raises(RuntimeError, match="saved"):
+            torch.autograd.grad(normed, b, grads)
