@@ -1026,8 +1026,9 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
 #pragma unroll
               for (int e = 0; e < 16; e++) {
                 const F2 dp = makeF2(__uint_as_float(d[x][2 * e]), __uint_as_float(d[x][2 * e + 1]));
-                F2 v = mulF2(w[x * 16 + e], SIDE == kQueries ? addF2(dp, rowDelta) : dp);
-                if (!decltype(all)::value) v = masked(v, x * 16 + e);  // what is masked may be anything
+                F2 of = SIDE == kQueries ? addF2(dp, rowDelta) : dp;
+                if (!decltype(all)::value) of = masked(of, x * 16 + e);  // what is masked may be anything
+                const F2 v = mulF2(w[x * 16 + e], of);
                 o[e] = pack2(v);
                 if constexpr (FINE) d[x][e] = pack2(remainder(v, o[e]));
                 if constexpr (decltype(rest)::value) o[e] = pack2(remainder(v, o[e]));
@@ -1040,6 +1041,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
               }
             }
           };
+          if (!every) {  // rows that see one key alone (a sequence's first; all with a window of one): its weight is one whatever the score is
+            const bool alone = a.window == 1 && a.sinks == 0;
+#pragma unroll
+            for (int x = 0; x < kCols / 32; x++) {
+              if (alone || (SIDE == kQueries && row == 0)) bits[x] = 0;
+              if (SIDE == kKeys && y0 + cols + x * 32 == 0) bits[x] &= ~1u;
+            }
+          }
           if (!FINE && again) gradients(std::false_type{}, std::true_type{});
           else if (every) gradients(std::true_type{}, std::false_type{});
           else gradients(std::false_type{}, std::false_type{});

@@ -376,3 +376,23 @@ def test_saved_tensors_that_are_something_else_are_refused():
             torch.autograd.grad(out, a, dout)
         with pytest.raises(RuntimeError, match="saved"):
             torch.autograd.grad(normed, b, grads)
+
+
+@pytest.mark.parametrize("S, window, sinks", [(1, 0, 0), (1, 1, 1), (5, 1, 0), (130, 1, 0), (700, 1, 0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_that_see_one_key_have_no_gradient_of_scores(S, window, sinks, D):
+    """Their one weight is one whatever the score is. Not even rounding noise is left of a difference that is zero by definition."""
+    q, k, v, dout = _inputs(S, 2, 4, 2, S, D)
+    got = _against_the_oracle(q, k, v, dout, window, sinks)
+    assert not got["dq"].any() and not got["dk"].any()
+
+
+@pytest.mark.parametrize("S, window, sinks", [(2, 0, 0), (300, 1, 1), (300, 0, 0), (700, 90, 5)])
+def test_a_sequences_first_row_sees_one_key(S, window, sinks):
+    q, k, v, dout = _inputs(S, 2, 4, 2, S, 64)
+    first = torch.zeros_like(dout)
+    first[:, :, 0] = dout[:, :, 0]
+    got = _both_ways(q, k, v, first, window, sinks)
+    assert not got["dq"].any() and not got["dk"].any()
+    q[0, 0, 0, 0] = math.nan
+    assert bool(torch.isnan(_both_ways(q, k, v, first, window, sinks)["dq"][0, 0, 0]).all())
