@@ -65,16 +65,18 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
 }
 
 // Weights and their gradients (P and dS) go to the tensor cores in bf16, each off by 2^-9 of itself. Over many keys that averages out. Where rows
-// see a few keys the gradient is a small difference of such numbers (3 tokens: 0.0039 to 0.0052 of its norm). So for the first kFineSeq queries
-// of a sequence, and where no row sees more than kFineKeys keys, they are handed over as the sum of two bf16 values, which leaves the
-// result's own rounding. The rule looks at a query's position alone: what a sequence answers does not hang on the batch that it is padded in.
+// see a few keys the gradient is a small difference of such numbers (3 tokens: 0.0039 to 0.0052 of its norm). So in sequences of at most
+// kFineSeq tokens, for the first kTile queries of longer ones, and where no row sees more than kFineKeys keys, they are handed over as the sum
+// of two bf16 values, which leaves the result's own rounding. The rule looks at a sequence's own length and a query's position: what a sequence
+// answers does not hang on the batch that it is padded in.
 //
 // Kernels for calls of such rows only (FINE) multiply by both values in one step. In the others the first tiles are streamed a second time, for
 // what rounding took: the same products in the same order, so the same bits, and the issuing warp need not know. (A question in each of its
-// steps made the windowed passes 5 to 7% slower, whatever the answer was.) 4096 tokens, 32 query and 8 key heads of 128, device time with the
-// first tiles streamed twice and once: window 1024 and 4 sinks, forward 88 and 84 us, backward 255 and 246; all earlier keys 136 and 133, 426 and 422.
+// steps made the windowed passes 5 to 7% slower, whatever the answer was.)
 // A window of 128 keys throughout as two values would take 55 instead of 47 us forward and 239 instead of 159 backward.
-constexpr int kFineSeq = 2 * kTile, kFineKeys = 64;  // kFineSeq: a pair of query tiles, so that a forward item is of one kind
+constexpr int kFineSeq = 2 * kTile, kFineKeys = 64;
+// So many of a sequence's first query tiles come a second time, where not all do in one step.
+template <bool FINE> __device__ __forceinline__ int secondTiles(int length) { return FINE ? 0 : length <= kFineSeq ? kFineSeq / kTile : 1; }
 
 template <int HD> struct FwdCfg {
   static constexpr int kMath = 16;                       // warps 0-7 and 8-15 are the two tiles' softmax
@@ -166,8 +168,8 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 
   // A pair of query tiles of one head and its key tiles.
   struct Item {
-    int h, b, kh, r0, L, count, nSinks, twice;  // twice: 1 where every tile comes a second time
-    bool two;
+    int h, b, kh, r0, L, count, nSinks, twice;  // twice: so many key tiles come twice, behind one another
+    bool two, one;                              // one: a second time for the first query tile only
     KeyRange own0, own1;
     __device__ Item(const FwdParams& p, uint32_t item) : own0(p.a, 0, 0), own1(p.a, 0, 0) {
       const Args& a = p.a;
@@ -177,21 +179,24 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       kh = h / a.group();
       r0 = (p.tiles - 1 - (int)(item / heads)) * 2 * kTile;  // the longest rows first
       L = lengthOf(a, b);
-      count = nSinks = 0;
+      count = nSinks = twice = 0;
       two = r0 + kTile < L;
-      twice = !FINE && r0 < kFineSeq;
+      one = secondTiles<FINE>(L) == 1;
       if (r0 >= L) return;
       own0 = KeyRange(a, r0, min(r0 + kTile, L) - 1);
       own1 = KeyRange(a, two ? r0 + kTile : r0, min(r0 + 2 * kTile, L) - 1);
       nSinks = min(own0.sinkTiles, own0.first);
-      count = (nSinks + own1.last - own0.first + 1) << twice;
+      twice = FINE || r0 ? 0 : one ? 1 : own1.last + 1;
+      count = nSinks + own1.last - own0.first + 1 + twice;
     }
     __device__ int tileOf(int n) const {
-      n >>= twice;
+      if constexpr (!FINE) n = n < 2 * twice ? n >> 1 : n - twice;
       return n < nSinks ? n : own0.first + n - nSinks;
     }
-    __device__ bool again(int n) const { return !FINE && (n & twice); }
-    __device__ bool active(int t, int n) const { return t == 0 ? own0.has(tileOf(n)) : two && own1.has(tileOf(n)); }
+    __device__ bool fine(int t) const { return FINE || (twice && !(t && one)); }
+    __device__ bool again(int n) const { return !FINE && n < 2 * twice && (n & 1); }
+    __device__ bool active(int t, int n) const { return t == 0 ? own0.has(tileOf(n)) : two && own1.has(tileOf(n)) && !(again(n) && one); }
+    __device__ bool last(int t, int n) const { return tileOf(n) == (t ? own1.last : own0.last) && (FINE || n >= 2 * twice || (n & 1) || (t && one)); }
     __device__ bool straddles(int n) const { return L - tileOf(n) * kTile < kTile; }
   };
 
@@ -259,7 +264,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
         const int slotV = after(slotK), slotNext = after(slotV);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const bool now = it.active(t, n), next = more && it.active(t, n + 1), last = it.tileOf(n) == (t ? it.own1.last : it.own0.last) && (FINE || (n & it.twice) == it.twice);
+          const bool now = it.active(t, n), next = more && it.active(t, n + 1), last = it.last(t, n);
           if (now) {
             if (!started[t]) {
               wait(&oFree[t], oTurn[t]);
@@ -358,7 +363,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
       bool any = false;
       for (int n = 0; n < it.count; n++) {
         const int tile = it.tileOf(n);
-        if (!own.has(tile)) continue;
+        if (!own.has(tile) || (t && it.again(n) && it.one)) continue;
         const int j0 = tile * kTile;
         const bool every = seesAll(a, rFirst, rLast, j0);
         if (!(ok = mbarWait(&sFull[t], sPhase, err, ERR_FWD_SOFTMAX))) break;
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
           }
         };
         // Masked scores have to become zeros, which the polynomial does not give.
-        if (!FINE && every && !it.twice) weights(std::true_type{}, std::false_type{});
+        if (!it.fine(t) && every) weights(std::true_type{}, std::false_type{});
         else if (!it.again(n)) weights(std::false_type{}, std::false_type{});
         else weights(std::false_type{}, std::true_type{});
         tmemStoreWait();
@@ -581,7 +586,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         sinkTiles = min(r.sinkTiles, r.first);
         yTiles = sinkTiles + r.last - r.first + 1;
         yh = xh / a.group();
-        count = x0 < L ? (!FINE && x0 < kFineSeq ? 2 * yTiles : yTiles) : 0;
+        count = x0 < L ? (xTile < secondTiles<FINE>(L) ? 2 * yTiles : yTiles) : 0;
       } else {
         xTile = turn < p.tiles ? turn : (turn - p.tiles) / p.farCount;
         if (turn >= p.tiles) far = (turn - p.tiles) % p.farCount;
@@ -598,17 +603,18 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         }
         if (x0 >= L || yTiles < 0) yTiles = 0;
         yh = xh * a.group();
-        count = (yTiles + (FINE ? 0 : max(0, min(kFineSeq / kTile, yFirst + yTiles) - yFirst))) * a.group();
+        count = (yTiles + max(0, min(secondTiles<FINE>(L), yFirst + yTiles) - yFirst)) * a.group();
         if (xTile < p.sinkTiles) partRows = min(kTile, a.sinks - x0);
       }
     }
     // The streamed tiles in their order; `again`: the second time, for what rounding took.
     __device__ int firstTile() const { return SIDE == kQueries && sinkTiles ? 0 : yFirst; }
     __device__ void next(int& tile, bool& again) const {
-      if constexpr (!FINE) {
-        again = !again && (SIDE == kQueries ? x0 : tile * kTile) < kFineSeq;
-        if (again) return;
+      if (!FINE && !again && (SIDE == kQueries ? xTile : tile) < secondTiles<FINE>(L)) {
+        again = true;
+        return;
       }
+      again = false;
       const int end = SIDE == kQueries ? sinkTiles : yFirst + yTiles;  // queries: from the sinks to the window; keys: to the next head's first
       tile = tile + 1 == end ? yFirst : tile + 1;
     }
@@ -941,12 +947,8 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
         }
       }
       const F2 c2 = makeF2(p.c, p.c), rowLse = makeF2(lse, lse), rowDelta = makeF2(-delta, -delta);
-      int tile = it.firstTile();
-      bool second = false;
-      for (int n = 0; n < it.count; n++, g++) {
-        const int y0 = tile * kTile;
-        const bool again = second;
-        it.next(tile, second);
+      const auto step = [&](int y0, auto rest) {  // rest: what rounding took
+        const bool again = rest;
         const bool every = !again && (SIDE == kQueries ? it.x0 + kTile <= it.L && seesAll(a, it.x0, it.x0 + kTile - 1, y0)
                                                        : y0 + kTile <= it.L && seesAll(a, y0, y0 + kTile - 1, it.x0));
         uint32_t bits[kCols / 32];
@@ -969,7 +971,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
           const uint32_t b = bits[e / 16] >> (2 * e % 32);
           return makeF2(b & 1 ? lo : 0.f, b & 2 ? hi : 0.f);
         };
-        if (!(ok = mbarWait(sFull, g & 1, err, ERR_BWD_MATH))) break;
+        if (!mbarWait(sFull, g & 1, err, ERR_BWD_MATH)) return false;
         tcFenceAfter();
         F2 w[kPairs];  // the weights
         {
@@ -1000,7 +1002,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
             tmemStore16(base + C::kS + cols + x * 16, o);
           }
         }
-        if (!(ok = mbarWait(dpFull, g & 1, err, ERR_BWD_MATH))) break;
+        if (!mbarWait(dpFull, g & 1, err, ERR_BWD_MATH)) return false;
         tcFenceAfter();
         {
           uint32_t d[kCols / 32][32];
@@ -1013,7 +1015,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
               uint32_t o[16];
 #pragma unroll
               for (int e = 0; e < 16; e++) o[e] = pack2(w[x * 16 + e]);
-              if (!FINE && again)
+              if (again)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[e] = pack2(remainder(w[x * 16 + e], o[e]));
               tmemStore16(base + C::kDp + cols + x * 16, o);
@@ -1049,14 +1051,24 @@ __global__ void __launch_bounds__(BwdCfg<HD, SIDE>::kThreads, 1) backwardKernel(
               if (SIDE == kKeys && y0 + cols + x * 32 == 0) bits[x] &= ~1u;
             }
           }
-          if (!FINE && again) gradients(std::false_type{}, std::true_type{});
-          else if (every) gradients(std::true_type{}, std::false_type{});
-          else gradients(std::false_type{}, std::false_type{});
+          if (every) gradients(std::true_type{}, std::false_type{});
+          else if (!again) gradients(std::false_type{}, std::false_type{});
+          else gradients(std::false_type{}, std::bool_constant<!FINE>{});
         }
         tmemStoreWait();
         tcFenceBefore();
         __syncwarp();
         if (lane == 0) mbarArrive(dsReady);
+        return true;
+      };
+      int tile = it.firstTile();
+      bool again = false;
+      for (int n = 0; n < it.count && ok; n++, g++) {
+        const int y0 = tile * kTile;
+        if constexpr (FINE) ok = step(y0, std::false_type{});
+        else if constexpr (SIDE == kQueries) ok = step(y0, again);
+        else ok = again ? step(y0, std::true_type{}) : step(y0, std::false_type{});
+        it.next(tile, again);
       }
       if (!ok || !(ok = mbarWait(done, donePhase, err, ERR_BWD_MATH))) break;
       donePhase ^= 1;

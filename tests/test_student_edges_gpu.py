@@ -62,16 +62,16 @@ def test_padding_changes_no_bit_of_a_sequence(D, window):
 @pytest.mark.parametrize("S, window, sinks", [(300, 0, 0), (700, 0, 0), (700, 200, 5), (1100, 70, 150)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_a_long_sequences_first_rows_are_as_exact_as_a_short_one(S, D, window, sinks):
-    """Their gradient is a difference of few weights. Answers and gradients of the first 256 rows do not depend on what follows; the keys' gradients do
-    not where the later rows' gradient is zero. So the bounds of a sequence of 256 tokens hold."""
+    """Their gradient is a difference of few weights. Answers and gradients of the first 128 rows do not depend on what follows; the keys' gradients do
+    not where the later rows' gradient is zero. So the bounds of a sequence of 128 tokens hold."""
     q, k, v, dout = _inputs(S + D, 2, 4, 2, S, D)
     q = q * 2
-    dout = torch.where(torch.arange(S, device="cuda").view(S, 1) < 256, dout, torch.zeros_like(dout))
+    dout = torch.where(torch.arange(S, device="cuda").view(S, 1) < 128, dout, torch.zeros_like(dout))
     got = _both_ways(q, k, v, dout, window, sinks)
-    ref = oracle.attention(*(t[:, :, :256] for t in (q, k, v)), window, sinks, None, 1 / math.sqrt(D), dout[:, :, :256])
+    ref = oracle.attention(*(t[:, :, :128] for t in (q, k, v)), window, sinks, None, 1 / math.sqrt(D), dout[:, :, :128])
     for n in NAMES:
-        oracle.off(n, got[n][:, :, :256], ref)
-    assert not got["dk"][:, :, 256:].any() and not got["dv"][:, :, 256:].any()
+        oracle.off(n, got[n][:, :, :128], ref)
+    assert not got["dk"][:, :, 128:].any() and not got["dv"][:, :, 128:].any()
 
 
 # ---- values that are not finite ---------------------------------------------------------------------------------------
