@@ -10,8 +10,9 @@
 // gradients) it keeps in registers, and goes from token to token. Forward, the rows of four heads per lane group are loaded together;
 // backward, where a row needs twice the registers, rows travel through shared memory, six tokens deep (a row at a time: 59 us).
 //
-// 4096 tokens, 32 + 8 + 8 heads of 128: forward 19 us for 84 MB (4.4 TB/s), backward 45 us for 142 MB (3.1 TB/s) and 5 for the weights' sums.
-// The backward pass is bound by its instructions (about 290 per pair of rows, issued in half of the cycles) rather than by memory.
+// 4096 tokens, 32 + 8 + 8 heads of 128: forward 20 us for 84 MB (4.2 TB/s), backward 47 us for 142 MB (3.0 TB/s) and 3 for the weights' sums; with
+// fp32 weights 23, 47 and 3. The backward pass fills neither memory nor the issue slots (half each; about 290 instructions per pair of rows):
+// with a quarter of an SM's warps, each waits for its token's row of the table.
 #include "rows.cuh"
 
 #include <type_traits>

@@ -9,9 +9,10 @@
 // The running maximum is moved, and O in tensor memory scaled down, only when a row's maximum has grown by more than 2^kSlack: weights stay
 // below 2^kSlack, which costs no precision in bf16 and fp32, and O is hardly ever touched in between.
 //
-// 4096 tokens, 32 query and 8 key heads of 128: 119 us for all earlier keys (137 GFLOP, 1.16 PFLOP/s), 83 for a window of 1024 with 4 sinks. It is
-// bound by the softmax: the tensor cores are busy for 48 to 59% of the time, the special-function pipe for 40, and instructions are issued
-// in half of the cycles; what is left over is waiting for one another, 100 to 200 cycles for each barrier that is already satisfied.
+// 4096 tokens, 32 query and 8 key heads of 128: 122 us for all earlier keys (137 GFLOP, 1.13 PFLOP/s), 85 for a window of 1024 with 4 sinks. No
+// unit is full: the tensor cores are busy for 47 to 57% of the time, the special-function pipe for 40, and instructions are issued in half of
+// the cycles. The softmax of a tile is the longest link; what is left over is waiting for one another, 100 to 200 cycles for each barrier
+// that is already satisfied.
 #pragma once
 
 #include <type_traits>
@@ -28,7 +29,7 @@ using namespace rows;
 constexpr int kTile = 128;  // queries and keys of a tile
 constexpr uint32_t kBox = kTile * 128;  // bytes of a TMA box: 128 rows of 64 elements
 constexpr float kSlack = 8.f;
-// Of a row's pairs of powers of two, one in so many is a polynomial (4096 tokens, 32 heads of 128, no window: 118 us; none 123, every other 125).
+// Of a row's pairs of powers of two, one in so many is a polynomial (4096 tokens, 32 heads of 128, no window: 124 us; none and every other 127, every fourth 124).
 constexpr int kPoly = 3;
 
 enum ErrCode : int { ERR_FWD_LOAD = 21, ERR_FWD_MMA, ERR_FWD_SOFTMAX, ERR_BWD_LOAD, ERR_BWD_MMA, ERR_BWD_MATH };
@@ -73,6 +74,7 @@ __device__ __forceinline__ bool seesAll(const Args& a, int r0, int rLast, int j0
 // Kernels for calls of such rows only (FINE) multiply by both values in one step. In the others the first tiles are streamed a second time, for
 // what rounding took: the same products in the same order, so the same bits, and the issuing warp need not know. (A question in each of its
 // steps made the windowed passes 5 to 7% slower, whatever the answer was.)
+// The second time takes 339 instead of 329 us of a window of 1024 with 4 sinks over 4096 tokens both ways, and 552 instead of 548 of all earlier keys.
 // A window of 128 keys throughout as two values would take 55 instead of 47 us forward and 239 instead of 159 backward.
 constexpr int kFineSeq = 2 * kTile, kFineKeys = 64;
 // So many of a sequence's first query tiles come a second time, where not all do in one step.
@@ -510,9 +512,9 @@ __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1) forwardKernel(const _
 // Keys that every later query sees (sinks) would keep their CTAs far longer than the others: the queries behind the window are split over
 // further items, whose fp32 sums joinSinks adds up in a fixed order.
 //
-// 4096 tokens, 32 query and 8 key heads of 128: queries 185 us, keys 219 for all earlier keys (344 GFLOP, and 137 more as both make S and dP), 119
-// and 144 for a window of 1024 with 4 sinks, whose partial sums take 5 more. Tensor cores are busy for 62 and 77% (48 and 69%) of that time; the
-// rest is the chain of a tile (scores, weights, gradients of scores, products), which only one tile of look-ahead covers.
+// 4096 tokens, 32 query and 8 key heads of 128: 390 us for all earlier keys (344 GFLOP, and 137 more as both make S and dP), 256 for a window of 1024
+// with 4 sinks (queries 116, keys 134, partial sums 3). Tensor cores are busy for 60 and 77% (48 and 68%) of that time; the rest is the chain of
+// a tile (scores, weights, gradients of scores, products), which only one tile of look-ahead covers.
 enum Side { kQueries, kKeys };
 
 struct BwdParams {

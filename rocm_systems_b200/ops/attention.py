@@ -3,7 +3,8 @@
 
 bf16 tensors, fp32 arithmetic, forward and backward. The calls enqueue on the current stream of the tensors' device and return at once (the
 first one on a device allocates an error word and should come before any stream capture);
-:func:`rocm_systems_b200.ops.train_ops.gemm_take_error` reports a kernel that gave up a wait."""
+:func:`rocm_systems_b200.ops.train_ops.gemm_take_error` reports a kernel that gave up a wait. Gradients of gradients and forward-mode
+derivatives are refused."""
 from __future__ import annotations
 
 from typing import Optional, Tuple
@@ -53,5 +54,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     to 128, any strides (rows that are not dense or not on 16 bytes are copied). ``window`` 0: every earlier key. ``scale``: 1 / sqrt(D) by
     default. ``lengths`` int32 [B] on the device: the sequences' lengths in a batch padded to S (0 to S; other values are taken as the nearest
     of these); what lies behind a sequence's end is not used, answers zeros and gets zero gradients. Returns [B, H, S, D] whose memory is
-    [B, S, H, D]. Results and gradients do not depend on the order in which anything runs."""
+    [B, S, H, D]. Results and gradients do not depend on the order in which anything runs.
+
+    The softmax's weights enter the products as bf16 values, of sequences of at most 256 tokens, the first 128 tokens of longer ones and windows (with
+    sinks) of at most 64 keys as the sum of two. That hangs on a sequence's own length: padding does not change its results (with sinks,
+    the rounding of their gradients' partial sums). For the backward pass a call keeps a second tensor of the answer's size, what rounding
+    took from it."""
     return _ext().window_attention(q, k, v, window, sinks, lengths, scale)

@@ -189,9 +189,10 @@ def distill_loss(logits: torch.Tensor, targets: torch.Tensor, teacher_ids: torch
     ``loss = (1 - weight) * cross_entropy(z, target) + weight * t^2 * KL(softmax(teacher_logits / t) || softmax(z / t))`` with the temperature
     ``t`` from 0.01 to 100; the first softmax runs over the row's stored entries, the second over the whole vocabulary. ``logits`` [T, V] bf16 with dense rows;
     V at most 851,968; ``targets`` int64 [T]; ``teacher_ids`` [T, K] int64 or int32, ``teacher_logits`` [T, K] fp32 or bf16, K at most 1024, in
-    any order. Entries of one id add up; an entry whose id is outside [0, V) counts nothing, and a row without entries has no second term. A
+    any order (the time grows with K's square: 1024 rows of 128256 take 0.14 ms with 64 entries and 3.2 ms with 1024). Entries of one id add up;
+    an entry whose id is outside [0, V), or whose logit is minus infinity, counts nothing, and a row without entries has no second term. A
     row whose target is outside [0, V) (padding) has zero loss and zero gradient. The gradient, times ``grad_scale``, goes to ``grad``
-    (``logits`` itself: in place), by default a new tensor."""
+    (``logits`` itself: in place, which autograd sees as a write), by default a new tensor. The loss records no graph."""
     from .attention import _ext  # this module is the first to be loaded
 
     return _ext().distill_loss(logits, targets, teacher_ids, teacher_logits, weight, temperature, grad_scale, grad)
