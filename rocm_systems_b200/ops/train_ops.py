@@ -187,8 +187,8 @@ def distill_loss(logits: torch.Tensor, targets: torch.Tensor, teacher_ids: torch
     """Cross-entropy mixed with the divergence from a teacher's top logits: the loss per row (fp32 [T]) and its gradient (bf16, like ``logits``).
 
     ``loss = (1 - weight) * cross_entropy(z, target) + weight * t^2 * KL(softmax(teacher_logits / t) || softmax(z / t))`` with the temperature
-    ``t`` from 0.01 to 100; the first softmax runs over the row's stored entries, the second over the whole vocabulary. ``logits`` [T, V] bf16 with dense rows;
-    V at most 851,968; ``targets`` int64 [T]; ``teacher_ids`` [T, K] int64 or int32, ``teacher_logits`` [T, K] fp32 or bf16, K at most 1024, in
+    ``t`` from 0.01 to 100; the first softmax runs over the row's stored entries, the second over the whole vocabulary. ``logits`` [T, V] bf16 with dense rows,
+    of magnitudes up to 1e8 (1e8 ``t`` where ``t`` is below one), V at most 851,968; ``targets`` int64 [T]; ``teacher_ids`` [T, K] int64 or int32, ``teacher_logits`` [T, K] fp32 or bf16, K at most 1024, in
     any order (the time grows with K's square: 1024 rows of 128256 take 0.14 ms with 64 entries and 3.2 ms with 1024). Entries of one id add up;
     an entry whose id is outside [0, V), or whose logit is minus infinity, counts nothing, and a row without entries has no second term. A
     row whose target is outside [0, V) (padding) has zero loss and zero gradient. The gradient, times ``grad_scale``, goes to ``grad``

@@ -396,3 +396,30 @@ def test_a_sequences_first_row_sees_one_key(S, window, sinks):
     assert not got["dq"].any() and not got["dk"].any()
     q[0, 0, 0, 0] = math.nan
     assert bool(torch.isnan(_both_ways(q, k, v, first, window, sinks)["dq"][0, 0, 0]).all())
+
+
+@pytest.mark.parametrize("weight, tau", [(0.0, 1.0), (1.0, 1.0), (1.0, 0.01), (1.0, 100.0), (0.5, 1.0), (0.5, 2.0), (0.5, 3.0), (0.5, 4.0), (0.5, 2.5), (0.5, 0.1)])
+@pytest.mark.parametrize("V", [500, 40000])
+def test_distill_loss_logits_up_to_a_hundred_million_temperatures(V, weight, tau):
+    """Two equal logits far above all others: a half each. The rounding of so large an offset is a factor of up to 16 of every power; it is taken out."""
+    from rocm_systems_b200.ops import train_ops
+
+    tops = (torch.logspace(1, 8, 300, device="cuda") * min(tau, 1.0)).clamp(min=3000 * max(tau, 1.0)).to(bf)
+    T = tops.numel()
+    g = _gen(V)
+    for sign in (1, -1):  # the others at zero, or the two at zero and the others far below
+        logits = torch.zeros(T, V, dtype=bf, device="cuda")
+        tgt = torch.randint(0, V // 2, (T,), device="cuda", generator=g)
+        two = torch.stack([tgt, tgt + V // 2], 1)  # in two slices where there are several
+        if sign > 0:
+            logits.scatter_(1, two, tops[:, None].expand(T, 2).contiguous())
+        else:
+            logits[:] = -tops[:, None]
+            logits.scatter_(1, two, 0)
+        loss, grad = train_ops.distill_loss(logits, tgt, tgt[:, None].contiguous(), torch.zeros(T, 1, device="cuda"), weight, tau)
+        want = (1 - weight + weight * tau ** 2) * math.log(2)
+        # as for small losses, and the rounding of the loss
+        assert float((loss.double() - want).abs().max()) <= (1 - weight + weight * tau ** 2) * (2.0 ** -20 + (V / 128 + 16) * 2.0 ** -24 + 2.0 ** -22)
+        dense = torch.zeros(T, V, dtype=torch.float64, device="cuda")
+        dense.scatter_(1, two, (1 - weight + weight * tau) * torch.tensor([[-0.5, 0.5]], dtype=torch.float64, device="cuda").expand(T, 2).contiguous())
+        assert float((grad.double() - dense).abs().max()) <= (1 - weight + weight * tau) * (0.5 * 2.0 ** -8 + 2.0 ** -18)
